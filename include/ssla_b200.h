@@ -124,6 +124,38 @@ int ssla_chunk_gla_fwd_noalloc(const void* q, const void* k, const void* v, cons
                                int64_t T, int64_t H, int64_t K, int64_t V, float scale,
                                const float* h0, void* o, float* ht, ssla_stream_t stream);
 
+/* ------------------------------------------------------------------ gated delta rule
+ * Per value head, with state S [K,V]:
+ *   S <- exp(g_t) S;  u_t = beta_t (v_t - S^T k_t);  S <- S + k_t u_t^T;  o_t = scale S^T q_t.
+ * No counterpart in the reference; layout and conventions of chunk_gla above.
+ * q,k,dq,dk [T,H,K]; v,o,do,dv [T,HV,V], HV a multiple of H (value head hv reads key head
+ * hv / (HV / H)); g,dg,beta,dbeta [T,HV] in dtype_g / dtype_beta (any of the three types);
+ * h0,ht,dht,dh0 [N,HV,K,V] fp32 (nullable).  1 <= K <= 128, 1 <= V <= 256.  Tokens outside every
+ * sequence get zero outputs and gradients.  g below -200 (-inf included) acts as -200: its decay
+ * is 0 in fp32 either way.
+ * The chunked forward fills `states` (ssla_gated_delta_rule_states_bytes) for the backward; both
+ * take scratch of ssla_gated_delta_rule_workspace_bytes (backward = 0 / 1).  states and workspace
+ * are 16-byte aligned. */
+size_t ssla_gated_delta_rule_states_bytes(int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V);
+size_t ssla_gated_delta_rule_workspace_bytes(int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
+                                             int backward);
+int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                                    int dtype, int dtype_g, int dtype_beta, const int64_t* cu_seqlens, int64_t n_seqs,
+                                    int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, float scale,
+                                    const float* h0, void* o, float* ht, void* states, size_t states_bytes,
+                                    void* workspace, size_t workspace_bytes, ssla_stream_t stream);
+int ssla_chunk_gated_delta_rule_bwd(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                                    int dtype, int dtype_g, int dtype_beta, const int64_t* cu_seqlens, int64_t n_seqs,
+                                    int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, float scale,
+                                    const void* states, size_t states_bytes, const void* dout, const float* dht,
+                                    void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dh0, void* workspace,
+                                    size_t workspace_bytes, ssla_stream_t stream);
+/* The same forward token by token (streaming, serving): the state stays in registers. */
+int ssla_recurrent_gated_delta_rule_fwd(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                                        int dtype, int dtype_g, int dtype_beta, const int64_t* cu_seqlens,
+                                        int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
+                                        float scale, const float* h0, void* o, float* ht, ssla_stream_t stream);
+
 /* ------------------------------------------------------------------ pixel grouping
  * group_events (utils/farsecnn_utils.py:130-174, utils/async_utils.py:10-84) followed, with
  * keep_first, by the hot-pixel truncation of model_mos.py:173-209: events [B,Nmax,C] fp32 rows

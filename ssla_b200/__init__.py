@@ -5,7 +5,8 @@ Import paths mirror the reference project (``ops.gla.chunk``, ``ops.common.scan`
 ``layers.mos_attention`` ...) under the ``ssla_b200`` package.
 """
 
-__all__ = ["chunk_gla", "fused_recurrent_gla", "chunk_gla_scalar", "scan"]
+__all__ = ["chunk_gla", "fused_recurrent_gla", "chunk_gla_scalar", "scan", "chunk_gated_delta_rule",
+           "fused_recurrent_gated_delta_rule"]
 
 
 def __getattr__(name):
@@ -21,4 +22,7 @@ def __getattr__(name):
     if name == "scan":
         from .ops.common.scan import scan
         return scan
+    if name in ("chunk_gated_delta_rule", "fused_recurrent_gated_delta_rule"):
+        from .ops import gated_delta_rule
+        return getattr(gated_delta_rule, name)
     raise AttributeError(name)

@@ -1,0 +1,325 @@
+// Shared definitions of the gated delta rule (chunked forward + backward).
+//
+// Per value head, with state S [K, V]:
+//   S <- exp(g_t) S;  u_t = beta_t (v_t - S^T k_t);  S <- S + k_t u_t^T;  o_t = scale S^T q_t
+//
+// Over a chunk of 64 tokens (gc = inclusive sum of g inside the chunk, G_ij = exp(gc_i - gc_j) for
+// i >= j, S the state at the chunk's start, gC the chunk's whole sum):
+//   T  = (I + A)^-1,  A_ij = beta_i G_ij k_i.k_j for i > j
+//   U  = T beta (V - exp(gc) K S)                       (the u_t of the chunk)
+//   O  = scale (exp(gc) Q S + (G o Q K^T) U)
+//   S' = exp(gC) S + Kl^T U,                            Kl_j = exp(gC - gc_j) k_j
+// With W = T beta exp(gc) K the chunk acts on its start state as an affine map,
+//   S' = exp(gC) S - (Kl^T W) S + Kl^T (T beta V)  =  exp(gC) S - PM S + B,
+// and its adjoint is dS = exp(gC) dS' - PM^T dS' + dB, so that everything but one [K,K] x [K,V]
+// product per chunk runs in parallel over chunks.  All exponents are differences i >= j of the
+// in-chunk sums (never positive for g <= 0), formed from sums held as two floats.
+#pragma once
+#include "common.cuh"
+#include "vec.cuh"
+
+namespace ssla {
+namespace delta {
+
+constexpr int BT = 64;            // tokens per chunk
+constexpr int LDC = BT + 4;       // row of a [64, 64] fp32 tile in shared memory
+constexpr int THREADS = 256;      // threads of the per-chunk kernels
+constexpr float kMinGate = -200.f;  // exp() of less is 0 in fp32; keeps in-chunk sums finite for g = -inf
+
+inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+inline int64_t max_chunks(int64_t N, int64_t T) { return (T + (BT - 1) * N) / BT; }
+inline int pad_k(int64_t K) { return K <= 64 ? 64 : 128; }
+inline int pad_v(int64_t V) { return (int)((V + 63) / 64 * 64); }
+
+// Segments: runs of `len` chunks of one sequence whose maps are composed first when there are too
+// few (sequence, head, column) chains to fill the GPU; len = 0 leaves sequences whole.
+struct Plan {
+  int64_t MC;    // upper bound of chunks
+  int64_t len;   // chunks per segment (0: no segments)
+  int64_t MS;    // upper bound of segments
+  int vs;        // state columns per chain
+  int vs_seg;    // the same inside segments
+};
+Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V);
+
+// What the forward leaves for the backward (caller's `states` buffer), all padded to KP x VP:
+//   chunk_off [N+1], seg_off [N+1] (device), chunk_tab [MC] {first token, rows | seq << 32},
+//   seg_tab [MS] {first chunk, chunks, seq}; per (chunk, value head) item: decay = exp(gC),
+//   tinv [64,64] = T, pm [KP,KP] and s [KP,VP] = state at the chunk's start (B before the scan).
+struct Saved {
+  int* chunk_off;
+  int* seg_off;
+  longlong2* chunk_tab;
+  int4* seg_tab;
+  float* decay;
+  float* tinv;
+  float* pm;
+  float* s;
+};
+
+inline size_t saved_layout(void* base, const Plan& p, int64_t N, int64_t HV, int KP, int VP, Saved* out) {
+  char* q = (char*)base;
+  const size_t items = (size_t)p.MC * HV;
+  auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
+  Saved s;
+  s.chunk_off = (int*)take(4 * (N + 1));
+  s.seg_off = (int*)take(4 * (N + 1));
+  s.chunk_tab = (longlong2*)take(16 * (size_t)p.MC);
+  s.seg_tab = (int4*)take(16 * (size_t)p.MS);
+  s.decay = (float*)take(4 * items);
+  s.tinv = (float*)take(4 * items * BT * BT);
+  s.pm = (float*)take(4 * items * KP * KP);
+  s.s = (float*)take(4 * items * KP * VP);
+  if (out) *out = s;
+  return (size_t)(q - (char*)base);
+}
+
+// Scratch of one call: the composed maps of the segments; the backward's adjoint states and, when
+// value heads share key heads, fp32 dq and dk of every value head.
+struct Work {
+  float* mseg;  // [MS*HV, KP, KP]
+  float* bseg;  // [MS*HV, KP, VP]
+  float* ds;    // [MC*HV, KP, VP]
+  float* dqk;   // [2, T, HV, K]
+};
+
+inline size_t work_layout(void* base, const Plan& p, int64_t T, int64_t H, int64_t HV, int64_t K, int KP, int VP,
+                          bool bwd, Work* out) {
+  char* q = (char*)base;
+  auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
+  Work w;
+  const size_t segs = p.len ? (size_t)p.MS * HV : 0;
+  w.mseg = (float*)take(4 * segs * KP * KP);
+  w.bseg = (float*)take(4 * segs * KP * VP);
+  w.ds = (float*)take(bwd ? 4 * (size_t)p.MC * HV * KP * VP : 0);
+  w.dqk = (float*)take(bwd && HV != H ? 8 * (size_t)T * HV * K : 0);
+  if (out) *out = w;
+  return (size_t)(q - (char*)base);
+}
+
+// One call's tensors and sizes (device pointers), shared by the kernels.
+struct Args {
+  const void *q, *k, *v, *g, *beta;
+  int dt_g, dt_b;
+  const int64_t* cu;
+  int64_t N, T, MC;
+  int H, HV, R, K, V;  // R = HV / H value heads per key head
+  float scale;
+  bool vec_k, vec_v;  // rows of q/k, v can be copied 16 bytes at a time
+};
+
+__device__ __forceinline__ float ld_any(const void* p, int dt, size_t i) {
+  if (dt == SSLA_F32) return ((const float*)p)[i];
+  if (dt == SSLA_BF16) return __bfloat162float(((const __nv_bfloat16*)p)[i]);
+  return __half2float(((const __half*)p)[i]);
+}
+__device__ __forceinline__ void st_any(void* p, int dt, size_t i, float x) {
+  if (dt == SSLA_F32) ((float*)p)[i] = x;
+  else if (dt == SSLA_BF16) ((__nv_bfloat16*)p)[i] = __float2bfloat16_rn(x);
+  else ((__half*)p)[i] = __float2half_rn(x);
+}
+
+// ------------------------------------------------------------------ tensor-core products
+// Warp-level C += A B on mma.sync m16n8k8 TF32 with fp32 accumulators.  The operands are read
+// through functors fa(row, k), fb(k, col) from shared memory.  A value that came from a 16-bit
+// input is exact in TF32 (AX, BX).  SPLIT: x = hi + lo with hi the TF32 rounding, products
+// hi hi + lo hi + hi lo, about 2^-22 relative; otherwise one product of TF32-rounded operands.
+__device__ __forceinline__ uint32_t tf32_rna(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+
+template <bool EXACT, bool SPLIT>
+__device__ __forceinline__ void operand(float x, uint32_t& hi, uint32_t& lo) {
+  if (EXACT) {
+    hi = __float_as_uint(x);
+  } else {
+    hi = tf32_rna(x);
+    if (SPLIT) lo = __float_as_uint(x - __uint_as_float(hi));
+  }
+}
+
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+template <bool AX, bool BX, bool SPLIT, int MT, int NT, class FA, class FB>
+__device__ __forceinline__ void warp_mma(float (&acc)[MT][NT][4], int m0, int n0, int k0, int k1, FA fa, FB fb) {
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  for (int k = k0; k < k1; k += 8) {
+    uint32_t ah[MT][4], al[MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      operand<AX, SPLIT>(fa(m0 + 16 * i + g, k + t), ah[i][0], al[i][0]);
+      operand<AX, SPLIT>(fa(m0 + 16 * i + g + 8, k + t), ah[i][1], al[i][1]);
+      operand<AX, SPLIT>(fa(m0 + 16 * i + g, k + t + 4), ah[i][2], al[i][2]);
+      operand<AX, SPLIT>(fa(m0 + 16 * i + g + 8, k + t + 4), ah[i][3], al[i][3]);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      uint32_t bh[2], bl[2];
+      operand<BX, SPLIT>(fb(k + t, n0 + 8 * j + g), bh[0], bl[0]);
+      operand<BX, SPLIT>(fb(k + t + 4, n0 + 8 * j + g), bh[1], bl[1]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        mma8(acc[i][j], ah[i], bh);
+        if (SPLIT && !AX) mma8(acc[i][j], al[i], bh);
+        if (SPLIT && !BX) mma8(acc[i][j], ah[i], bl);
+      }
+    }
+  }
+}
+
+template <int MT, int NT> __device__ __forceinline__ void zero(float (&acc)[MT][NT][4]) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = 0.f;
+}
+
+// f(row, col, value0, value1) for the accumulator's pairs (row, col), (row, col + 1)
+template <int MT, int NT, class F>
+__device__ __forceinline__ void each_pair(float (&acc)[MT][NT][4], int m0, int n0, F f) {
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      f(m0 + 16 * i + g, n0 + 8 * j + 2 * t, acc[i][j][0], acc[i][j][1]);
+      f(m0 + 16 * i + g + 8, n0 + 8 * j + 2 * t, acc[i][j][2], acc[i][j][3]);
+    }
+}
+
+// ------------------------------------------------------------------ copies into shared memory
+__device__ __forceinline__ void cp16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// dst[64][LD] (COLS used) = rows of src; zeros behind `rows` and `cols`.  Asynchronous when vec.
+template <class TI, int LD, int COLS>
+__device__ __forceinline__ void load_rows(TI* dst, const TI* src, size_t stride, int rows, int cols, bool vec) {
+  constexpr int E = 16 / sizeof(TI), PR = COLS / E;
+  if (vec) {
+    for (int i = threadIdx.x; i < BT * PR; i += THREADS) {
+      const int r = i / PR, c = (i - r * PR) * E;
+      if (r < rows && c < cols) cp16(dst + r * LD + c, src + r * stride + c);
+      else *reinterpret_cast<uint4*>(dst + r * LD + c) = make_uint4(0, 0, 0, 0);
+    }
+  } else {
+    for (int i = threadIdx.x; i < BT * COLS; i += THREADS) {
+      const int r = i / COLS, c = i - r * COLS;
+      TI x = TI(0.f);
+      if (r < rows && c < cols) x = src[r * stride + c];
+      dst[r * LD + c] = x;
+    }
+  }
+}
+
+// dst[ROWS][LD] = COLS columns of the fp32 matrix src (row length `stride`), 16-byte copies
+template <int LD, int ROWS, int COLS>
+__device__ __forceinline__ void load_f32(float* dst, const float* src, int stride) {
+  constexpr int PR = COLS / 4;
+  for (int i = threadIdx.x; i < ROWS * PR; i += THREADS) {
+    const int r = i / PR, c = (i - r * PR) * 4;
+    cp16(dst + r * LD + c, src + (size_t)r * stride + c);
+  }
+}
+
+// ------------------------------------------------------------------ gates of one chunk
+struct Gates {
+  float hi[BT], lo[BT];  // in-chunk sums gc (two floats)
+  float beta[BT];
+  float start[BT];       // exp(gc)
+  float left[BT];        // exp(gC - gc)
+  float whole;           // exp(gC)
+  // exp(gc_i - gc_j), i >= j
+  __device__ __forceinline__ float fade(int i, int j) const { return expf((hi[i] - hi[j]) + (lo[i] - lo[j])); }
+};
+
+// One warp.  g below kMinGate counts as kMinGate (both decay to 0), NaN stays.
+__device__ __forceinline__ void load_gates(Gates& s, const Args& a, int64_t t0, int rows, int hv) {
+  const int lane = threadIdx.x & 31;
+  double x[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 2 * lane + i;
+    float g = 0.f, b = 0.f;
+    if (r < rows) {
+      const size_t at = (size_t)(t0 + r) * a.HV + hv;
+      g = ld_any(a.g, a.dt_g, at);
+      b = ld_any(a.beta, a.dt_b, at);
+      g = g < kMinGate ? kMinGate : g;
+    }
+    s.beta[r] = b;
+    x[i] = g;
+  }
+  double sum = x[0] + x[1];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += y;
+  }
+  const double all = __shfl_sync(0xffffffffu, sum, 31);
+  const double c[2] = {sum - x[1], sum};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 2 * lane + i;
+    s.hi[r] = (float)c[i];
+    s.lo[r] = (float)(c[i] - (double)s.hi[r]);
+    const float e = expf(s.hi[r]);
+    s.start[r] = fmaf(e, s.lo[r], e);
+    s.left[r] = expf((float)(all - c[i]));
+  }
+  if (lane == 0) s.whole = expf((float)all);
+}
+
+template <class TI> struct Io16 { static constexpr bool exact = true; };
+template <> struct Io16<float> { static constexpr bool exact = false; };
+// Products whose results leave in bf16 only need less than bf16's own rounding (2^-8): one TF32
+// product (2^-11 per operand).  fp16 and fp32 results need the split.
+template <class TI> struct OutSplit { static constexpr bool v = true; };
+template <> struct OutSplit<__nv_bfloat16> { static constexpr bool v = false; };
+
+template <class TI, int KP> struct KTile { static constexpr int LD = KP + (sizeof(TI) == 4 ? 4 : 8); };
+
+__device__ __forceinline__ bool locate(const longlong2* tab, int64_t MC, int64_t chunk, int64_t& t0, int& rows) {
+  if (chunk >= MC) return false;
+  const longlong2 e = tab[chunk];
+  t0 = e.x;
+  rows = (int)(e.y & 0xffffffff);
+  return e.y >= 0;
+}
+
+// Rows of [T, n] outside every sequence become 0 (all CTAs share the work).
+template <class TO>
+__device__ __forceinline__ void zero_uncovered(TO* out, const Args& a, int64_t n) {
+  int64_t b = a.cu[0], e = a.cu[a.N];
+  b = b < 0 ? 0 : (b > a.T ? a.T : b);
+  e = e < b ? b : (e > a.T ? a.T : e);
+  const int64_t head = b * n, total = head + (a.T - e) * n;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x)
+    out[i < head ? i : e * n + (i - head)] = TO(0.f);
+}
+
+// delta_rule.cu
+int check_args(const char* name, int dtype, int dtype_g, int dtype_b, int64_t N, int64_t T, int64_t H, int64_t HV,
+               int64_t K, int64_t V);
+Args make_args(const void* q, const void* k, const void* v, const void* g, const void* beta, int dtype, int dtype_g,
+               int dtype_b, const int64_t* cu, int64_t N, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
+               float scale);
+// The affine chunk maps along every sequence: forward S' = decay S - PM S + B (s: B in, start states
+// out), reverse the adjoint with PM^T (s: dB in, adjoint of every chunk's end state out).
+int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const float* init, float* last, int64_t N,
+              int HV, int K, int V, bool reverse, cudaStream_t st);
+
+}  // namespace delta
+}  // namespace ssla

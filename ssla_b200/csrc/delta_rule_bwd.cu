@@ -1,0 +1,489 @@
+// Chunked gated delta rule, backward.  With P = G o Q K^T (lower), S the state at a chunk's start,
+// D the adjoint of the state at its end, X = V - exp(gc) K S, U = T beta X:
+//   adjoint of the chunk map   dB = scale qh^T dO,  qh = exp(gc) Q - P W,  W = T beta exp(gc) K
+//   dU = scale P^T dO + Kl D;  F = T^T dU;  dV = beta F
+//   dP = scale (dO U^T) o G (lower),  E = (F U^T) o G (strictly lower)
+//   dQ = scale exp(gc) dO S^T + dP K
+//   dK = [-beta exp(gc) F S^T - beta E K] + [exp(gC - gc) U D^T + dP^T Q - E^T beta K]
+//   dbeta_i = F_i . X_i - k_i . (E K)_i
+// The first bracket of dK is K's part as the row (later) index of the scores, the second as the
+// column; every decay exp(gc_i - gc_j) pairs a row with a column, so that
+//   dgc_i = q_i . dq_i + k_i . dk_i[row] - k_i . dk_i[column]
+// plus, at the chunk's last token, sum_j k_j . (exp(gC - gc) U D^T)_j + exp(gC) <S, D>.
+#include "delta_rule.cuh"
+
+namespace ssla {
+namespace delta {
+namespace {
+
+template <class TI, int KP> struct AdjSmem {
+  static constexpr int LDK = KTile<TI, KP>::LD, LDW = KP + 8, LDO = 72;
+  TI k[BT * LDK];
+  TI q[BT * LDK];
+  TI d[BT * LDO];
+  float p[BT * LDC];
+  float t[BT * LDC];
+  float w[BT * LDW];
+  Gates gates;
+};
+
+// dB of every (chunk, value head) into ds.
+template <class TI, int KP, bool SP>
+__global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<TI, KP>) <= 113 * 1024 ? 2 : 1)
+    adjoint_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
+                   const TI* __restrict__ dout, float* __restrict__ ds) {
+  using S = AdjSmem<TI, KP>;
+  constexpr bool X = Io16<TI>::exact;
+  constexpr int LDK = S::LDK, LDW = S::LDW, LDO = S::LDO, NK = KP / 16;
+  extern __shared__ __align__(16) unsigned char raw[];
+  S& s = *reinterpret_cast<S*>(raw);
+  const int64_t chunk = blockIdx.x / a.HV;
+  const int hv = (int)(blockIdx.x - chunk * a.HV), h = hv / a.R;
+  const size_t item = blockIdx.x;
+  int64_t t0;
+  int rows;
+  if (!locate(tab, a.MC, chunk, t0, rows)) return;
+  const int warp = threadIdx.x >> 5;
+  const size_t qk = ((size_t)t0 * a.H + h) * a.K;
+  load_rows<TI, LDK, KP>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  load_rows<TI, LDK, KP>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  load_f32<LDC, BT, BT>(s.t, tinv + item * (BT * BT), BT);
+  const size_t vo = ((size_t)t0 * a.HV + hv) * a.V;
+  const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
+  load_rows<TI, LDO, 64>(s.d, dout + vo, (size_t)a.HV * a.V, rows, a.V, vec_d);
+  cp_commit();
+  if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
+  cp_wait<0>();
+  __syncthreads();
+  const TI *sk = s.k, *sq = s.q;
+  const int m0 = (warp >> 1) * 16, n0 = (warp & 1) * 32, k0 = (warp & 1) * (KP / 2);
+  {
+    float acc[1][4][4];
+    zero(acc);
+    if (n0 <= m0)
+      warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return ldf(sq + m * LDK + k); },
+                         [&](int k, int n) { return ldf(sk + n * LDK + k); });
+    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
+      s.p[i * LDC + j] = i >= j ? s.gates.fade(i, j) * x : 0.f;
+      s.p[i * LDC + j + 1] = i > j ? s.gates.fade(i, j + 1) * y : 0.f;
+    });
+  }
+  float acc[1][NK][4];
+  zero(acc);
+  warp_mma<false, X, SP>(acc, m0, k0, 0, m0 + 16,
+                         [&](int i, int j) { return s.t[i * LDC + j] * (s.gates.beta[j] * s.gates.start[j]); },
+                         [&](int j, int n) { return ldf(sk + j * LDK + n); });
+  each_pair(acc, m0, k0, [&](int i, int n, float x, float y) {
+    *reinterpret_cast<float2*>(s.w + i * LDW + n) = make_float2(x, y);
+  });
+  __syncthreads();
+  zero(acc);
+  warp_mma<false, false, SP>(acc, m0, k0, 0, m0 + 16, [&](int i, int j) { return s.p[i * LDC + j]; },
+                             [&](int j, int n) { return s.w[j * LDW + n]; });
+  __syncthreads();
+  each_pair(acc, m0, k0, [&](int i, int n, float x, float y) {
+    const float e = s.gates.start[i];
+    *reinterpret_cast<float2*>(s.w + i * LDW + n) =
+        make_float2(a.scale * (e * ldf(sq + i * LDK + n) - x), a.scale * (e * ldf(sq + i * LDK + n + 1) - y));
+  });
+  constexpr int MT = KP / 64;
+  const int mk = (warp >> 1) * 16 * MT;
+  for (int v0 = 0; v0 < VP; v0 += 64) {
+    if (v0) {
+      __syncthreads();
+      load_rows<TI, LDO, 64>(s.d, dout + vo + v0, (size_t)a.HV * a.V, rows, a.V - v0, vec_d);
+      cp_commit();
+      cp_wait<0>();
+    }
+    __syncthreads();
+    float db[MT][4][4];
+    zero(db);
+    warp_mma<false, X, SP>(db, mk, n0, 0, BT, [&](int m, int j) { return s.w[j * LDW + m]; },
+                           [&](int j, int n) { return ldf(s.d + j * LDO + n); });
+    each_pair(db, mk, n0, [&](int m, int n, float x, float y) {
+      *reinterpret_cast<float2*>(ds + (item * KP + m) * VP + v0 + n) = make_float2(x, y);
+    });
+  }
+}
+
+template <class TI, int KP> struct BwdSmem {
+  static constexpr int VB = 32, LDK = KTile<TI, KP>::LD, LDO = VB + (sizeof(TI) == 4 ? 4 : 8), LDX = VB + 4;
+  TI k[BT * LDK];
+  TI q[BT * LDK];
+  TI d[BT * LDO];
+  float p[BT * LDC];  // P, then dP
+  float t[BT * LDC];  // T, then E
+  float x[BT * LDX];  // beta X, then U
+  float f[BT * LDX];  // dU, then F
+  float s[KP * LDX];
+  float e[KP * LDX];  // D
+  float red[6][2][BT];
+  float dots[THREADS / 32];
+  Gates gates;
+};
+
+template <class TI, int KP>
+__global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024 ? 2 : 1)
+    backward_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
+                    const float* __restrict__ states, const float* __restrict__ ds, const TI* __restrict__ dout,
+                    TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv, void* __restrict__ dg,
+                    void* __restrict__ dbeta, float* __restrict__ dqk) {
+  using S = BwdSmem<TI, KP>;
+  constexpr bool X = Io16<TI>::exact, SP = OutSplit<TI>::v;
+  constexpr int VB = S::VB, LDK = S::LDK, LDO = S::LDO, LDX = S::LDX, NT = VB / 16, NK = KP / 16;
+  extern __shared__ __align__(16) unsigned char raw[];
+  S& s = *reinterpret_cast<S*>(raw);
+  const size_t TK = (size_t)a.T * a.HV * a.K;
+  if (dqk) {
+    zero_uncovered(dqk, a, (int64_t)a.HV * a.K);
+    zero_uncovered(dqk + TK, a, (int64_t)a.HV * a.K);
+  } else {
+    zero_uncovered(dq, a, (int64_t)a.H * a.K);
+    zero_uncovered(dk, a, (int64_t)a.H * a.K);
+  }
+  zero_uncovered(dv, a, (int64_t)a.HV * a.V);
+  if (a.dt_g == SSLA_F32) zero_uncovered((float*)dg, a, a.HV);
+  else zero_uncovered((__half*)dg, a, a.HV);  // 0 has the same bits in both 16-bit types
+  if (a.dt_b == SSLA_F32) zero_uncovered((float*)dbeta, a, a.HV);
+  else zero_uncovered((__half*)dbeta, a, a.HV);
+
+  const int64_t chunk = blockIdx.x / a.HV;
+  const int hv = (int)(blockIdx.x - chunk * a.HV), h = hv / a.R;
+  const size_t item = blockIdx.x;
+  int64_t t0;
+  int rows;
+  if (!locate(tab, a.MC, chunk, t0, rows)) return;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const size_t qk = ((size_t)t0 * a.H + h) * a.K;
+  load_rows<TI, LDK, KP>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  load_rows<TI, LDK, KP>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  load_f32<LDC, BT, BT>(s.t, tinv + item * (BT * BT), BT);
+  cp_commit();
+  if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
+  const TI *sk = s.k, *sq = s.q, *sd = s.d;
+  const int m0 = (warp >> 1) * 16, half = warp & 1, n0 = half * (VB / 2), p0 = half * 32, k0 = half * (KP / 2);
+  const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
+  const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
+  const TI* gv = (const TI*)a.v + vo;
+  auto fk_row = [&](int m, int k) { return ldf(sk + m * LDK + k); };
+  auto fx = [&](int k, int n) { return s.x[k * LDX + n]; };
+
+  float aq[1][NK][4], ar[1][NK][4], ac[1][NK][4];  // dO S^T, F S^T, U D^T
+  float ap[1][4][4], ae[1][4][4];                  // dO U^T, F U^T
+  zero(aq); zero(ar); zero(ac); zero(ap); zero(ae);
+  float rb[2] = {0.f, 0.f};  // F . X of rows m0 + lane/4 (+ 8)
+  float dot = 0.f;           // <S, D>
+  const bool low = p0 <= m0;
+  for (int v0 = 0; v0 < a.V; v0 += VB) {
+    __syncthreads();
+    load_f32<LDX, KP, VB>(s.s, states + item * KP * VP + v0, VP);
+    load_f32<LDX, KP, VB>(s.e, ds + item * KP * VP + v0, VP);
+    load_rows<TI, LDO, VB>(s.d, dout + vo + v0, vstride, rows, a.V - v0, vec_d);
+    cp_commit();
+    if (v0 == 0) {
+      cp_wait<1>();
+      __syncthreads();
+      float acc[1][4][4];
+      zero(acc);
+      if (low)
+        warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return ldf(sq + m * LDK + k); },
+                           [&](int k, int n) { return ldf(sk + n * LDK + k); });
+      each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
+        s.p[i * LDC + j] = i >= j ? s.gates.fade(i, j) * x : 0.f;
+        s.p[i * LDC + j + 1] = i > j ? s.gates.fade(i, j + 1) * y : 0.f;
+      });
+    }
+    float xv[1][NT][4];
+    each_pair(xv, m0, n0, [&](int i, int n, float& x, float& y) {
+      const int c = v0 + n;
+      x = i < rows && c < a.V ? ldf(gv + i * vstride + c) : 0.f;
+      y = i < rows && c + 1 < a.V ? ldf(gv + i * vstride + c + 1) : 0.f;
+    });
+    cp_wait<0>();
+    __syncthreads();
+    float ks[1][NT][4], du[1][NT][4];
+    zero(ks);
+    zero(du);
+    warp_mma<X, false, SP>(ks, m0, n0, 0, KP, fk_row, [&](int k, int n) { return s.s[k * LDX + n]; });
+    warp_mma<X, false, SP>(du, m0, n0, 0, KP, fk_row, [&](int k, int n) { return s.e[k * LDX + n]; });
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = m0 + (lane >> 2) + (r >= 2 ? 8 : 0);
+        xv[0][j][r] -= s.gates.start[i] * ks[0][j][r];
+        du[0][j][r] *= s.gates.left[i];
+      }
+    each_pair(xv, m0, n0, [&](int i, int n, float x, float y) {
+      const float b = s.gates.beta[i];
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(b * x, b * y);
+    });
+    for (int i = tid; i < KP * (VB / 4); i += THREADS) {
+      const int r = i / (VB / 4), c = (i % (VB / 4)) * 4;
+      const float4 x = *reinterpret_cast<const float4*>(s.s + r * LDX + c);
+      const float4 y = *reinterpret_cast<const float4*>(s.e + r * LDX + c);
+      dot += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
+    }
+    __syncthreads();
+    zero(ks);
+    warp_mma<false, false, SP>(ks, m0, n0, 0, m0 + 16, [&](int m, int k) { return s.t[m * LDC + k]; }, fx);  // U
+    {
+      float pd[1][NT][4];
+      zero(pd);
+      warp_mma<false, X, SP>(pd, m0, n0, m0, BT, [&](int m, int k) { return s.p[k * LDC + m]; },
+                             [&](int k, int n) { return ldf(sd + k * LDO + n); });
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) du[0][j][r] = fmaf(a.scale, pd[0][j][r], du[0][j][r]);
+    }
+    __syncthreads();
+    each_pair(ks, m0, n0, [&](int i, int n, float x, float y) {
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(x, y);
+    });
+    each_pair(du, m0, n0, [&](int i, int n, float x, float y) {
+      *reinterpret_cast<float2*>(s.f + i * LDX + n) = make_float2(x, y);
+    });
+    __syncthreads();
+    zero(du);
+    warp_mma<false, false, SP>(du, m0, n0, m0, BT, [&](int m, int k) { return s.t[k * LDC + m]; },
+                               [&](int k, int n) { return s.f[k * LDX + n]; });  // F
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      rb[0] += du[0][j][0] * xv[0][j][0] + du[0][j][1] * xv[0][j][1];
+      rb[1] += du[0][j][2] * xv[0][j][2] + du[0][j][3] * xv[0][j][3];
+    }
+    each_pair(du, m0, n0, [&](int i, int n, float x, float y) {
+      const int c = v0 + n;
+      if (i < rows) {
+        const float b = s.gates.beta[i];
+        TI* p = dv + vo + i * vstride + c;
+        if (c < a.V) stf(p, b * x);
+        if (c + 1 < a.V) stf(p + 1, b * y);
+      }
+    });
+    __syncthreads();
+    each_pair(du, m0, n0, [&](int i, int n, float x, float y) {
+      *reinterpret_cast<float2*>(s.f + i * LDX + n) = make_float2(x, y);
+    });
+    __syncthreads();
+    auto ff = [&](int m, int k) { return s.f[m * LDX + k]; };
+    auto fd = [&](int m, int k) { return ldf(sd + m * LDO + k); };
+    auto fu_t = [&](int k, int n) { return s.x[n * LDX + k]; };
+    auto fs_t = [&](int k, int n) { return s.s[n * LDX + k]; };
+    if (low) {
+      warp_mma<X, false, SP>(ap, m0, p0, 0, VB, fd, fu_t);
+      warp_mma<false, false, SP>(ae, m0, p0, 0, VB, ff, fu_t);
+    }
+    warp_mma<X, false, SP>(aq, m0, k0, 0, VB, fd, fs_t);
+    warp_mma<false, false, SP>(ar, m0, k0, 0, VB, ff, fs_t);
+    warp_mma<false, false, SP>(ac, m0, k0, 0, VB, [&](int m, int k) { return s.x[m * LDX + k]; },
+                               [&](int k, int n) { return s.e[n * LDX + k]; });
+  }
+  __syncthreads();
+  // dP and E take the places of P and T
+  each_pair(ap, m0, p0, [&](int i, int j, float x, float y) {
+    s.p[i * LDC + j] = i >= j ? a.scale * s.gates.fade(i, j) * x : 0.f;
+    s.p[i * LDC + j + 1] = i > j ? a.scale * s.gates.fade(i, j + 1) * y : 0.f;
+  });
+  each_pair(ae, m0, p0, [&](int i, int j, float x, float y) {
+    s.t[i * LDC + j] = i > j ? s.gates.fade(i, j) * x : 0.f;
+    s.t[i * LDC + j + 1] = i > j + 1 ? s.gates.fade(i, j + 1) * y : 0.f;
+  });
+  __syncthreads();
+  auto fk_tok = [&](int k, int n) { return ldf(sk + k * LDK + n); };
+  const int i0 = m0 + (lane >> 2);
+  float rl[2] = {0.f, 0.f}, rq[2] = {0.f, 0.f}, rr[2] = {0.f, 0.f}, rc[2] = {0.f, 0.f}, rg[2] = {0.f, 0.f};
+  // sums over an accumulator's columns of tile * accumulator, per row
+  auto row_dot = [&](float (&acc)[1][NK][4], const TI* tile, float (&out)[2]) {
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      const int c = k0 + 8 * j + 2 * (lane & 3);
+      out[0] += acc[0][j][0] * ldf(tile + i0 * LDK + c) + acc[0][j][1] * ldf(tile + i0 * LDK + c + 1);
+      out[1] += acc[0][j][2] * ldf(tile + (i0 + 8) * LDK + c) + acc[0][j][3] * ldf(tile + (i0 + 8) * LDK + c + 1);
+    }
+  };
+  {
+    float ag[1][NK][4];
+    zero(ag);
+    warp_mma<false, X, SP>(ag, m0, k0, 0, m0 + 16, [&](int m, int k) { return s.t[m * LDC + k]; }, fk_tok);
+    row_dot(ag, sk, rg);
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = i0 + (r >= 2 ? 8 : 0);
+        const float b = s.gates.beta[i], e = s.gates.start[i];
+        ar[0][j][r] = -b * fmaf(e, ar[0][j][r], ag[0][j][r]);
+        aq[0][j][r] *= a.scale * e;
+        ac[0][j][r] *= s.gates.left[i];
+      }
+  }
+  row_dot(ar, sk, rr);
+  row_dot(ac, sk, rl);
+  warp_mma<false, X, SP>(aq, m0, k0, 0, m0 + 16, [&](int m, int k) { return s.p[m * LDC + k]; }, fk_tok);
+  row_dot(aq, sq, rq);
+  warp_mma<false, X, SP>(ac, m0, k0, m0, BT, [&](int m, int k) { return s.p[k * LDC + m]; },
+                         [&](int k, int n) { return ldf(sq + k * LDK + n); });
+  warp_mma<false, X, SP>(ac, m0, k0, m0, BT, [&](int m, int k) { return -s.gates.beta[k] * s.t[k * LDC + m]; }, fk_tok);
+  row_dot(ac, sk, rc);
+  const size_t qo = dqk ? ((size_t)t0 * a.HV + hv) * a.K : qk, qstride = (size_t)(dqk ? a.HV : a.H) * a.K;
+  auto put = [&](size_t at, int c, float x, float y, TI* out, float* part) {
+    if (part) {
+      if (c < a.K) part[at] = x;
+      if (c + 1 < a.K) part[at + 1] = y;
+    } else {
+      if (c < a.K) stf(out + at, x);
+      if (c + 1 < a.K) stf(out + at + 1, y);
+    }
+  };
+  each_pair(aq, m0, k0, [&](int i, int c, float x, float y) {
+    if (i < rows) put(qo + i * qstride + c, c, x, y, dq, dqk);
+  });
+#pragma unroll
+  for (int j = 0; j < NK; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ac[0][j][r] += ar[0][j][r];
+  each_pair(ac, m0, k0, [&](int i, int c, float x, float y) {
+    if (i < rows) put(qo + i * qstride + c, c, x, y, dk, dqk ? dqk + TK : nullptr);
+  });
+  // rows: over the four lanes of a row, then over the two warps that share it
+  auto reduce = [&](float (&x)[2], int slot) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float y = x[r];
+      y += __shfl_xor_sync(0xffffffffu, y, 1);
+      y += __shfl_xor_sync(0xffffffffu, y, 2);
+      if ((lane & 3) == 0) s.red[slot][half][i0 + 8 * r] = y;
+    }
+  };
+  reduce(rb, 0);
+  reduce(rg, 1);
+  reduce(rq, 2);
+  reduce(rr, 3);
+  reduce(rc, 4);
+  reduce(rl, 5);
+#pragma unroll
+  for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
+  if (lane == 0) s.dots[warp] = dot;
+  __syncthreads();
+  if (warp) return;
+  float sum = 0.f, gc[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int i = 2 * lane + r;
+    auto row = [&](int slot) { return s.red[slot][0][i] + s.red[slot][1][i]; };
+    gc[r] = row(2) + row(3) - row(4);
+    sum += row(5);
+    if (i < rows) st_any(dbeta, a.dt_b, (size_t)(t0 + i) * a.HV + hv, row(0) - row(1));
+  }
+#pragma unroll
+  for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) all += s.dots[w];
+  sum = fmaf(s.gates.whole, all, sum);
+  float suf = gc[0] + gc[1];  // inclusive suffix sums over lanes
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const float y = __shfl_down_sync(0xffffffffu, suf, m);
+    if (lane + m < 32) suf += y;
+  }
+  const size_t at = (size_t)(t0 + 2 * lane) * a.HV + hv;
+  if (2 * lane < rows) st_any(dg, a.dt_g, at, suf + sum);
+  if (2 * lane + 1 < rows) st_any(dg, a.dt_g, at + a.HV, suf - gc[0] + sum);
+}
+
+// dq, dk [T, H, K] = sums over the value heads of a key head, in their order.
+template <class TI>
+__global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ dqk, int64_t T, int H, int R, int K,
+                                                        TI* __restrict__ dq, TI* __restrict__ dk) {
+  const int64_t n = T * H * K;
+  const float* p = dqk + (blockIdx.y ? n * R : 0);
+  TI* out = blockIdx.y ? dk : dq;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t th = i / K;
+    const int k = (int)(i - th * K);
+    float x = 0.f;
+    for (int r = 0; r < R; ++r) x += p[(th * R + r) * K + k];
+    stf(out + i, x);
+  }
+}
+
+template <class TI, int KP, bool SP>
+int run_adjoint(const Args& a, const Saved& sv, int VP, const void* dout, float* ds, int64_t items, cudaStream_t st) {
+  const size_t smem = sizeof(AdjSmem<TI, KP>);
+  cudaFuncSetAttribute(adjoint_kernel<TI, KP, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  adjoint_kernel<TI, KP, SP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, (const TI*)dout, ds);
+  SSLA_CHECK_LAUNCH("gated_delta_rule adjoint");
+  return SSLA_OK;
+}
+
+template <class TI, int KP>
+int run_bwd(const Args& a, const Plan& p, const Saved& sv, const Work& w, int VP, const void* dout, const float* dht,
+            void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dh0, cudaStream_t st) {
+  const int64_t items = p.MC * a.HV;
+  int rc = SSLA_OK;
+  if (items > 0) {
+    // dh0 leaves in fp32: its increments take the split even for bf16 tokens
+    rc = OutSplit<TI>::v || dh0 ? run_adjoint<TI, KP, true>(a, sv, VP, dout, w.ds, items, st)
+                                : run_adjoint<TI, KP, OutSplit<TI>::v>(a, sv, VP, dout, w.ds, items, st);
+    if (rc) return rc;
+  }
+  rc = run_chain(p, sv, w, w.ds, dht, dh0, a.N, a.HV, a.K, a.V, true, st);
+  if (rc || a.T == 0) return rc;
+  float* dqk = a.R > 1 ? w.dqk : nullptr;
+  const size_t smem = sizeof(BwdSmem<TI, KP>);
+  cudaFuncSetAttribute(backward_kernel<TI, KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  backward_kernel<TI, KP><<<(unsigned)(items > 0 ? items : 1), THREADS, smem, st>>>(
+      a, sv.chunk_tab, VP, sv.tinv, sv.s, w.ds, (const TI*)dout, (TI*)dq, (TI*)dk, (TI*)dv, dg, dbeta, dqk);
+  SSLA_CHECK_LAUNCH("gated_delta_rule backward");
+  if (dqk) {
+    const int64_t n = a.T * a.H * a.K;
+    const int64_t blocks = (n + 255) / 256;
+    sum_heads_kernel<TI><<<dim3((unsigned)(blocks < 8 * kNumSMs ? blocks : 8 * kNumSMs), 2), 256, 0, st>>>(
+        dqk, a.T, a.H, a.R, a.K, (TI*)dq, (TI*)dk);
+    SSLA_CHECK_LAUNCH("gated_delta_rule sum_heads");
+  }
+  return SSLA_OK;
+}
+
+}  // namespace
+}  // namespace delta
+}  // namespace ssla
+
+using namespace ssla;
+using namespace ssla::delta;
+
+extern "C" int ssla_chunk_gated_delta_rule_bwd(const void* q, const void* k, const void* v, const void* g,
+                                               const void* beta, int dtype, int dtype_g, int dtype_beta,
+                                               const int64_t* cu_seqlens, int64_t n_seqs, int64_t T, int64_t H,
+                                               int64_t HV, int64_t K, int64_t V, float scale, const void* states,
+                                               size_t states_bytes, const void* dout, const float* dht, void* dq,
+                                               void* dk, void* dv, void* dg, void* dbeta, float* dh0, void* workspace,
+                                               size_t workspace_bytes, ssla_stream_t stream) {
+  const char* name = "ssla_chunk_gated_delta_rule_bwd";
+  int rc = check_args(name, dtype, dtype_g, dtype_beta, n_seqs, T, H, HV, K, V);
+  if (rc) return rc;
+  if (HV == 0) return SSLA_OK;
+  SSLA_CHECK_ARG(cu_seqlens && states, "%s: null pointer", name);
+  SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && dout && dq && dk && dv && dg && dbeta), "%s: null pointer", name);
+  const Plan p = make_plan(n_seqs, T, HV, K, V);
+  const int KP = pad_k(K), VP = pad_v(V);
+  Saved sv;
+  Work w;
+  const size_t need = saved_layout(const_cast<void*>(states), p, n_seqs, HV, KP, VP, &sv);
+  const size_t need_w = work_layout(workspace, p, T, H, HV, K, KP, VP, true, &w);
+  if (states_bytes < need || workspace_bytes < need_w || (need_w && !workspace)) {
+    set_error("%s: states of %zu bytes and workspace of %zu, %zu and %zu needed", name, states_bytes, workspace_bytes,
+              need, need_w);
+    return SSLA_ERR_WORKSPACE;
+  }
+  SSLA_CHECK_ARG(aligned_to(states, 16) && aligned_to(workspace, 16), "%s: states and workspace must be 16-byte aligned", name);
+  cudaStream_t st = (cudaStream_t)stream;
+  const Args a = make_args(q, k, v, g, beta, dtype, dtype_g, dtype_beta, cu_seqlens, n_seqs, T, H, HV, K, V, scale);
+  return SSLA_DISPATCH_DTYPE(dtype, T_, [&] {
+    return KP == 64 ? run_bwd<T_, 64>(a, p, sv, w, VP, dout, dht, dq, dk, dv, dg, dbeta, dh0, st)
+                    : run_bwd<T_, 128>(a, p, sv, w, VP, dout, dht, dq, dk, dv, dg, dbeta, dh0, st);
+  });
+}

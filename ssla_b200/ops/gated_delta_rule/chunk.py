@@ -1,0 +1,179 @@
+"""Chunked gated delta rule over packed variable-length sequences.
+
+Next to ``chunk_gla`` (whose layout, argument order and conventions it keeps) for states that are
+corrected instead of only added to: before a token writes its value, what the state already
+returns for its key is subtracted.  Per value head, with state S [K, V]::
+
+    S <- exp(g_t) S;   u_t = beta_t (v_t - S^T k_t);   S <- S + k_t u_t^T;   o_t = scale S^T q_t
+
+``beta k^T k`` should stay below 2 (keys of unit length, beta in [0, 1] or [0, 2)): beyond that the
+recurrence itself grows without bound.  The kernels are ``ssla_chunk_gated_delta_rule_fwd`` /
+``_bwd`` of the C ABI; the project ssla follows has no delta rule.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ... import _lib
+from ..utils.guard import prepare_cu_seqlens
+
+
+def norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, what):
+    """Checked, contiguous inputs of one dtype (q's) on q's device; gates in their own dtype."""
+    if q.dim() != 3 or k.shape != q.shape or v.dim() != 3 or v.shape[0] != q.shape[0]:
+        raise ValueError(
+            f"{what} expects q, k [T, H, K] and v [T, HV, V]; got q {tuple(q.shape)}, k {tuple(k.shape)}, "
+            f"v {tuple(v.shape)}"
+        )
+    T, H, K = q.shape
+    HV, V = v.shape[1:]
+    if H == 0 or HV == 0 or HV % H:
+        raise ValueError(f"{what}: the {HV} value heads must be a positive multiple of the {H} key heads")
+    if g.shape != (T, HV) or beta.shape != (T, HV):
+        raise ValueError(f"{what} expects g, beta [T, HV] = [{T}, {HV}]; got {tuple(g.shape)}, {tuple(beta.shape)}")
+    if not (1 <= K <= 128 and 1 <= V <= 256):
+        raise ValueError(f"{what}: K={K}, V={V} not supported (1 <= K <= 128, 1 <= V <= 256)")
+    _lib.require_cuda(q, k, v, g, beta, initial_state, what=what)
+    dev, dt = q.device, q.dtype
+    _lib.dtype_code(q)
+    for x in (k, v, g, beta, initial_state):
+        if x is not None and x.device != dev:
+            raise RuntimeError(f"{what}: all tensors must be on one device, got {dev} and {x.device}")
+    cu = prepare_cu_seqlens(cu_seqlens, dev)
+    if initial_state is not None:
+        N = cu.numel() - 1
+        if initial_state.dim() == 0 or initial_state.shape[0] != N:
+            raise ValueError(
+                f"The number of initial states is expected to be equal to the number of input sequences, "
+                f"i.e., {N} rather than {initial_state.shape[0] if initial_state.dim() else 0}."
+            )
+        if initial_state.shape != (N, HV, K, V):
+            raise ValueError(f"{what}: initial_state must be [N, HV, K, V] = {(N, HV, K, V)}; got "
+                             f"{tuple(initial_state.shape)}")
+        initial_state = initial_state.float().contiguous()
+    if k.dtype != dt:
+        k = k.to(dt)
+    if v.dtype != dt:
+        v = v.to(dt)
+    if g.dtype not in _lib._DT:
+        g = g.float()
+    if beta.dtype not in _lib._DT:
+        beta = beta.float()
+    return (q.contiguous(), k.contiguous(), v.contiguous(), g.contiguous(), beta.contiguous(), cu, initial_state)
+
+
+def tensor_args(q, k, v, g, beta, cu, scale):
+    """The arguments that every entry point of the family starts with."""
+    T, H, K = q.shape
+    HV, V = v.shape[1:]
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), _lib.dtype_code(q),
+            _lib.dtype_code(g), _lib.dtype_code(beta), cu.data_ptr(), cu.numel() - 1, T, H, HV, K, V, float(scale))
+
+
+def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
+    """(o, final state or None, states): ``states`` is what the backward needs of the chunks."""
+    T, H, K = q.shape
+    HV, V = v.shape[1:]
+    N = cu.numel() - 1
+    L = _lib.load()
+    dev = q.device
+    o = torch.empty_like(v)
+    ht = torch.empty((N, HV, K, V), device=dev, dtype=torch.float32) if output_final_state else None
+    nb = L.ssla_gated_delta_rule_states_bytes(N, T, H, HV, K, V)
+    states = torch.empty(nb, device=dev, dtype=torch.uint8)
+    wb = L.ssla_gated_delta_rule_workspace_bytes(N, T, H, HV, K, V, 0)
+    ws = torch.empty(wb, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        _lib.check(
+            L.ssla_chunk_gated_delta_rule_fwd(
+                *tensor_args(q, k, v, g, beta, cu, scale), _lib.ptr(h0), o.data_ptr(), _lib.ptr(ht),
+                states.data_ptr(), nb, ws.data_ptr(), wb, _lib.stream_of(q),
+            ),
+            "chunk_gated_delta_rule forward",
+        )
+    return o, ht, states
+
+
+def chunk_bwd(q, k, v, g, beta, cu, scale, has_h0, states, do, dht):
+    T, H, K = q.shape
+    HV, V = v.shape[1:]
+    N = cu.numel() - 1
+    L = _lib.load()
+    dev = q.device
+    do = do.to(q.dtype).contiguous()
+    dht = dht.float().contiguous() if dht is not None else None
+    dq, dk, dv, dg, dbeta = (torch.empty_like(x) for x in (q, k, v, g, beta))
+    dh0 = torch.empty((N, HV, K, V), device=dev, dtype=torch.float32) if has_h0 else None
+    wb = L.ssla_gated_delta_rule_workspace_bytes(N, T, H, HV, K, V, 1)
+    ws = torch.empty(wb, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        _lib.check(
+            L.ssla_chunk_gated_delta_rule_bwd(
+                *tensor_args(q, k, v, g, beta, cu, scale), states.data_ptr(), states.numel(), do.data_ptr(),
+                _lib.ptr(dht), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
+                _lib.ptr(dh0), ws.data_ptr(), wb, _lib.stream_of(q),
+            ),
+            "chunk_gated_delta_rule backward",
+        )
+    return dq, dk, dv, dg, dbeta, dh0
+
+
+class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, cu_seqlens, scale, initial_state, output_final_state):
+        q, k, v, g, beta, cu, h0 = norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, "chunk_gated_delta_rule")
+        o, ht, states = chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
+        ctx.save_for_backward(q, k, v, g, beta, cu, states)
+        ctx.scale = scale
+        ctx.has_h0 = h0 is not None
+        return o, ht
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dht):
+        q, k, v, g, beta, cu, states = ctx.saved_tensors
+        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, ctx.has_h0, states, do, dht)
+        return dq, dk, dv, dg, dbeta, None, None, dh0, None
+
+
+def needs_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+@torch.compiler.disable
+def chunk_gated_delta_rule(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    g: torch.Tensor,
+    beta: torch.Tensor,
+    cu_seqlens: torch.LongTensor,
+    scale: Optional[float] = None,
+    initial_state: Optional[torch.Tensor] = None,
+    output_final_state: bool = False,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    r"""Chunked gated delta rule.
+
+    Args:
+        q, k: ``[T, H, K]`` (K <= 128); v: ``[T, HV, V]`` (V <= 256), HV a multiple of H: every key
+            head serves ``HV / H`` consecutive value heads.
+        g: log forget gates ``[T, HV]`` (g <= 0; ``-inf`` empties the state before the token).
+        beta: writing strengths ``[T, HV]``.
+        cu_seqlens: cumulative sequence lengths ``[N+1]``; tokens outside every sequence get zero
+            outputs and zero gradients.
+        scale: read-out scale, default ``K ** -0.5``.
+        initial_state: ``[N, HV, K, V]`` or None.
+        output_final_state: also return the final state ``[N, HV, K, V]`` (fp32).
+    Returns:
+        ``(o [T, HV, V], final_state or None)``.
+    """
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if needs_grad(q, k, v, g, beta, initial_state):
+        return ChunkGatedDeltaRuleFunction.apply(q, k, v, g, beta, cu_seqlens, scale, initial_state,
+                                                 output_final_state)
+    q, k, v, g, beta, cu, h0 = norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, "chunk_gated_delta_rule")
+    return chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)[:2]

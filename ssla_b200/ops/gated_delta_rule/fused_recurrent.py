@@ -1,0 +1,75 @@
+"""Token-by-token gated delta rule for serving: one or a few tokens of every sequence.
+
+Same arguments and results as ``chunk_gated_delta_rule``; carry ``final_state`` into the next call
+as ``initial_state``.  The forward is ``ssla_recurrent_gated_delta_rule_fwd`` (the state stays in
+registers over a sequence's tokens and crosses HBM once each way); gradients are those of the same
+function and come from the chunked kernels.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ... import _lib
+from .chunk import chunk_bwd, chunk_fwd, needs_grad, norm_inputs, tensor_args
+
+_NAME = "fused_recurrent_gated_delta_rule"
+
+
+def recurrent_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
+    HV, V = v.shape[1:]
+    o = torch.empty_like(v)
+    ht = None
+    if output_final_state:
+        ht = torch.empty((cu.numel() - 1, HV, q.shape[-1], V), device=q.device, dtype=torch.float32)
+    with torch.cuda.device(q.device):
+        _lib.check(
+            _lib.load().ssla_recurrent_gated_delta_rule_fwd(
+                *tensor_args(q, k, v, g, beta, cu, scale), _lib.ptr(h0), o.data_ptr(), _lib.ptr(ht),
+                _lib.stream_of(q),
+            ),
+            _NAME,
+        )
+    return o, ht
+
+
+class FusedRecurrentGatedDeltaRuleFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, cu_seqlens, scale, initial_state, output_final_state):
+        q, k, v, g, beta, cu, h0 = norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, _NAME)
+        o, ht = recurrent_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
+        ctx.save_for_backward(q, k, v, g, beta, cu, h0)
+        ctx.scale = scale
+        return o, ht
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do, dht):
+        q, k, v, g, beta, cu, h0 = ctx.saved_tensors
+        states = chunk_fwd(q, k, v, g, beta, cu, ctx.scale, h0, False)[2]
+        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, h0 is not None, states, do, dht)
+        return dq, dk, dv, dg, dbeta, None, None, dh0, None
+
+
+@torch.compiler.disable
+def fused_recurrent_gated_delta_rule(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    g: torch.Tensor,
+    beta: torch.Tensor,
+    cu_seqlens: torch.LongTensor,
+    scale: Optional[float] = None,
+    initial_state: Optional[torch.Tensor] = None,
+    output_final_state: bool = False,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    r"""Recurrent gated delta rule; arguments and returns as ``chunk_gated_delta_rule``."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if needs_grad(q, k, v, g, beta, initial_state):
+        return FusedRecurrentGatedDeltaRuleFunction.apply(q, k, v, g, beta, cu_seqlens, scale, initial_state,
+                                                          output_final_state)
+    q, k, v, g, beta, cu, h0 = norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, _NAME)
+    return recurrent_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)

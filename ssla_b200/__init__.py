@@ -6,7 +6,7 @@ Import paths mirror the reference project (``ops.gla.chunk``, ``ops.common.scan`
 """
 
 __all__ = ["chunk_gla", "fused_recurrent_gla", "chunk_gla_scalar", "scan", "chunk_gated_delta_rule",
-           "fused_recurrent_gated_delta_rule"]
+           "fused_recurrent_gated_delta_rule", "group_norm_act"]
 
 
 def __getattr__(name):
@@ -25,4 +25,7 @@ def __getattr__(name):
     if name in ("chunk_gated_delta_rule", "fused_recurrent_gated_delta_rule"):
         from .ops import gated_delta_rule
         return getattr(gated_delta_rule, name)
+    if name == "group_norm_act":
+        from .ops.norm import group_norm_act
+        return group_norm_act
     raise AttributeError(name)

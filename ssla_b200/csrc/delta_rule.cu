@@ -4,95 +4,11 @@
 //   chain       S' = exp(gC) S - PM S + B along every sequence: the one sequential part
 //   output      per (chunk, value head): O from the start state
 #include "delta_rule.cuh"
+#include "pack_tables.cuh"
 
 namespace ssla {
 namespace delta {
 namespace {
-
-// ------------------------------------------------------------------ tables
-__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : (x > hi ? hi : x); }
-
-__global__ void __launch_bounds__(1024) tables_kernel(const int64_t* __restrict__ cu, int64_t N, int64_t T, int64_t MC,
-                                                      int64_t len, int64_t MS, int* chunk_off, int* seg_off,
-                                                      longlong2* chunk_tab, int4* seg_tab) {
-  __shared__ int wc[32], ws[32], run[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) run[0] = run[1] = 0;
-  __syncthreads();
-  for (int64_t n0 = 0; n0 < N; n0 += 1024) {
-    const int64_t n = n0 + tid;
-    int c = 0, g = 0;
-    if (n < N) {
-      const int64_t b = clamp64(cu[n], 0, T), e = clamp64(cu[n + 1], b, T);
-      c = (int)((e - b + BT - 1) / BT);
-      g = len ? (int)((c + len - 1) / len) : 0;
-    }
-    int sc = c, sg = g;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sc, d), y = __shfl_up_sync(0xffffffffu, sg, d);
-      if (lane >= d) { sc += x; sg += y; }
-    }
-    if (lane == 31) { wc[warp] = sc; ws[warp] = sg; }
-    __syncthreads();
-    if (warp == 0) {
-      int a = wc[lane], b = ws[lane];
-      const int a0 = a, b0 = b;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, a, d), y = __shfl_up_sync(0xffffffffu, b, d);
-        if (lane >= d) { a += x; b += y; }
-      }
-      wc[lane] = a - a0;
-      ws[lane] = b - b0;
-    }
-    __syncthreads();
-    const int ac = run[0] + wc[warp] + sc, ag = run[1] + ws[warp] + sg;
-    if (n < N) {
-      chunk_off[n] = (int)clamp64(ac - c, 0, MC);  // MC, MS bound well-formed sequences; the clamp keeps
-      seg_off[n] = (int)clamp64(ag - g, 0, MS);    // malformed offsets inside the buffers
-    }
-    __syncthreads();
-    if (tid == 1023) { run[0] = ac; run[1] = ag; }
-    __syncthreads();
-  }
-  if (tid == 0) {
-    chunk_off[N] = (int)clamp64(run[0], 0, MC);
-    seg_off[N] = (int)clamp64(run[1], 0, MS);
-  }
-  __threadfence_block();
-  __syncthreads();
-  auto owner = [&](const int* off, int64_t c) {  // last n with off[n] <= c
-    int64_t lo = 0, hi = N;
-    while (hi - lo > 1) {
-      const int64_t m = (lo + hi) >> 1;
-      if (off[m] <= c) lo = m; else hi = m;
-    }
-    return lo;
-  };
-  const int total = chunk_off[N], segs = seg_off[N];
-  for (int64_t c = tid; c < MC; c += 1024) {
-    longlong2 e = make_longlong2(0, -1);
-    if (c < total) {
-      const int64_t n = owner(chunk_off, c);
-      const int64_t b = clamp64(cu[n], 0, T), t1 = clamp64(cu[n + 1], b, T), t0 = b + (c - chunk_off[n]) * BT;
-      const int64_t rows = t1 - t0 < BT ? t1 - t0 : BT;
-      if (rows > 0) e = make_longlong2(t0, rows | (n << 32));
-    }
-    chunk_tab[c] = e;
-  }
-  for (int64_t s = tid; s < MS; s += 1024) {
-    int4 e = make_int4(0, 0, -1, 0);
-    if (s < segs) {
-      const int n = (int)owner(seg_off, s);
-      const int first = chunk_off[n] + (int)((s - seg_off[n]) * len);
-      int cnt = chunk_off[n + 1] - first;
-      cnt = cnt < 0 ? 0 : (cnt > len ? (int)len : cnt);
-      e = make_int4(first, cnt, n, 0);
-    }
-    seg_tab[s] = e;
-  }
-}
 
 // ------------------------------------------------------------------ (I + A)^-1 of a 64 x 64 tile
 // sA strictly lower triangular -> sT, upper triangle zero; sY is scratch (>= 2048 floats).
@@ -696,9 +612,9 @@ extern "C" int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, con
   }
   SSLA_CHECK_ARG(aligned_to(states, 16) && aligned_to(workspace, 16), "%s: states and workspace must be 16-byte aligned", name);
   cudaStream_t st = (cudaStream_t)stream;
-  tables_kernel<<<1, 1024, 0, st>>>(cu_seqlens, n_seqs, T, p.MC, p.len, p.MS, sv.chunk_off, sv.seg_off, sv.chunk_tab,
-                                    sv.seg_tab);
-  SSLA_CHECK_LAUNCH(name);
+  rc = launch_pack_tables(cu_seqlens, n_seqs, T, BT, p.MC, p.len, p.MS, sv.chunk_off, sv.seg_off, sv.chunk_tab,
+                          sv.seg_tab, st);
+  if (rc) return rc;
   const Args a = make_args(q, k, v, g, beta, dtype, dtype_g, dtype_beta, cu_seqlens, n_seqs, T, H, HV, K, V, scale);
   return SSLA_DISPATCH_DTYPE(dtype, T_, [&] {
     return KP == 64 ? run_fwd<T_, 64>(a, p, sv, w, VP, h0, o, ht, st) : run_fwd<T_, 128>(a, p, sv, w, VP, h0, o, ht, st);

@@ -101,12 +101,12 @@ template <class TI, int KP> struct PrepSmem {
   TI v[BT * LDV];
   float a[BT * LDC];
   float t[BT * LDC];
-  float y[BT * 72];
+  float y[BT * 68];
   float col[BT];
   Gates gates;
 };
 
-template <class TI, int KP>
+template <class TI, int KP, bool SP>
 __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong2* __restrict__ tab, int VP,
                                                           float* __restrict__ decay, float* __restrict__ tinv,
                                                           float* __restrict__ pm, float* __restrict__ bout) {
@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
     float acc[1][4][4];
     zero(acc);
     if (n0 <= m0)
-      warp_mma<X, X, true>(acc, m0, n0, 0, KP, [&](int m, int k) { return ldf(sk + m * LDK + k); },
-                           [&](int k, int n) { return ldf(sk + n * LDK + k); });
+      warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sk + m * LDK + k); },
+                         [&](int k, int n) { return pair(sk + n * LDK + k); });
     each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
       const float b = s.gates.beta[i];
       s.a[i * LDC + j] = i > j ? b * s.gates.fade(i, j) * x : 0.f;
@@ -169,14 +169,17 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
     {
       float acc[1][4][4];
       zero(acc);
-      auto fa = [&](int i, int j) { return s.t[i * LDC + j] * s.col[j]; };
+      auto fa = [&](int i, int j) {
+        const float2 x = pair(s.t + i * LDC + j), c = pair(s.col + j);
+        return make_float2(x.x * c.x, x.y * c.y);
+      };
       if (w)
-        warp_mma<false, X, true>(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return ldf(sk + j * LDK + c0 + n); });
+        warp_mma<false, X, SP>(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return column<LDK>(sk + j * LDK + c0 + n); });
       else
-        warp_mma<false, X, true>(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return ldf(s.v + j * LDV + n); });
+        warp_mma<false, X, SP>(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return column<LDV>(s.v + j * LDV + n); });
       each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
         const float l = s.gates.left[i];
-        *reinterpret_cast<float2*>(s.y + i * 72 + j) = make_float2(x * l, y * l);
+        *reinterpret_cast<float2*>(s.y + i * 68 + j) = stage2<SP>(x * l, y * l);
       });
     }
     __syncthreads();
@@ -185,12 +188,12 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
       float acc[MT][4][4];
       zero(acc);
       const int mk = (warp >> 1) * 16 * MT;
-      warp_mma<X, false, true>(acc, mk, n0, 0, BT, [&](int m, int j) { return ldf(sk + j * LDK + m); },
-                               [&](int j, int n) { return s.y[j * 72 + n]; });
+      warp_mma<X, !SP, SP>(acc, mk, n0, 0, BT, [&](int m, int j) { return column<LDK>(sk + j * LDK + m); },
+                           [&](int j, int n) { return column<68>(s.y + j * 68 + n); });
       float* out = w ? pm + item * KP * KP : bout + item * KP * VP;
       const int ld = w ? KP : VP;
       each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
-        *reinterpret_cast<float2*>(out + (size_t)m * ld + c0 + n) = make_float2(x, y);
+        *reinterpret_cast<float2*>(out + (size_t)m * ld + c0 + n) = w ? stage2<SP>(x, y) : make_float2(x, y);
       });
     }
   }
@@ -210,13 +213,13 @@ struct ChainArgs {
   const float* init;      // [n * HV + hv][K][V] unpadded (padded: [KP][VP])
   float* last;            // likewise
   float* mseg;            // composing: [n * HV + hv][KP][KP] for the columns from VP on, start from I
-  bool init_padded, last_padded, reverse, compose;
+  bool init_padded, last_padded, reverse, compose, round;
   int HV, K, V, VP, slices;
 };
 
-template <int KP, int VS, bool TRANS>
+template <int KP, int VS, bool TRANS, bool SP>
 __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
-  constexpr int NTH = KP * 2, NT = VS / 8, LDP = KP + (TRANS ? 8 : 4), LDS = VS + 8;
+  constexpr int NTH = KP * 2, NT = VS / 8, LDP = KP + (TRANS ? 4 : 8), LDS = VS + 4;
   extern __shared__ __align__(16) unsigned char raw[];
   float* sp = reinterpret_cast<float*>(raw);
   float* ss = sp + 2 * KP * LDP;
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
     const size_t it = (size_t)at(i) * a.HV + hv;
     float* sc = ss + (i & 1) * KP * LDS;
     each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-      *reinterpret_cast<float2*>(sc + r * LDS + c) = make_float2(x, y);
+      *reinterpret_cast<float2*>(sc + r * LDS + c) = stage2<SP>(x, y);
     });
     const float d = a.decay ? a.decay[it] : 0.f;
 #pragma unroll
@@ -297,7 +300,8 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
       for (int r = 0; r < 4; ++r) bc[j][r] = bn[j][r];
     if (a.s && !ident)
       each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-        *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
+        *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) =
+            a.round ? make_float2(tf32(x), tf32(y)) : make_float2(x, y);
       });
     cp_wait<0>();
     __syncthreads();  // map i and the state are there, step i - 1 is read
@@ -309,9 +313,9 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
     const float* pc = sp + (i & 1) * KP * LDP;
     float acc[1][NT][4];
     zero(acc);
-    warp_mma<false, false, true>(acc, m0, 0, 0, KP,
-                                 [&](int m, int k) { return TRANS ? pc[k * LDP + m] : pc[m * LDP + k]; },
-                                 [&](int k, int n) { return sc[k * LDS + n]; });
+    warp_mma<!SP, !SP, SP>(acc, m0, 0, 0, KP,
+                           [&](int m, int k) { return TRANS ? column<LDP>(pc + k * LDP + m) : pair(pc + m * LDP + k); },
+                           [&](int k, int n) { return column<LDS>(sc + k * LDS + n); });
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -338,34 +342,36 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
   }
 }
 
-template <int KP, int VS, bool TRANS> int launch_chain(const ChainArgs& a, int64_t lists, cudaStream_t st) {
-  constexpr size_t smem = 4 * (2 * KP * (KP + (TRANS ? 8 : 4)) + 2 * KP * (VS + 8));
-  cudaFuncSetAttribute(chain_kernel<KP, VS, TRANS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <int KP, int VS, bool TRANS, bool SP> int launch_chain(const ChainArgs& a, int64_t lists, cudaStream_t st) {
+  constexpr size_t smem = 4 * (2 * KP * (KP + (TRANS ? 4 : 8)) + 2 * KP * (VS + 4));
+  cudaFuncSetAttribute(chain_kernel<KP, VS, TRANS, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   const int64_t grid = lists * a.HV * a.slices;
   if (grid == 0) return SSLA_OK;
-  chain_kernel<KP, VS, TRANS><<<(unsigned)grid, KP * 2, smem, st>>>(a);
+  chain_kernel<KP, VS, TRANS, SP><<<(unsigned)grid, KP * 2, smem, st>>>(a);
   SSLA_CHECK_LAUNCH("gated_delta_rule chain");
   return SSLA_OK;
 }
 
-int chain(ChainArgs a, int KP, int vs, bool trans, int64_t lists, cudaStream_t st) {
+template <int KP, int VS> int chain_vs(const ChainArgs& a, bool trans, bool split, int64_t lists, cudaStream_t st) {
+  if (split) return trans ? launch_chain<KP, VS, true, true>(a, lists, st) : launch_chain<KP, VS, false, true>(a, lists, st);
+  return trans ? launch_chain<KP, VS, true, false>(a, lists, st) : launch_chain<KP, VS, false, false>(a, lists, st);
+}
+
+template <int KP> int chain_kp(const ChainArgs& a, int vs, bool trans, bool split, int64_t lists, cudaStream_t st) {
+  if (vs == 8) return chain_vs<KP, 8>(a, trans, split, lists, st);
+  if (vs == 16) return chain_vs<KP, 16>(a, trans, split, lists, st);
+  if (vs == 32) return chain_vs<KP, 32>(a, trans, split, lists, st);
+  return chain_vs<KP, 64>(a, trans, split, lists, st);
+}
+
+int chain(ChainArgs a, int KP, int vs, bool trans, bool split, int64_t lists, cudaStream_t st) {
   a.slices = (a.VP + (a.compose ? KP : 0)) / vs;
-#define SSLA_CHAIN(KP_, VS_)                                     \
-  return trans ? launch_chain<KP_, VS_, true>(a, lists, st) : launch_chain<KP_, VS_, false>(a, lists, st)
-  if (KP == 64) {
-    if (vs == 16) SSLA_CHAIN(64, 16);
-    if (vs == 32) SSLA_CHAIN(64, 32);
-    SSLA_CHAIN(64, 64);
-  }
-  if (vs == 16) SSLA_CHAIN(128, 16);
-  if (vs == 32) SSLA_CHAIN(128, 32);
-  SSLA_CHAIN(128, 64);
-#undef SSLA_CHAIN
+  return KP == 64 ? chain_kp<64>(a, vs, trans, split, lists, st) : chain_kp<128>(a, vs, trans, split, lists, st);
 }
 
 // ------------------------------------------------------------------ output
 template <class TI, int KP, int VB> struct OutSmem {
-  static constexpr int LDK = KTile<TI, KP>::LD, LDV = VB + 8, LDX = VB + 8;
+  static constexpr int LDK = KTile<TI, KP>::LD, LDV = VB + 8, LDX = VB + 4;
   TI k[BT * LDK];
   TI q[BT * LDK];
   TI v[BT * LDV];
@@ -377,15 +383,14 @@ template <class TI, int KP, int VB> struct OutSmem {
 };
 
 template <class TI, int KP, int VB>
-__global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlong2* __restrict__ tab, int VP,
-                                                            const float* __restrict__ tinv,
-                                                            const float* __restrict__ states, TI* __restrict__ o) {
+__device__ __forceinline__ void output_chunk(const Args& a, const longlong2* __restrict__ tab, int VP,
+                                             const float* __restrict__ tinv, const float* __restrict__ states,
+                                             TI* __restrict__ o) {
   using S = OutSmem<TI, KP, VB>;
   constexpr bool X = Io16<TI>::exact, SP = OutSplit<TI>::v;
   constexpr int LDK = S::LDK, LDV = S::LDV, LDX = S::LDX, NT = VB / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
-  zero_uncovered(o, a, (int64_t)a.HV * a.V);
   const int64_t chunk = blockIdx.x / a.HV;
   const int hv = (int)(blockIdx.x - chunk * a.HV), h = hv / a.R;
   const size_t item = blockIdx.x;
@@ -415,11 +420,11 @@ __global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlo
       float acc[1][4][4];
       zero(acc);
       if (p0 <= m0)
-        warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return ldf(sq + m * LDK + k); },
-                           [&](int k, int n) { return ldf(sk + n * LDK + k); });
+        warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
+                           [&](int k, int n) { return pair(sk + n * LDK + k); });
       each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
-        s.p[i * LDC + j] = i >= j ? s.gates.fade(i, j) * x : 0.f;
-        s.p[i * LDC + j + 1] = i > j ? s.gates.fade(i, j + 1) * y : 0.f;
+        *reinterpret_cast<float2*>(s.p + i * LDC + j) =
+            stage2<SP>(i >= j ? s.gates.fade(i, j) * x : 0.f, i > j ? s.gates.fade(i, j + 1) * y : 0.f);
       });
     }
     cp_wait<0>();
@@ -427,28 +432,28 @@ __global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlo
     float aq[1][NT][4], ak[1][NT][4];
     zero(aq);
     zero(ak);
-    auto fs = [&](int k, int n) { return s.s[k * LDX + n]; };
-    warp_mma<X, false, SP>(ak, m0, n0, 0, KP, [&](int m, int k) { return ldf(sk + m * LDK + k); }, fs);
-    warp_mma<X, false, SP>(aq, m0, n0, 0, KP, [&](int m, int k) { return ldf(sq + m * LDK + k); }, fs);
+    auto fs = [&](int k, int n) { return column<LDX>(s.s + k * LDX + n); };
+    warp_mma<X, !SP, SP>(ak, m0, n0, 0, KP, [&](int m, int k) { return pair(sk + m * LDK + k); }, fs);
+    warp_mma<X, !SP, SP>(aq, m0, n0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); }, fs);
     each_pair(ak, m0, n0, [&](int i, int n, float x, float y) {
       const float b = s.gates.beta[i], e = s.gates.start[i];
       *reinterpret_cast<float2*>(s.x + i * LDX + n) =
-          make_float2(b * (ldf(s.v + i * LDV + n) - e * x), b * (ldf(s.v + i * LDV + n + 1) - e * y));
+          stage2<SP>(b * (ldf(s.v + i * LDV + n) - e * x), b * (ldf(s.v + i * LDV + n + 1) - e * y));
     });
     __syncthreads();
     zero(ak);
-    auto fx = [&](int k, int n) { return s.x[k * LDX + n]; };
-    warp_mma<false, false, SP>(ak, m0, n0, 0, m0 + 16, [&](int m, int k) { return s.t[m * LDC + k]; }, fx);
+    auto fx = [&](int k, int n) { return column<LDX>(s.x + k * LDX + n); };
+    warp_mma<false, !SP, SP>(ak, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDC + k); }, fx);
     __syncthreads();
     each_pair(ak, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(x, y);
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = stage2<SP>(x, y);
     });
     each_pair(aq, m0, n0, [&](int i, int, float& x, float& y) {
       x *= s.gates.start[i];
       y *= s.gates.start[i];
     });
     __syncthreads();
-    warp_mma<false, false, SP>(aq, m0, n0, 0, m0 + 16, [&](int m, int k) { return s.p[m * LDC + k]; }, fx);
+    warp_mma<!SP, !SP, SP>(aq, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.p + m * LDC + k); }, fx);
     each_pair(aq, m0, n0, [&](int i, int n, float x, float y) {
       const int c = v0 + n;
       if (i < rows) {
@@ -460,17 +465,26 @@ __global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlo
   }
 }
 
+template <class TI, int KP, int VB>
+__global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlong2* __restrict__ tab, int VP,
+                                                            const float* __restrict__ tinv,
+                                                            const float* __restrict__ states, TI* __restrict__ o) {
+  output_chunk<TI, KP, VB>(a, tab, VP, tinv, states, o);
+  zero_uncovered(o, a, (int64_t)a.HV * a.V);
+}
+
 template <class TI, int KP>
 int run_fwd(const Args& a, const Plan& p, const Saved& sv, const Work& w, int VP, const float* h0, void* o, float* ht,
-            cudaStream_t st) {
+            bool split, cudaStream_t st) {
   const int64_t items = p.MC * a.HV;
   if (items > 0) {
     const size_t smem = sizeof(PrepSmem<TI, KP>);
-    cudaFuncSetAttribute(prep_kernel<TI, KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    prep_kernel<TI, KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, sv.tinv, sv.pm, sv.s);
+    auto* prep = split ? prep_kernel<TI, KP, true> : prep_kernel<TI, KP, OutSplit<TI>::v>;
+    cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    prep<<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, sv.tinv, sv.pm, sv.s);
     SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   }
-  int rc = run_chain(p, sv, w, sv.s, h0, ht, a.N, a.HV, a.K, a.V, false, st);
+  int rc = run_chain(p, sv, w, sv.s, h0, ht, a.N, a.HV, a.K, a.V, false, split, !OutSplit<TI>::v, st);
   if (rc || a.T == 0) return rc;
   constexpr int VB = KP == 64 ? 64 : 32;
   const size_t smem = sizeof(OutSmem<TI, KP, VB>);
@@ -487,7 +501,7 @@ Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V) {
   p.MC = max_chunks(N, T);
   const int VP = pad_v(V), KP = pad_k(K);
   (void)KP;
-  p.vs = 16;
+  p.vs = 8;
   p.vs_seg = 16;
   while (p.vs < 64 && N * HV * (VP / p.vs) >= 4 * kNumSMs) p.vs *= 2;
   p.len = 0;
@@ -527,13 +541,14 @@ Args make_args(const void* q, const void* k, const void* v, const void* g, const
 }
 
 int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const float* init, float* last, int64_t N,
-              int HV, int K, int V, bool reverse, cudaStream_t st) {
+              int HV, int K, int V, bool reverse, bool split, bool round, cudaStream_t st) {
   ChainArgs c = {};
   c.HV = HV;
   c.K = K;
   c.V = V;
   c.VP = pad_v(V);
   c.reverse = reverse;
+  c.round = round;
   const int KP = pad_k(K);
   c.pm = sv.pm;
   c.b = s;
@@ -543,7 +558,7 @@ int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const flo
     c.off = sv.chunk_off;
     c.init = init;
     c.last = last;
-    return chain(c, KP, p.vs, reverse, N, st);
+    return chain(c, KP, p.vs, reverse, split, N, st);
   }
   // compose the maps of every segment, run along the segments, run inside them
   ChainArgs d = c;
@@ -553,7 +568,7 @@ int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const flo
   d.mseg = w.mseg;
   d.last = w.bseg;
   d.last_padded = true;
-  int rc = chain(d, KP, p.vs_seg, reverse, p.MS, st);
+  int rc = chain(d, KP, p.vs_seg, reverse, split, p.MS, st);
   if (rc) return rc;
   d = c;
   d.pm = w.mseg;
@@ -562,11 +577,12 @@ int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const flo
   d.off = sv.seg_off;
   d.init = init;
   d.last = last;
-  if ((rc = chain(d, KP, 16, false, N, st))) return rc;
+  d.round = false;
+  if ((rc = chain(d, KP, 16, false, split, N, st))) return rc;
   c.seg = sv.seg_tab;
   c.init = w.bseg;
   c.init_padded = true;
-  return chain(c, KP, p.vs_seg, reverse, p.MS, st);
+  return chain(c, KP, p.vs_seg, reverse, split, p.MS, st);
 }
 
 }  // namespace delta
@@ -616,7 +632,9 @@ extern "C" int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, con
                           sv.seg_tab, st);
   if (rc) return rc;
   const Args a = make_args(q, k, v, g, beta, dtype, dtype_g, dtype_beta, cu_seqlens, n_seqs, T, H, HV, K, V, scale);
+  const bool split = state_split(dtype, h0, ht);
   return SSLA_DISPATCH_DTYPE(dtype, T_, [&] {
-    return KP == 64 ? run_fwd<T_, 64>(a, p, sv, w, VP, h0, o, ht, st) : run_fwd<T_, 128>(a, p, sv, w, VP, h0, o, ht, st);
+    return KP == 64 ? run_fwd<T_, 64>(a, p, sv, w, VP, h0, o, ht, split, st)
+                    : run_fwd<T_, 128>(a, p, sv, w, VP, h0, o, ht, split, st);
   });
 }

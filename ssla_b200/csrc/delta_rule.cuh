@@ -22,7 +22,9 @@ namespace ssla {
 namespace delta {
 
 constexpr int BT = 64;            // tokens per chunk
-constexpr int LDC = BT + 4;       // row of a [64, 64] fp32 tile in shared memory
+// Rows of fp32 tiles in shared memory: 8 more than a multiple of 32 where products read pairs along
+// them, 4 more where they read down the columns (no bank conflicts either way).
+constexpr int LDC = BT + 8;       // [64, 64] tiles
 constexpr int THREADS = 256;      // threads of the per-chunk kernels
 constexpr float kMinGate = -200.f;  // exp() of less is 0 in fp32; keeps in-chunk sums finite for g = -inf
 
@@ -120,23 +122,37 @@ __device__ __forceinline__ void st_any(void* p, int dt, size_t i, float x) {
 }
 
 // ------------------------------------------------------------------ tensor-core products
-// Warp-level C += A B on mma.sync m16n8k8 TF32 with fp32 accumulators.  The operands are read
-// through functors fa(row, k), fb(k, col) from shared memory.  A value that came from a 16-bit
-// input is exact in TF32 (AX, BX).  SPLIT: x = hi + lo with hi the TF32 rounding, products
-// hi hi + lo hi + hi lo, about 2^-22 relative; otherwise one product of TF32-rounded operands.
-__device__ __forceinline__ uint32_t tf32_rna(float x) {
+// Warp-level C += A B on mma.sync m16n8k8 TF32 with fp32 accumulators.  Operands come from shared
+// memory through functors that return a pair along the contraction, fa(row, k) = {A[row][k],
+// A[row][k+1]}, fb(k, col) likewise: the order of k inside an MMA is free as long as both agree, so
+// lane t takes k = 2t, 2t + 1 of every 8, one 64-bit (16-bit tiles: 32-bit) load for tiles that are
+// contiguous in k.
+//
+// AX, BX: the operand is exact in TF32 (a value of a 16-bit input, or rounded when it was stored).
+// SPLIT: x = hi + lo with hi the TF32 rounding, hi hi + lo hi + hi lo, about 2^-22 relative; the
+// small products have accumulators of their own, which also shortens the chain of additions that
+// the tensor core truncates.  Without SPLIT one product of TF32-rounded operands.
+__device__ __forceinline__ float tf32(float x) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
+  return __uint_as_float(r);
+}
+// what a tile stores for later products: fp32 for split ones, else the TF32 rounding
+template <bool SPLIT> __device__ __forceinline__ float stage(float x) { return SPLIT ? x : tf32(x); }
+template <bool SPLIT> __device__ __forceinline__ float2 stage2(float x, float y) {
+  return make_float2(stage<SPLIT>(x), stage<SPLIT>(y));
 }
 
 template <bool EXACT, bool SPLIT>
 __device__ __forceinline__ void operand(float x, uint32_t& hi, uint32_t& lo) {
   if (EXACT) {
     hi = __float_as_uint(x);
+  } else if (SPLIT) {
+    // round to nearest by hand, ties away: a NaN or infinity leaves lo NaN, so it is not lost
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
   } else {
-    hi = tf32_rna(x);
-    if (SPLIT) lo = __float_as_uint(x - __uint_as_float(hi));
+    hi = __float_as_uint(tf32(x));
   }
 }
 
@@ -149,30 +165,55 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], cons
 
 template <bool AX, bool BX, bool SPLIT, int MT, int NT, class FA, class FB>
 __device__ __forceinline__ void warp_mma(float (&acc)[MT][NT][4], int m0, int n0, int k0, int k1, FA fa, FB fb) {
+  constexpr bool SMALL = SPLIT && !(AX && BX);
   const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+  float small[SMALL ? MT : 1][SMALL ? NT : 1][4];
+  if (SMALL)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) small[i][j][0] = small[i][j][1] = small[i][j][2] = small[i][j][3] = 0.f;
+#pragma unroll 2
   for (int k = k0; k < k1; k += 8) {
     uint32_t ah[MT][4], al[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      operand<AX, SPLIT>(fa(m0 + 16 * i + g, k + t), ah[i][0], al[i][0]);
-      operand<AX, SPLIT>(fa(m0 + 16 * i + g + 8, k + t), ah[i][1], al[i][1]);
-      operand<AX, SPLIT>(fa(m0 + 16 * i + g, k + t + 4), ah[i][2], al[i][2]);
-      operand<AX, SPLIT>(fa(m0 + 16 * i + g + 8, k + t + 4), ah[i][3], al[i][3]);
+      const float2 x = fa(m0 + 16 * i + g, k + 2 * t), y = fa(m0 + 16 * i + g + 8, k + 2 * t);
+      operand<AX, SPLIT>(x.x, ah[i][0], al[i][0]);
+      operand<AX, SPLIT>(y.x, ah[i][1], al[i][1]);
+      operand<AX, SPLIT>(x.y, ah[i][2], al[i][2]);
+      operand<AX, SPLIT>(y.y, ah[i][3], al[i][3]);
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       uint32_t bh[2], bl[2];
-      operand<BX, SPLIT>(fb(k + t, n0 + 8 * j + g), bh[0], bl[0]);
-      operand<BX, SPLIT>(fb(k + t + 4, n0 + 8 * j + g), bh[1], bl[1]);
+      const float2 z = fb(k + 2 * t, n0 + 8 * j + g);
+      operand<BX, SPLIT>(z.x, bh[0], bl[0]);
+      operand<BX, SPLIT>(z.y, bh[1], bl[1]);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         mma8(acc[i][j], ah[i], bh);
-        if (SPLIT && !AX) mma8(acc[i][j], al[i], bh);
-        if (SPLIT && !BX) mma8(acc[i][j], ah[i], bl);
+        if (SPLIT && !AX) mma8(small[i][j], al[i], bh);
+        if (SPLIT && !BX) mma8(small[i][j], ah[i], bl);
       }
     }
   }
+  if (SMALL)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] += small[i][j][r];
 }
+
+// pairs along a row of a tile (contiguous), and along a column
+__device__ __forceinline__ float2 pair(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 pair(const __nv_bfloat16* p) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+}
+__device__ __forceinline__ float2 pair(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
+template <int LD, class T> __device__ __forceinline__ float2 column(const T* p) { return make_float2(ldf(p), ldf(p + LD)); }
 
 template <int MT, int NT> __device__ __forceinline__ void zero(float (&acc)[MT][NT][4]) {
 #pragma unroll
@@ -288,8 +329,11 @@ template <> struct Io16<float> { static constexpr bool exact = false; };
 // product (2^-11 per operand).  fp16 and fp32 results need the split.
 template <class TI> struct OutSplit { static constexpr bool v = true; };
 template <> struct OutSplit<__nv_bfloat16> { static constexpr bool v = false; };
+// The states themselves: split unless every output that depends on them leaves in bf16, that is
+// bf16 tokens without a final state or a gradient of the initial one.
+inline bool state_split(int dtype, const void* h0, const void* ht) { return dtype != SSLA_BF16 || h0 || ht; }
 
-template <class TI, int KP> struct KTile { static constexpr int LD = KP + (sizeof(TI) == 4 ? 4 : 8); };
+template <class TI, int KP> struct KTile { static constexpr int LD = KP + 8; };
 
 __device__ __forceinline__ bool locate(const longlong2* tab, int64_t MC, int64_t chunk, int64_t& t0, int& rows) {
   if (chunk >= MC) return false;
@@ -318,8 +362,10 @@ Args make_args(const void* q, const void* k, const void* v, const void* g, const
                float scale);
 // The affine chunk maps along every sequence: forward S' = decay S - PM S + B (s: B in, start states
 // out), reverse the adjoint with PM^T (s: dB in, adjoint of every chunk's end state out).
+// split: products at fp32 accuracy; round: the states kept for the per-chunk kernels are rounded to
+// TF32, which is all that their single products read.
 int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const float* init, float* last, int64_t N,
-              int HV, int K, int V, bool reverse, cudaStream_t st);
+              int HV, int K, int V, bool reverse, bool split, bool round, cudaStream_t st);
 
 }  // namespace delta
 }  // namespace ssla

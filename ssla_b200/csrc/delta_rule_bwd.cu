@@ -17,7 +17,7 @@ namespace delta {
 namespace {
 
 template <class TI, int KP> struct AdjSmem {
-  static constexpr int LDK = KTile<TI, KP>::LD, LDW = KP + 8, LDO = 72;
+  static constexpr int LDK = KTile<TI, KP>::LD, LDW = KP + 4, LDO = 72;
   TI k[BT * LDK];
   TI q[BT * LDK];
   TI d[BT * LDO];
@@ -61,30 +61,33 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<TI, KP>) <= 113 * 1024
     float acc[1][4][4];
     zero(acc);
     if (n0 <= m0)
-      warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return ldf(sq + m * LDK + k); },
-                         [&](int k, int n) { return ldf(sk + n * LDK + k); });
+      warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
+                         [&](int k, int n) { return pair(sk + n * LDK + k); });
     each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
-      s.p[i * LDC + j] = i >= j ? s.gates.fade(i, j) * x : 0.f;
-      s.p[i * LDC + j + 1] = i > j ? s.gates.fade(i, j + 1) * y : 0.f;
+      *reinterpret_cast<float2*>(s.p + i * LDC + j) =
+          stage2<SP>(i >= j ? s.gates.fade(i, j) * x : 0.f, i > j ? s.gates.fade(i, j + 1) * y : 0.f);
     });
   }
   float acc[1][NK][4];
   zero(acc);
   warp_mma<false, X, SP>(acc, m0, k0, 0, m0 + 16,
-                         [&](int i, int j) { return s.t[i * LDC + j] * (s.gates.beta[j] * s.gates.start[j]); },
-                         [&](int j, int n) { return ldf(sk + j * LDK + n); });
+                         [&](int i, int j) {
+                           const float2 x = pair(s.t + i * LDC + j), b = pair(s.gates.beta + j), e = pair(s.gates.start + j);
+                           return make_float2(x.x * (b.x * e.x), x.y * (b.y * e.y));
+                         },
+                         [&](int j, int n) { return column<LDK>(sk + j * LDK + n); });
   each_pair(acc, m0, k0, [&](int i, int n, float x, float y) {
-    *reinterpret_cast<float2*>(s.w + i * LDW + n) = make_float2(x, y);
+    *reinterpret_cast<float2*>(s.w + i * LDW + n) = stage2<SP>(x, y);
   });
   __syncthreads();
   zero(acc);
-  warp_mma<false, false, SP>(acc, m0, k0, 0, m0 + 16, [&](int i, int j) { return s.p[i * LDC + j]; },
-                             [&](int j, int n) { return s.w[j * LDW + n]; });
+  warp_mma<!SP, !SP, SP>(acc, m0, k0, 0, m0 + 16, [&](int i, int j) { return pair(s.p + i * LDC + j); },
+                         [&](int j, int n) { return column<LDW>(s.w + j * LDW + n); });
   __syncthreads();
   each_pair(acc, m0, k0, [&](int i, int n, float x, float y) {
     const float e = s.gates.start[i];
     *reinterpret_cast<float2*>(s.w + i * LDW + n) =
-        make_float2(a.scale * (e * ldf(sq + i * LDK + n) - x), a.scale * (e * ldf(sq + i * LDK + n + 1) - y));
+        stage2<SP>(a.scale * (e * ldf(sq + i * LDK + n) - x), a.scale * (e * ldf(sq + i * LDK + n + 1) - y));
   });
   constexpr int MT = KP / 64;
   const int mk = (warp >> 1) * 16 * MT;
@@ -98,8 +101,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<TI, KP>) <= 113 * 1024
     __syncthreads();
     float db[MT][4][4];
     zero(db);
-    warp_mma<false, X, SP>(db, mk, n0, 0, BT, [&](int m, int j) { return s.w[j * LDW + m]; },
-                           [&](int j, int n) { return ldf(s.d + j * LDO + n); });
+    warp_mma<!SP, X, SP>(db, mk, n0, 0, BT, [&](int m, int j) { return column<LDW>(s.w + j * LDW + m); },
+                         [&](int j, int n) { return column<LDO>(s.d + j * LDO + n); });
     each_pair(db, mk, n0, [&](int m, int n, float x, float y) {
       *reinterpret_cast<float2*>(ds + (item * KP + m) * VP + v0 + n) = make_float2(x, y);
     });
@@ -107,46 +110,35 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<TI, KP>) <= 113 * 1024
 }
 
 template <class TI, int KP> struct BwdSmem {
-  static constexpr int VB = 32, LDK = KTile<TI, KP>::LD, LDO = VB + (sizeof(TI) == 4 ? 4 : 8), LDX = VB + 4;
+  // p and t, s and e are read both along rows and down columns: one of the two conflicts either way
+  static constexpr int VB = 32, LDK = KTile<TI, KP>::LD, LDO = VB + 8, LDX = VB + 8, LDS = VB + 4, LDP = BT + 4;
   TI k[BT * LDK];
   TI q[BT * LDK];
   TI d[BT * LDO];
-  float p[BT * LDC];  // P, then dP
-  float t[BT * LDC];  // T, then E
+  float p[BT * LDP];  // P, then dP
+  float t[BT * LDP];  // T, then E
   float x[BT * LDX];  // beta X, then U
   float f[BT * LDX];  // dU, then F
-  float s[KP * LDX];
-  float e[KP * LDX];  // D
+  float s[KP * LDS];
+  float e[KP * LDS];  // D
   float red[6][2][BT];
   float dots[THREADS / 32];
   Gates gates;
 };
 
 template <class TI, int KP>
-__global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024 ? 2 : 1)
-    backward_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
-                    const float* __restrict__ states, const float* __restrict__ ds, const TI* __restrict__ dout,
-                    TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv, void* __restrict__ dg,
-                    void* __restrict__ dbeta, float* __restrict__ dqk) {
+__device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* __restrict__ tab, int VP,
+                                               const float* __restrict__ tinv, const float* __restrict__ states,
+                                               const float* __restrict__ ds, const TI* __restrict__ dout,
+                                               TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv,
+                                               void* __restrict__ dg, void* __restrict__ dbeta,
+                                               float* __restrict__ dqk) {
   using S = BwdSmem<TI, KP>;
   constexpr bool X = Io16<TI>::exact, SP = OutSplit<TI>::v;
-  constexpr int VB = S::VB, LDK = S::LDK, LDO = S::LDO, LDX = S::LDX, NT = VB / 16, NK = KP / 16;
+  constexpr int VB = S::VB, LDK = S::LDK, LDO = S::LDO, LDX = S::LDX, LDS = S::LDS, LDP = S::LDP, NT = VB / 16, NK = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
   const size_t TK = (size_t)a.T * a.HV * a.K;
-  if (dqk) {
-    zero_uncovered(dqk, a, (int64_t)a.HV * a.K);
-    zero_uncovered(dqk + TK, a, (int64_t)a.HV * a.K);
-  } else {
-    zero_uncovered(dq, a, (int64_t)a.H * a.K);
-    zero_uncovered(dk, a, (int64_t)a.H * a.K);
-  }
-  zero_uncovered(dv, a, (int64_t)a.HV * a.V);
-  if (a.dt_g == SSLA_F32) zero_uncovered((float*)dg, a, a.HV);
-  else zero_uncovered((__half*)dg, a, a.HV);  // 0 has the same bits in both 16-bit types
-  if (a.dt_b == SSLA_F32) zero_uncovered((float*)dbeta, a, a.HV);
-  else zero_uncovered((__half*)dbeta, a, a.HV);
-
   const int64_t chunk = blockIdx.x / a.HV;
   const int hv = (int)(blockIdx.x - chunk * a.HV), h = hv / a.R;
   const size_t item = blockIdx.x;
@@ -157,7 +149,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
   const size_t qk = ((size_t)t0 * a.H + h) * a.K;
   load_rows<TI, LDK, KP>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   load_rows<TI, LDK, KP>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
-  load_f32<LDC, BT, BT>(s.t, tinv + item * (BT * BT), BT);
+  load_f32<LDP, BT, BT>(s.t, tinv + item * (BT * BT), BT);
   cp_commit();
   if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
   const TI *sk = s.k, *sq = s.q, *sd = s.d;
@@ -165,8 +157,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
   const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
   const TI* gv = (const TI*)a.v + vo;
-  auto fk_row = [&](int m, int k) { return ldf(sk + m * LDK + k); };
-  auto fx = [&](int k, int n) { return s.x[k * LDX + n]; };
+  auto fk_row = [&](int m, int k) { return pair(sk + m * LDK + k); };
+  auto fx = [&](int k, int n) { return column<LDX>(s.x + k * LDX + n); };
 
   float aq[1][NK][4], ar[1][NK][4], ac[1][NK][4];  // dO S^T, F S^T, U D^T
   float ap[1][4][4], ae[1][4][4];                  // dO U^T, F U^T
@@ -176,8 +168,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
   const bool low = p0 <= m0;
   for (int v0 = 0; v0 < a.V; v0 += VB) {
     __syncthreads();
-    load_f32<LDX, KP, VB>(s.s, states + item * KP * VP + v0, VP);
-    load_f32<LDX, KP, VB>(s.e, ds + item * KP * VP + v0, VP);
+    load_f32<LDS, KP, VB>(s.s, states + item * KP * VP + v0, VP);
+    load_f32<LDS, KP, VB>(s.e, ds + item * KP * VP + v0, VP);
     load_rows<TI, LDO, VB>(s.d, dout + vo + v0, vstride, rows, a.V - v0, vec_d);
     cp_commit();
     if (v0 == 0) {
@@ -186,11 +178,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
       float acc[1][4][4];
       zero(acc);
       if (low)
-        warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return ldf(sq + m * LDK + k); },
-                           [&](int k, int n) { return ldf(sk + n * LDK + k); });
+        warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
+                           [&](int k, int n) { return pair(sk + n * LDK + k); });
       each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
-        s.p[i * LDC + j] = i >= j ? s.gates.fade(i, j) * x : 0.f;
-        s.p[i * LDC + j + 1] = i > j ? s.gates.fade(i, j + 1) * y : 0.f;
+        *reinterpret_cast<float2*>(s.p + i * LDP + j) =
+            stage2<SP>(i >= j ? s.gates.fade(i, j) * x : 0.f, i > j ? s.gates.fade(i, j + 1) * y : 0.f);
       });
     }
     float xv[1][NT][4];
@@ -204,8 +196,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
     float ks[1][NT][4], du[1][NT][4];
     zero(ks);
     zero(du);
-    warp_mma<X, false, SP>(ks, m0, n0, 0, KP, fk_row, [&](int k, int n) { return s.s[k * LDX + n]; });
-    warp_mma<X, false, SP>(du, m0, n0, 0, KP, fk_row, [&](int k, int n) { return s.e[k * LDX + n]; });
+    warp_mma<X, !SP, SP>(ks, m0, n0, 0, KP, fk_row, [&](int k, int n) { return column<LDS>(s.s + k * LDS + n); });
+    warp_mma<X, !SP, SP>(du, m0, n0, 0, KP, fk_row, [&](int k, int n) { return column<LDS>(s.e + k * LDS + n); });
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -216,22 +208,22 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
       }
     each_pair(xv, m0, n0, [&](int i, int n, float x, float y) {
       const float b = s.gates.beta[i];
-      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(b * x, b * y);
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = stage2<SP>(b * x, b * y);
     });
     for (int i = tid; i < KP * (VB / 4); i += THREADS) {
       const int r = i / (VB / 4), c = (i % (VB / 4)) * 4;
-      const float4 x = *reinterpret_cast<const float4*>(s.s + r * LDX + c);
-      const float4 y = *reinterpret_cast<const float4*>(s.e + r * LDX + c);
+      const float4 x = *reinterpret_cast<const float4*>(s.s + r * LDS + c);
+      const float4 y = *reinterpret_cast<const float4*>(s.e + r * LDS + c);
       dot += x.x * y.x + x.y * y.y + x.z * y.z + x.w * y.w;
     }
     __syncthreads();
     zero(ks);
-    warp_mma<false, false, SP>(ks, m0, n0, 0, m0 + 16, [&](int m, int k) { return s.t[m * LDC + k]; }, fx);  // U
+    warp_mma<false, !SP, SP>(ks, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDP + k); }, fx);  // U
     {
       float pd[1][NT][4];
       zero(pd);
-      warp_mma<false, X, SP>(pd, m0, n0, m0, BT, [&](int m, int k) { return s.p[k * LDC + m]; },
-                             [&](int k, int n) { return ldf(sd + k * LDO + n); });
+      warp_mma<!SP, X, SP>(pd, m0, n0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
+                           [&](int k, int n) { return column<LDO>(sd + k * LDO + n); });
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -239,15 +231,15 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
     }
     __syncthreads();
     each_pair(ks, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(x, y);
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = stage2<SP>(x, y);
     });
     each_pair(du, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.f + i * LDX + n) = make_float2(x, y);
+      *reinterpret_cast<float2*>(s.f + i * LDX + n) = stage2<SP>(x, y);
     });
     __syncthreads();
     zero(du);
-    warp_mma<false, false, SP>(du, m0, n0, m0, BT, [&](int m, int k) { return s.t[k * LDC + m]; },
-                               [&](int k, int n) { return s.f[k * LDX + n]; });  // F
+    warp_mma<false, !SP, SP>(du, m0, n0, m0, BT, [&](int m, int k) { return column<LDP>(s.t + k * LDP + m); },
+                             [&](int k, int n) { return column<LDX>(s.f + k * LDX + n); });  // F
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       rb[0] += du[0][j][0] * xv[0][j][0] + du[0][j][1] * xv[0][j][1];
@@ -264,34 +256,34 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
     });
     __syncthreads();
     each_pair(du, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.f + i * LDX + n) = make_float2(x, y);
+      *reinterpret_cast<float2*>(s.f + i * LDX + n) = stage2<SP>(x, y);
     });
     __syncthreads();
-    auto ff = [&](int m, int k) { return s.f[m * LDX + k]; };
-    auto fd = [&](int m, int k) { return ldf(sd + m * LDO + k); };
-    auto fu_t = [&](int k, int n) { return s.x[n * LDX + k]; };
-    auto fs_t = [&](int k, int n) { return s.s[n * LDX + k]; };
+    auto ff = [&](int m, int k) { return pair(s.f + m * LDX + k); };
+    auto fd = [&](int m, int k) { return pair(sd + m * LDO + k); };
+    auto fu_t = [&](int k, int n) { return pair(s.x + n * LDX + k); };
+    auto fs_t = [&](int k, int n) { return pair(s.s + n * LDS + k); };
     if (low) {
-      warp_mma<X, false, SP>(ap, m0, p0, 0, VB, fd, fu_t);
-      warp_mma<false, false, SP>(ae, m0, p0, 0, VB, ff, fu_t);
+      warp_mma<X, !SP, SP>(ap, m0, p0, 0, VB, fd, fu_t);
+      warp_mma<!SP, !SP, SP>(ae, m0, p0, 0, VB, ff, fu_t);
     }
-    warp_mma<X, false, SP>(aq, m0, k0, 0, VB, fd, fs_t);
-    warp_mma<false, false, SP>(ar, m0, k0, 0, VB, ff, fs_t);
-    warp_mma<false, false, SP>(ac, m0, k0, 0, VB, [&](int m, int k) { return s.x[m * LDX + k]; },
-                               [&](int k, int n) { return s.e[n * LDX + k]; });
+    warp_mma<X, !SP, SP>(aq, m0, k0, 0, VB, fd, fs_t);
+    warp_mma<!SP, !SP, SP>(ar, m0, k0, 0, VB, ff, fs_t);
+    warp_mma<!SP, !SP, SP>(ac, m0, k0, 0, VB, [&](int m, int k) { return pair(s.x + m * LDX + k); },
+                           [&](int k, int n) { return pair(s.e + n * LDS + k); });
   }
   __syncthreads();
   // dP and E take the places of P and T
   each_pair(ap, m0, p0, [&](int i, int j, float x, float y) {
-    s.p[i * LDC + j] = i >= j ? a.scale * s.gates.fade(i, j) * x : 0.f;
-    s.p[i * LDC + j + 1] = i > j ? a.scale * s.gates.fade(i, j + 1) * y : 0.f;
+    *reinterpret_cast<float2*>(s.p + i * LDP + j) = stage2<SP>(
+        i >= j ? a.scale * s.gates.fade(i, j) * x : 0.f, i > j ? a.scale * s.gates.fade(i, j + 1) * y : 0.f);
   });
   each_pair(ae, m0, p0, [&](int i, int j, float x, float y) {
-    s.t[i * LDC + j] = i > j ? s.gates.fade(i, j) * x : 0.f;
-    s.t[i * LDC + j + 1] = i > j + 1 ? s.gates.fade(i, j + 1) * y : 0.f;
+    *reinterpret_cast<float2*>(s.t + i * LDP + j) =
+        stage2<SP>(i > j ? s.gates.fade(i, j) * x : 0.f, i > j + 1 ? s.gates.fade(i, j + 1) * y : 0.f);
   });
   __syncthreads();
-  auto fk_tok = [&](int k, int n) { return ldf(sk + k * LDK + n); };
+  auto fk_tok = [&](int k, int n) { return column<LDK>(sk + k * LDK + n); };
   const int i0 = m0 + (lane >> 2);
   float rl[2] = {0.f, 0.f}, rq[2] = {0.f, 0.f}, rr[2] = {0.f, 0.f}, rc[2] = {0.f, 0.f}, rg[2] = {0.f, 0.f};
   // sums over an accumulator's columns of tile * accumulator, per row
@@ -306,7 +298,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
   {
     float ag[1][NK][4];
     zero(ag);
-    warp_mma<false, X, SP>(ag, m0, k0, 0, m0 + 16, [&](int m, int k) { return s.t[m * LDC + k]; }, fk_tok);
+    warp_mma<!SP, X, SP>(ag, m0, k0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDP + k); }, fk_tok);
     row_dot(ag, sk, rg);
 #pragma unroll
     for (int j = 0; j < NK; ++j)
@@ -321,11 +313,16 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
   }
   row_dot(ar, sk, rr);
   row_dot(ac, sk, rl);
-  warp_mma<false, X, SP>(aq, m0, k0, 0, m0 + 16, [&](int m, int k) { return s.p[m * LDC + k]; }, fk_tok);
+  warp_mma<!SP, X, SP>(aq, m0, k0, 0, m0 + 16, [&](int m, int k) { return pair(s.p + m * LDP + k); }, fk_tok);
   row_dot(aq, sq, rq);
-  warp_mma<false, X, SP>(ac, m0, k0, m0, BT, [&](int m, int k) { return s.p[k * LDC + m]; },
-                         [&](int k, int n) { return ldf(sq + k * LDK + n); });
-  warp_mma<false, X, SP>(ac, m0, k0, m0, BT, [&](int m, int k) { return -s.gates.beta[k] * s.t[k * LDC + m]; }, fk_tok);
+  warp_mma<!SP, X, SP>(ac, m0, k0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
+                       [&](int k, int n) { return column<LDK>(sq + k * LDK + n); });
+  warp_mma<false, X, SP>(ac, m0, k0, m0, BT,
+                         [&](int m, int k) {
+                           const float2 x = column<LDP>(s.t + k * LDP + m), b = pair(s.gates.beta + k);
+                           return make_float2(-b.x * x.x, -b.y * x.y);
+                         },
+                         fk_tok);
   row_dot(ac, sk, rc);
   const size_t qo = dqk ? ((size_t)t0 * a.HV + hv) * a.K : qk, qstride = (size_t)(dqk ? a.HV : a.H) * a.K;
   auto put = [&](size_t at, int c, float x, float y, TI* out, float* part) {
@@ -394,19 +391,54 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024
   if (2 * lane + 1 < rows) st_any(dg, a.dt_g, at + a.HV, suf - gc[0] + sum);
 }
 
-// dq, dk [T, H, K] = sums over the value heads of a key head, in their order.
+template <class TI, int KP>
+__global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024 ? 2 : 1)
+    backward_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
+                    const float* __restrict__ states, const float* __restrict__ ds, const TI* __restrict__ dout,
+                    TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv, void* __restrict__ dg,
+                    void* __restrict__ dbeta, float* __restrict__ dqk) {
+  backward_chunk<TI, KP>(a, tab, VP, tinv, states, ds, dout, dq, dk, dv, dg, dbeta, dqk);
+  const size_t TK = (size_t)a.T * a.HV * a.K;
+  if (dqk) {
+    zero_uncovered(dqk, a, (int64_t)a.HV * a.K);
+    zero_uncovered(dqk + TK, a, (int64_t)a.HV * a.K);
+  } else {
+    zero_uncovered(dq, a, (int64_t)a.H * a.K);
+    zero_uncovered(dk, a, (int64_t)a.H * a.K);
+  }
+  zero_uncovered(dv, a, (int64_t)a.HV * a.V);
+  if (a.dt_g == SSLA_F32) zero_uncovered((float*)dg, a, a.HV);
+  else zero_uncovered((__half*)dg, a, a.HV);  // 0 has the same bits in both 16-bit types
+  if (a.dt_b == SSLA_F32) zero_uncovered((float*)dbeta, a, a.HV);
+  else zero_uncovered((__half*)dbeta, a, a.HV);
+}
+
+// dq, dk [T, H, K] = sums over the value heads of a key head, in their order.  One warp a row of K.
 template <class TI>
-__global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ dqk, int64_t T, int H, int R, int K,
+__global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ dqk, int64_t TH, int R, int K,
                                                         TI* __restrict__ dq, TI* __restrict__ dk) {
-  const int64_t n = T * H * K;
-  const float* p = dqk + (blockIdx.y ? n * R : 0);
+  const float* p = dqk + (blockIdx.y ? (size_t)TH * R * K : 0);
   TI* out = blockIdx.y ? dk : dq;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t th = i / K;
-    const int k = (int)(i - th * K);
-    float x = 0.f;
-    for (int r = 0; r < R; ++r) x += p[(th * R + r) * K + k];
-    stf(out + i, x);
+  const int lane = threadIdx.x & 31;
+  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < TH; row += (int64_t)gridDim.x * 8) {
+    const float* src = p + (size_t)row * R * K;
+    if (K % 4 == 0) {
+      for (int c = lane * 4; c < K; c += 128) {
+        float4 x = *reinterpret_cast<const float4*>(src + c);
+        for (int r = 1; r < R; ++r) {
+          const float4 y = *reinterpret_cast<const float4*>(src + (size_t)r * K + c);
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
+        const float v[4] = {x.x, x.y, x.z, x.w};
+        Vec<TI, 4>::store(out + (size_t)row * K + c, v);
+      }
+    } else {
+      for (int c = lane; c < K; c += 32) {
+        float x = src[c];
+        for (int r = 1; r < R; ++r) x += src[(size_t)r * K + c];
+        stf(out + (size_t)row * K + c, x);
+      }
+    }
   }
 }
 
@@ -430,7 +462,7 @@ int run_bwd(const Args& a, const Plan& p, const Saved& sv, const Work& w, int VP
                                 : run_adjoint<TI, KP, OutSplit<TI>::v>(a, sv, VP, dout, w.ds, items, st);
     if (rc) return rc;
   }
-  rc = run_chain(p, sv, w, w.ds, dht, dh0, a.N, a.HV, a.K, a.V, true, st);
+  rc = run_chain(p, sv, w, w.ds, dht, dh0, a.N, a.HV, a.K, a.V, true, OutSplit<TI>::v || dh0, !OutSplit<TI>::v, st);
   if (rc || a.T == 0) return rc;
   float* dqk = a.R > 1 ? w.dqk : nullptr;
   const size_t smem = sizeof(BwdSmem<TI, KP>);
@@ -439,10 +471,9 @@ int run_bwd(const Args& a, const Plan& p, const Saved& sv, const Work& w, int VP
       a, sv.chunk_tab, VP, sv.tinv, sv.s, w.ds, (const TI*)dout, (TI*)dq, (TI*)dk, (TI*)dv, dg, dbeta, dqk);
   SSLA_CHECK_LAUNCH("gated_delta_rule backward");
   if (dqk) {
-    const int64_t n = a.T * a.H * a.K;
-    const int64_t blocks = (n + 255) / 256;
-    sum_heads_kernel<TI><<<dim3((unsigned)(blocks < 8 * kNumSMs ? blocks : 8 * kNumSMs), 2), 256, 0, st>>>(
-        dqk, a.T, a.H, a.R, a.K, (TI*)dq, (TI*)dk);
+    const int64_t blocks = (a.T * a.H + 7) / 8;
+    sum_heads_kernel<TI><<<dim3((unsigned)(blocks < 16 * kNumSMs ? blocks : 16 * kNumSMs), 2), 256, 0, st>>>(
+        dqk, a.T * a.H, a.R, a.K, (TI*)dq, (TI*)dk);
     SSLA_CHECK_LAUNCH("gated_delta_rule sum_heads");
   }
   return SSLA_OK;

@@ -17,20 +17,19 @@ namespace {
 
 constexpr int RWARPS = 4;
 
-template <class TI, int KP, bool VEC>
-__global__ void __launch_bounds__(RWARPS * 32) recurrent_kernel(Args a, const float* __restrict__ h0, TI* __restrict__ o,
-                                                                float* __restrict__ ht) {
-  constexpr int KR = KP / 4, LD = KR + 4;  // the pad keeps the four row groups on different banks
-  __shared__ __align__(16) float tok[RWARPS][2][4 * LD];
-  zero_uncovered(o, a, (int64_t)a.HV * a.V);
+template <class TI, int KP, int RG, bool VEC>
+__device__ __forceinline__ void recurrent_warp(const Args& a, const float* __restrict__ h0, TI* __restrict__ o,
+                                               float* __restrict__ ht, float* tok) {
+  constexpr int KR = KP / RG, LD = KR + 4;  // the pad keeps the row groups on different banks
+  constexpr int CL = 32 / RG, COLS = 4 * CL;  // lanes of a row, columns of a warp
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int slices = (a.V + 31) / 32;
-  const int64_t warp = (int64_t)blockIdx.x * RWARPS + wid;
-  const int64_t sh = warp / slices;
-  if (sh >= a.N * a.HV) return;
-  const int64_t seq = sh / a.HV;
+  const unsigned slices = (unsigned)(a.V + COLS - 1) / COLS;
+  const unsigned warp = blockIdx.x * RWARPS + wid;
+  const unsigned sh = warp / slices;
+  if (sh >= (unsigned)(a.N * a.HV)) return;
+  const unsigned seq = sh / (unsigned)a.HV;
   const int hv = (int)(sh - seq * a.HV), h = hv / a.R;
-  const int r = lane >> 3, col = (int)(warp - sh * slices) * 32 + (lane & 7) * 4;
+  const int r = lane / CL, col = (int)(warp - sh * slices) * COLS + (lane % CL) * 4;
   int64_t t0 = a.cu[seq], t1 = a.cu[seq + 1];
   t0 = t0 < 0 ? 0 : (t0 > a.T ? a.T : t0);
   t1 = t1 < t0 ? t0 : (t1 > a.T ? a.T : t1);
@@ -55,8 +54,8 @@ __global__ void __launch_bounds__(RWARPS * 32) recurrent_kernel(Args a, const fl
       }
     }
   }
-  float* sk = tok[wid][0];
-  float* sq = tok[wid][1];
+  float* sk = tok;
+  float* sq = tok + RG * LD;
   for (int64_t t = t0; t < t1; ++t) {
     const size_t kb = ((size_t)t * a.H + h) * a.K, vb = ((size_t)t * a.HV + hv) * a.V + col;
     float kq = 0.f;
@@ -95,7 +94,7 @@ __global__ void __launch_bounds__(RWARPS * 32) recurrent_kernel(Args a, const fl
         }
     }
 #pragma unroll
-    for (int m = 8; m <= 16; m <<= 1)
+    for (int m = CL; m <= 16; m <<= 1)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         pk[c] += __shfl_xor_sync(0xffffffffu, pk[c], m);
@@ -144,13 +143,22 @@ __global__ void __launch_bounds__(RWARPS * 32) recurrent_kernel(Args a, const fl
   }
 }
 
-template <class TI, int KP>
+template <class TI, int KP, int RG, bool VEC>
+__global__ void __launch_bounds__(RWARPS * 32) recurrent_kernel(Args a, const float* __restrict__ h0, TI* __restrict__ o,
+                                                                float* __restrict__ ht) {
+  __shared__ __align__(16) float tok[RWARPS][2 * RG * (KP / RG + 4)];
+  recurrent_warp<TI, KP, RG, VEC>(a, h0, o, ht, tok[threadIdx.x >> 5]);
+  zero_uncovered(o, a, (int64_t)a.HV * a.V);
+}
+
+template <class TI, int KP, int RG>
 int launch(const Args& a, const float* h0, void* o, float* ht, cudaStream_t st) {
-  const int64_t warps = a.N * a.HV * ((a.V + 31) / 32);
+  constexpr int COLS = 128 / RG;
+  const int64_t warps = a.N * a.HV * ((a.V + COLS - 1) / COLS);
   const unsigned grid = (unsigned)((warps + RWARPS - 1) / RWARPS);
   const bool vec = a.V % 4 == 0 && aligned_to(h0, 16) && aligned_to(ht, 16) && aligned_to(o, 4 * sizeof(TI));
-  if (vec) recurrent_kernel<TI, KP, true><<<grid ? grid : 1, RWARPS * 32, 0, st>>>(a, h0, (TI*)o, ht);
-  else recurrent_kernel<TI, KP, false><<<grid ? grid : 1, RWARPS * 32, 0, st>>>(a, h0, (TI*)o, ht);
+  if (vec) recurrent_kernel<TI, KP, RG, true><<<grid ? grid : 1, RWARPS * 32, 0, st>>>(a, h0, (TI*)o, ht);
+  else recurrent_kernel<TI, KP, RG, false><<<grid ? grid : 1, RWARPS * 32, 0, st>>>(a, h0, (TI*)o, ht);
   SSLA_CHECK_LAUNCH("ssla_recurrent_gated_delta_rule_fwd");
   return SSLA_OK;
 }
@@ -174,7 +182,7 @@ extern "C" int ssla_recurrent_gated_delta_rule_fwd(const void* q, const void* k,
                  (long long)H);
   SSLA_CHECK_ARG(K >= 1 && V >= 1 && K <= 128 && V <= 256, "%s: K=%lld V=%lld not supported (1 <= K <= 128, 1 <= V <= 256)",
                  name, (long long)K, (long long)V);
-  SSLA_CHECK_ARG(n_seqs < (int64_t(1) << 31) && n_seqs * HV < (int64_t(1) << 30), "%s: too many states (%lld x %lld)",
+  SSLA_CHECK_ARG(n_seqs < (int64_t(1) << 28) && n_seqs * HV < (int64_t(1) << 28), "%s: too many states (%lld x %lld)",
                  name, (long long)n_seqs, (long long)HV);
   if (HV == 0) return SSLA_OK;
   SSLA_CHECK_ARG(cu_seqlens, "%s: null cu_seqlens", name);
@@ -183,9 +191,9 @@ extern "C" int ssla_recurrent_gated_delta_rule_fwd(const void* q, const void* k,
   cudaStream_t st = (cudaStream_t)stream;
   const Args a = make_args(q, k, v, g, beta, dtype, dtype_g, dtype_beta, cu_seqlens, n_seqs, T, H, HV, K, V, scale);
   return SSLA_DISPATCH_DTYPE(dtype, T_, [&] {
-    if (K <= 16) return launch<T_, 16>(a, h0, o, ht, st);
-    if (K <= 32) return launch<T_, 32>(a, h0, o, ht, st);
-    if (K <= 64) return launch<T_, 64>(a, h0, o, ht, st);
-    return launch<T_, 128>(a, h0, o, ht, st);
+    if (K <= 16) return launch<T_, 16, 4>(a, h0, o, ht, st);
+    if (K <= 32) return launch<T_, 32, 4>(a, h0, o, ht, st);
+    if (K <= 64) return launch<T_, 64, 4>(a, h0, o, ht, st);
+    return launch<T_, 128, 8>(a, h0, o, ht, st);
   });
 }

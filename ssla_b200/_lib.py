@@ -5,6 +5,7 @@ on a CUDA device the call raises; there is no CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 from pathlib import Path
@@ -131,6 +132,19 @@ def ptr(t):
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """Context with ``dev`` current; free when it already is (a decoding step is bound by the host)."""
+    return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def raw_stream(dev: torch.device) -> int:
+    """``stream_of`` without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def require_cuda(*ts, what: str = "ssla_b200") -> None:

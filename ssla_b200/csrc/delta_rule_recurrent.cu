@@ -3,8 +3,9 @@
 //
 // A single token is bound by HBM: the fp32 state [K, V] is read and written once, the token's
 // vectors are small.  One warp owns a 32-column slice of one (sequence, value head) state: lane
-// 8 r + c keeps rows [r KP/4, (r+1) KP/4) of columns [4c, 4c+4) as float4 registers, so every load
-// of a warp takes four whole 128-byte row pieces and all of a slice's loads are in flight at once.
+// 8 r + c keeps rows r, r + 4, ... of columns [4c, 4c+4) as float4 registers, so every load of a
+// warp takes four neighbouring 128-byte row pieces (rows a quarter of K apart: 5% slower at K = 32)
+// and all of a slice's loads are in flight at once.
 // Both products with the state are formed in one pass over the registers before the update,
 //   S_new^T q = exp(g) S^T q + (k.q) u,
 // which leaves one reduction over the four row groups per token (two shuffles) in the token's
@@ -15,12 +16,14 @@ namespace ssla {
 namespace delta {
 namespace {
 
-constexpr int RWARPS = 4;
+constexpr int RWARPS = 2;  // small blocks leave their place to the next one early: 4 warps 2-5% slower
 
 template <class TI, int KP, int RG, bool VEC>
 __device__ __forceinline__ void recurrent_warp(const Args& a, const float* __restrict__ h0, TI* __restrict__ o,
                                                float* __restrict__ ht, float* tok) {
   constexpr int KR = KP / RG, LD = KR + 4;  // the pad keeps the row groups on different banks
+  constexpr bool STREAM = KP > 64;  // evict-first: 198 us against 225 for 8192 states of 128 x 128, but 418
+                                    // against 394 for 262144 of 32 x 32
   constexpr int CL = 32 / RG, COLS = 4 * CL;  // lanes of a row, columns of a warp
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const unsigned slices = (unsigned)(a.V + COLS - 1) / COLS;
@@ -38,13 +41,14 @@ __device__ __forceinline__ void recurrent_warp(const Args& a, const float* __res
   const size_t base = (size_t)sh * a.K * a.V + col;
 #pragma unroll
   for (int i = 0; i < KR; ++i) {
-    const int row = r * KR + i;
+    const int row = RG * i + r;
     S[i][0] = S[i][1] = S[i][2] = S[i][3] = 0.f;
     if (h0 && row < a.K) {
       const float* p = h0 + base + (size_t)row * a.V;
       if (VEC) {
         if (col < a.V) {
-          const float4 x = __ldcs(reinterpret_cast<const float4*>(p));
+          const float4* q4 = reinterpret_cast<const float4*>(p);
+          const float4 x = STREAM ? __ldcs(q4) : __ldg(q4);
           S[i][0] = x.x; S[i][1] = x.y; S[i][2] = x.z; S[i][3] = x.w;
         }
       } else {
@@ -67,7 +71,7 @@ __device__ __forceinline__ void recurrent_warp(const Args& a, const float* __res
         x = ldf((const TI*)a.k + kb + i);
         y = ldf((const TI*)a.q + kb + i);
       }
-      const int at = (i / KR) * LD + i % KR;
+      const int at = (i % RG) * LD + i / RG;
       sk[at] = x;
       sq[at] = y;
       kq = fmaf(x, y, kq);
@@ -130,11 +134,15 @@ __device__ __forceinline__ void recurrent_warp(const Args& a, const float* __res
   if (!ht) return;
 #pragma unroll
   for (int i = 0; i < KR; ++i) {
-    const int row = r * KR + i;
+    const int row = RG * i + r;
     if (row >= a.K) continue;
     float* p = ht + base + (size_t)row * a.V;
     if (VEC) {
-      if (col < a.V) __stcs(reinterpret_cast<float4*>(p), make_float4(S[i][0], S[i][1], S[i][2], S[i][3]));
+      const float4 x = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
+      if (col < a.V) {
+        if (STREAM) __stcs(reinterpret_cast<float4*>(p), x);
+        else *reinterpret_cast<float4*>(p) = x;
+      }
     } else {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
@@ -143,8 +151,10 @@ __device__ __forceinline__ void recurrent_warp(const Args& a, const float* __res
   }
 }
 
+// Resident blocks: as many as the state's registers leave (14 blocks at K = 32 keep 112 KB of loads in
+// flight; fewer registers spill, fewer blocks lose 4-15%).
 template <class TI, int KP, int RG, bool VEC>
-__global__ void __launch_bounds__(RWARPS * 32) recurrent_kernel(Args a, const float* __restrict__ h0, TI* __restrict__ o,
+__global__ void __launch_bounds__(RWARPS * 32, KP <= 32 ? 14 : KP == 64 ? 8 : 4) recurrent_kernel(Args a, const float* __restrict__ h0, TI* __restrict__ o,
                                                                 float* __restrict__ ht) {
   __shared__ __align__(16) float tok[RWARPS][2 * RG * (KP / RG + 4)];
   recurrent_warp<TI, KP, RG, VEC>(a, h0, o, ht, tok[threadIdx.x >> 5]);
@@ -194,6 +204,6 @@ extern "C" int ssla_recurrent_gated_delta_rule_fwd(const void* q, const void* k,
     if (K <= 16) return launch<T_, 16, 4>(a, h0, o, ht, st);
     if (K <= 32) return launch<T_, 32, 4>(a, h0, o, ht, st);
     if (K <= 64) return launch<T_, 64, 4>(a, h0, o, ht, st);
-    return launch<T_, 128, 8>(a, h0, o, ht, st);
+    return launch<T_, 128, 4>(a, h0, o, ht, st);
   });
 }

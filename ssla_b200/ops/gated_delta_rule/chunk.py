@@ -86,11 +86,11 @@ def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
     states = torch.empty(nb, device=dev, dtype=torch.uint8)
     wb = L.ssla_gated_delta_rule_workspace_bytes(N, T, H, HV, K, V, 0)
     ws = torch.empty(wb, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.check(
             L.ssla_chunk_gated_delta_rule_fwd(
                 *tensor_args(q, k, v, g, beta, cu, scale), _lib.ptr(h0), o.data_ptr(), _lib.ptr(ht),
-                states.data_ptr(), nb, ws.data_ptr(), wb, _lib.stream_of(q),
+                states.data_ptr(), nb, ws.data_ptr(), wb, _lib.raw_stream(q.device),
             ),
             "chunk_gated_delta_rule forward",
         )
@@ -109,12 +109,12 @@ def chunk_bwd(q, k, v, g, beta, cu, scale, has_h0, states, do, dht):
     dh0 = torch.empty((N, HV, K, V), device=dev, dtype=torch.float32) if has_h0 else None
     wb = L.ssla_gated_delta_rule_workspace_bytes(N, T, H, HV, K, V, 1)
     ws = torch.empty(wb, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.check(
             L.ssla_chunk_gated_delta_rule_bwd(
                 *tensor_args(q, k, v, g, beta, cu, scale), states.data_ptr(), states.numel(), do.data_ptr(),
                 _lib.ptr(dht), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
-                _lib.ptr(dh0), ws.data_ptr(), wb, _lib.stream_of(q),
+                _lib.ptr(dh0), ws.data_ptr(), wb, _lib.raw_stream(q.device),
             ),
             "chunk_gated_delta_rule backward",
         )

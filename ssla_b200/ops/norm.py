@@ -56,11 +56,11 @@ def _fwd(x, w, b, cu, T, C, G, eps, act):
     stats = torch.empty((N, G, 2), device=x.device, dtype=torch.float32) if cu is not None else None
     nb = L.ssla_group_norm_act_workspace_bytes(T, C, G, int(cu is not None), N, 0) if cu is not None else 0
     ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device):
         _lib.check(
             L.ssla_group_norm_act_fwd(
                 x.data_ptr(), _lib.dtype_code(x), T, C, G, _lib.ptr(w), _lib.ptr(b), float(eps), act, _lib.ptr(cu), N,
-                y.data_ptr(), _lib.ptr(stats), _lib.ptr(ws), nb, _lib.stream_of(x),
+                y.data_ptr(), _lib.ptr(stats), _lib.ptr(ws), nb, _lib.raw_stream(x.device),
             ),
             "group_norm_act forward",
         )
@@ -89,12 +89,12 @@ class GroupNormActFunction(torch.autograd.Function):
         dw, db = torch.empty((2, C), device=x.device, dtype=torch.float32)
         nb = L.ssla_group_norm_act_workspace_bytes(T, C, G, int(cu is not None), N, 1)
         ws = torch.empty(nb, device=x.device, dtype=torch.uint8)
-        with torch.cuda.device(x.device):
+        with _lib.on_device(x.device):
             _lib.check(
                 L.ssla_group_norm_act_bwd(
                     x.data_ptr(), dy.data_ptr(), _lib.dtype_code(x), T, C, G, _lib.ptr(w), _lib.ptr(b), float(eps),
                     act, _lib.ptr(cu), N, _lib.ptr(stats), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
-                    nb, _lib.stream_of(x),
+                    nb, _lib.raw_stream(x.device),
                 ),
                 "group_norm_act backward",
             )

@@ -258,22 +258,24 @@ int ssla_layernorm_residual_fwd(const float* x, const float* r, const float* w, 
 
 /* Group norm with an activation over channels-last rows x [T,C], G groups of C/G channels:
  *   y = act(w (x - mean) / sqrt(var + eps) + b),  w, b [C] fp32 (NULL: 1, 0).
- * cu_seqlens NULL: statistics of each token's groups (C/G <= 1024); otherwise of each packed
- * sequence's groups (over its tokens), written to stats [N,G,2] fp32 = (mean, 1/sqrt(var + eps)) for
- * the backward, rows outside every sequence 0.  act: 0 none, 1 SiLU, 2 ReLU.  dw, db [C] fp32 are
- * sums over all rows in a fixed order.  workspace (16-byte aligned) of
- * ssla_group_norm_act_workspace_bytes (packed, backward: 0 / 1).  No counterpart in the reference
- * (its layers close with nn.LayerNorm, layers/mos_attention.py:144). */
+ * cu_seqlens NULL: statistics of each token's groups (C/G <= 1024; no saved buffer); otherwise of
+ * each packed sequence's groups (over its tokens), rows outside every sequence 0, and the forward
+ * leaves its chunk tables and statistics in `saved` (ssla_group_norm_act_saved_bytes) for the
+ * backward.  act: 0 none, 1 SiLU, 2 ReLU.  dw, db [C] fp32 are sums over all rows in a fixed order.
+ * workspace of ssla_group_norm_act_workspace_bytes (packed, backward: 0 / 1); both buffers 16-byte
+ * aligned.  No counterpart in the reference (its layers close with nn.LayerNorm,
+ * layers/mos_attention.py:144). */
 #define SSLA_ACT_NONE 0
 #define SSLA_ACT_SILU 1
 #define SSLA_ACT_RELU 2
+size_t ssla_group_norm_act_saved_bytes(int64_t T, int64_t C, int64_t G, int64_t n_seqs);
 size_t ssla_group_norm_act_workspace_bytes(int64_t T, int64_t C, int64_t G, int packed, int64_t n_seqs, int backward);
 int ssla_group_norm_act_fwd(const void* x, int dtype, int64_t T, int64_t C, int64_t G, const float* w, const float* b,
-                            float eps, int act, const int64_t* cu_seqlens, int64_t n_seqs, void* y, float* stats,
-                            void* workspace, size_t workspace_bytes, ssla_stream_t stream);
+                            float eps, int act, const int64_t* cu_seqlens, int64_t n_seqs, void* y, void* saved,
+                            size_t saved_bytes, void* workspace, size_t workspace_bytes, ssla_stream_t stream);
 int ssla_group_norm_act_bwd(const void* x, const void* dy, int dtype, int64_t T, int64_t C, int64_t G, const float* w,
                             const float* b, float eps, int act, const int64_t* cu_seqlens, int64_t n_seqs,
-                            const float* stats, void* dx, float* dw, float* db, void* workspace,
+                            const void* saved, size_t saved_bytes, void* dx, float* dw, float* db, void* workspace,
                             size_t workspace_bytes, ssla_stream_t stream);
 
 /* ---------------------------------------------------------------- event routing

@@ -69,8 +69,9 @@ SIGNATURES = {
     "ssla_mos_patch_scan_proj_fwd": (i32, [p, i64, p, i64, p, p, p, p, i64, i64, p, p]),
     "ssla_layernorm_residual_fwd": (i32, [p, p, p, p, i64, i64, f32, p, p]),
     "ssla_group_norm_act_workspace_bytes": (sz, [i64, i64, i64, i32, i64, i32]),
-    "ssla_group_norm_act_fwd": (i32, [p, i32, i64, i64, i64, p, p, f32, i32, p, i64, p, p, p, sz, p]),
-    "ssla_group_norm_act_bwd": (i32, [p, p, i32, i64, i64, i64, p, p, f32, i32, p, i64, p, p, p, p, p, sz, p]),
+    "ssla_group_norm_act_saved_bytes": (sz, [i64] * 4),
+    "ssla_group_norm_act_fwd": (i32, [p, i32, i64, i64, i64, p, p, f32, i32, p, i64, p, p, sz, p, sz, p]),
+    "ssla_group_norm_act_bwd": (i32, [p, p, i32, i64, i64, i64, p, p, f32, i32, p, i64, p, sz, p, p, p, p, sz, p]),
     "ssla_rows_matmul_smem_bytes": (sz, [i64, i64]),
     "ssla_batched_nms_workspace_bytes": (sz, [i64]),
     "ssla_batched_nms": (i32, [p, p, i64, i64, i32, f32, f32, i64, p, p, p, sz, p]),

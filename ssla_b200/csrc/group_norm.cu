@@ -14,6 +14,8 @@
 #include "pack_tables.cuh"
 #include "vec.cuh"
 
+#include <type_traits>
+
 namespace ssla {
 namespace gn {
 namespace {
@@ -24,23 +26,46 @@ inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 enum { ACT_NONE = SSLA_ACT_NONE, ACT_SILU = SSLA_ACT_SILU, ACT_RELU = SSLA_ACT_RELU };
 
 // 1 / (1 + exp(-z)) on the two special-function instructions, each good to about 2^-22: with the
-// library's expf and division the instructions, not the memory, bound the kernels (token_bwd of
-// 16384 x 4096 bf16: 265 us).  exp(-z) = inf gives 0.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+// library's expf and division the instructions, not the memory, bound the kernels (token_fwd of
+// 16384 x 4096 bf16: 113 us).  exp(-z) = inf gives 0.
+__device__ __forceinline__ float sigmoid(float z) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
 
-__device__ __forceinline__ float act_fwd(float z, int act) {
-  if (act == ACT_SILU) return z * sigmoid(z);
-  if (act == ACT_RELU) return z <= 0.f ? 0.f : z;  // NaN stays
+template <int ACT> __device__ __forceinline__ float act_fwd(float z) {
+  if (ACT == ACT_SILU) return z * sigmoid(z);
+  if (ACT == ACT_RELU) return z <= 0.f ? 0.f : z;  // NaN stays
   return z;
 }
-__device__ __forceinline__ float act_bwd(float dy, float z, int act) {
-  if (act == ACT_SILU) {
+template <int ACT> __device__ __forceinline__ float act_bwd(float dy, float z) {
+  if (ACT == ACT_SILU) {
     const float s = sigmoid(z);
     return dy * (s * fmaf(z, 1.f - s, 1.f));
   }
-  if (act == ACT_RELU) return z <= 0.f ? 0.f : dy;
+  if (ACT == ACT_RELU) return z <= 0.f ? 0.f : dy;
   return dy;
 }
+// f(integral constant of the activation): the loops inside carry no test of it
+template <class F> __device__ __forceinline__ void with_act(int act, F f) {
+  if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>());
+  else if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>());
+  else f(std::integral_constant<int, ACT_NONE>());
+}
+// sum over aligned groups of L lanes
+__device__ __forceinline__ float lane_sum(float x, int L) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1)
+    if (d < L) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
+
+// VEC elements as they lie in memory: loads for the next token wait in these while this one computes.
+template <class TI, int VEC> struct alignas(sizeof(TI) * VEC) Raw {
+  TI e[VEC];
+};
 
 template <int VEC> __device__ __forceinline__ void load_param(const float* p, int at, float dflt, float* x) {
 #pragma unroll
@@ -72,52 +97,71 @@ __global__ void __launch_bounds__(TH) token_fwd(const TI* __restrict__ x, int64_
       load_param<VEC>(b, g * Cg + c, 0.f, bb[j]);
     }
   }
-  for (int64_t t0 = (int64_t)blockIdx.x * m.TP; t0 < T; t0 += (int64_t)gridDim.x * m.TP) {
-    const int64_t t = t0 + tp;
-    const bool on = live && t < T;
-    const size_t base = (size_t)t * C + (size_t)g * Cg;
-    float v[NV][VEC], s = 0.f;
+  using R = Raw<TI, VEC>;
+  const int64_t step = (int64_t)gridDim.x * m.TP;
+  R rx[NV];
+  const int64_t first = (int64_t)blockIdx.x * m.TP + tp;
+  const TI* px = x + (size_t)first * C + (size_t)g * Cg;
+  TI* py = y + (size_t)first * C + (size_t)g * Cg;
+  const size_t stride = (size_t)step * C;
+  auto fetch = [&](int64_t t) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * m.L + l) * VEC;
-      const bool in = on && c < Cg;
-      if (in) Vec<TI, VEC>::load(x + base + c, v[j]);
+      if (live && t < T && c < Cg) {
+        rx[j] = *reinterpret_cast<const R*>(px + c);
+      } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (!in) v[j][i] = 0.f;
-        s += v[j][i];
+        for (int i = 0; i < VEC; ++i) rx[j].e[i] = TI(0.f);
       }
     }
-    for (int d = m.L >> 1; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float mean = s * inv;
+  };
+  fetch(first);
+  for (int64_t t0 = (int64_t)blockIdx.x * m.TP; t0 < T; t0 += step, py += stride) {
+    const int64_t t = t0 + tp;
+    const bool on = live && t < T;
+    float v[NV][VEC], s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[j][i] = ldf(&rx[j].e[i]);
+        s += v[j][i];
+      }
+    px += stride;
+    fetch(t + step);
+    const float mean = lane_sum(s, m.L) * inv;
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const bool in = (j * m.L + l) * VEC < Cg;
+      if ((j * m.L + l) * VEC < Cg)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        v[j][i] -= mean;
-        if (in) q = fmaf(v[j][i], v[j][i], q);
-      }
+        for (int i = 0; i < VEC; ++i) {
+          v[j][i] -= mean;
+          q = fmaf(v[j][i], v[j][i], q);
+        }
     }
-    for (int d = m.L >> 1; d; d >>= 1) q += __shfl_xor_sync(0xffffffffu, q, d);
-    const float rstd = 1.f / sqrtf(q * inv + eps);
+    const float rstd = rsqrtf(lane_sum(q, m.L) * inv + eps);
+    with_act(act, [&](auto A) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * m.L + l) * VEC;
-      if (on && c < Cg) {
-        float o[VEC];
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * m.L + l) * VEC;
+        if (on && c < Cg) {
+          float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = act_fwd(fmaf(v[j][i] * rstd, ww[j][i], bb[j][i]), act);
-        Vec<TI, VEC>::store(y + base + c, o);
+          for (int i = 0; i < VEC; ++i) o[i] = act_fwd<A.value>(fmaf(v[j][i] * rstd, ww[j][i], bb[j][i]));
+          Vec<TI, VEC>::store(py + c, o);
+        }
       }
-    }
+    });
   }
 }
 
 // part [2][gridDim.x * TP][C]: this block's sums of dz xh and dz over its tokens
+constexpr int tok_resident(int per_lane) { return per_lane <= 8 ? 3 : per_lane <= 16 ? 2 : 1; }
+
 template <class TI, int VEC, int NV>
-__global__ void __launch_bounds__(TH) token_bwd(const TI* __restrict__ x, const TI* __restrict__ dy, int64_t T, int C,
+__global__ void __launch_bounds__(TH, tok_resident(VEC * NV)) token_bwd(const TI* __restrict__ x, const TI* __restrict__ dy, int64_t T, int C,
                                                 int G, TokMap m, const float* __restrict__ w,
                                                 const float* __restrict__ b, float eps, int act, TI* __restrict__ dx,
                                                 float* __restrict__ part) {
@@ -136,62 +180,73 @@ __global__ void __launch_bounds__(TH) token_bwd(const TI* __restrict__ x, const 
       load_param<VEC>(b, g * Cg + c, 0.f, bb[j]);
     }
   }
-  for (int64_t t0 = (int64_t)blockIdx.x * m.TP; t0 < T; t0 += (int64_t)gridDim.x * m.TP) {
-    const int64_t t = t0 + tp;
-    const bool on = live && t < T;
-    const size_t base = (size_t)t * C + (size_t)g * Cg;
-    float v[NV][VEC], e[NV][VEC], s = 0.f;
+  using R = Raw<TI, VEC>;
+  const int64_t step = (int64_t)gridDim.x * m.TP;
+  R rx[NV], ry[NV];
+  const int64_t first = (int64_t)blockIdx.x * m.TP + tp;
+  const size_t start = (size_t)first * C + (size_t)g * Cg, stride = (size_t)step * C;
+  const TI *px = x + start, *pd = dy + start;
+  TI* po = dx + start;
+  auto fetch = [&](int64_t t) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * m.L + l) * VEC;
-      const bool in = on && c < Cg;
-      if (in) {
-        Vec<TI, VEC>::load(x + base + c, v[j]);
-        Vec<TI, VEC>::load(dy + base + c, e[j]);
-      }
+      if (live && t < T && c < Cg) {
+        rx[j] = *reinterpret_cast<const R*>(px + c);
+        ry[j] = *reinterpret_cast<const R*>(pd + c);
+      } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (!in) v[j][i] = e[j][i] = 0.f;
-        s += v[j][i];
+        for (int i = 0; i < VEC; ++i) rx[j].e[i] = ry[j].e[i] = TI(0.f);
       }
     }
-    for (int d = m.L >> 1; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float mean = s * inv;
+  };
+  fetch(first);
+  for (int64_t t0 = (int64_t)blockIdx.x * m.TP; t0 < T; t0 += step, po += stride) {
+    const int64_t t = t0 + tp;
+    const bool on = live && t < T;
+    float v[NV][VEC], e[NV][VEC], s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[j][i] = ldf(&rx[j].e[i]);
+        e[j][i] = ldf(&ry[j].e[i]);
+        s += v[j][i];
+      }
+    px += stride;
+    pd += stride;
+    fetch(t + step);
+    const float mean = lane_sum(s, m.L) * inv;
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const bool in = (j * m.L + l) * VEC < Cg;
+      if ((j * m.L + l) * VEC < Cg)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        v[j][i] -= mean;
-        if (in) q = fmaf(v[j][i], v[j][i], q);
-      }
+        for (int i = 0; i < VEC; ++i) {
+          v[j][i] -= mean;
+          q = fmaf(v[j][i], v[j][i], q);
+        }
     }
-    for (int d = m.L >> 1; d; d >>= 1) q += __shfl_xor_sync(0xffffffffu, q, d);
-    const float rstd = 1.f / sqrtf(q * inv + eps);
+    const float rstd = rsqrtf(lane_sum(q, m.L) * inv + eps);
     float s1 = 0.f, s2 = 0.f;
+    with_act(act, [&](auto A) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const bool in = on && (j * m.L + l) * VEC < Cg;
+      for (int j = 0; j < NV; ++j)
+        if (on && (j * m.L + l) * VEC < Cg)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (!in) continue;
-        const float xh = v[j][i] * rstd;
-        const float dz = act_bwd(e[j][i], fmaf(xh, ww[j][i], bb[j][i]), act);
-        dw[j][i] = fmaf(dz, xh, dw[j][i]);
-        db[j][i] += dz;
-        v[j][i] = xh;
-        e[j][i] = dz * ww[j][i];
-        s1 += e[j][i];
-        s2 = fmaf(e[j][i], xh, s2);
-      }
-    }
-    for (int d = m.L >> 1; d; d >>= 1) {
-      s1 += __shfl_xor_sync(0xffffffffu, s1, d);
-      s2 += __shfl_xor_sync(0xffffffffu, s2, d);
-    }
-    s1 *= inv;
-    s2 *= inv;
+          for (int i = 0; i < VEC; ++i) {
+            const float xh = v[j][i] * rstd;
+            const float dz = act_bwd<A.value>(e[j][i], fmaf(xh, ww[j][i], bb[j][i]));
+            dw[j][i] = fmaf(dz, xh, dw[j][i]);
+            db[j][i] += dz;
+            v[j][i] = xh;
+            e[j][i] = dz * ww[j][i];
+            s1 += e[j][i];
+            s2 = fmaf(e[j][i], xh, s2);
+          }
+    });
+    s1 = lane_sum(s1, m.L) * inv;
+    s2 = lane_sum(s2, m.L) * inv;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * m.L + l) * VEC;
@@ -199,7 +254,7 @@ __global__ void __launch_bounds__(TH) token_bwd(const TI* __restrict__ x, const 
         float o[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = rstd * (e[j][i] - s1 - v[j][i] * s2);
-        Vec<TI, VEC>::store(dx + base + c, o);
+        Vec<TI, VEC>::store(po + c, o);
       }
     }
   }
@@ -361,14 +416,16 @@ __global__ void __launch_bounds__(TH) pack_fwd(const TI* __restrict__ x, int64_t
     load_param<VEC>(w, ch, 1.f, ww);
     load_param<VEC>(b, ch, 0.f, bb);
     const size_t base = (size_t)t0 * C + ch;
+    with_act(act, [&](auto A) {
 #pragma unroll 4
-    for (int r = rl; r < rows; r += m.RP) {
-      float v[VEC];
-      Vec<TI, VEC>::load(x + base + (size_t)r * C, v);
+      for (int r = rl; r < rows; r += m.RP) {
+        float v[VEC];
+        Vec<TI, VEC>::load(x + base + (size_t)r * C, v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = act_fwd(fmaf((v[i] - st.x) * st.y, ww[i], bb[i]), act);
-      Vec<TI, VEC>::store(y + base + (size_t)r * C, v);
-    }
+        for (int i = 0; i < VEC; ++i) v[i] = act_fwd<A.value>(fmaf((v[i] - st.x) * st.y, ww[i], bb[i]));
+        Vec<TI, VEC>::store(y + base + (size_t)r * C, v);
+      }
+    });
   }
 }
 
@@ -381,8 +438,7 @@ __global__ void __launch_bounds__(TH) pack_sums(const TI* __restrict__ x, const 
   __shared__ float sm[2][VEC][TH];
   int64_t t0, seq;
   int rows;
-  const bool have = chunk_at(tab, blockIdx.x, t0, rows, seq);
-  if (!have) rows = 0;  // entries behind the last chunk are zeros for the column sums
+  if (!chunk_at(tab, blockIdx.x, t0, rows, seq)) return;
   const int Cg = C / G, g0 = blockIdx.y * m.GB, cv = min(m.GB, G - g0) * Cg / VEC;
   const int tc = threadIdx.x % m.TC, rl = threadIdx.x / m.TC;
   for (int c0 = 0; c0 < cv; c0 += m.TC) {
@@ -391,25 +447,27 @@ __global__ void __launch_bounds__(TH) pack_sums(const TI* __restrict__ x, const 
     float dw[VEC], db[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[i] = db[i] = 0.f;
-    if (in && have) {
+    if (in) {
       const float2 st = stats[seq * G + ch / Cg];
       float ww[VEC], bb[VEC];
       load_param<VEC>(w, ch, 1.f, ww);
       load_param<VEC>(b, ch, 0.f, bb);
       const size_t base = (size_t)t0 * C + ch;
+      with_act(act, [&](auto A) {
 #pragma unroll 4
-      for (int r = rl; r < rows; r += m.RP) {
-        float v[VEC], e[VEC];
-        Vec<TI, VEC>::load(x + base + (size_t)r * C, v);
-        Vec<TI, VEC>::load(dy + base + (size_t)r * C, e);
+        for (int r = rl; r < rows; r += m.RP) {
+          float v[VEC], e[VEC];
+          Vec<TI, VEC>::load(x + base + (size_t)r * C, v);
+          Vec<TI, VEC>::load(dy + base + (size_t)r * C, e);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float xh = (v[i] - st.x) * st.y;
-          const float dz = act_bwd(e[i], fmaf(xh, ww[i], bb[i]), act);
-          dw[i] = fmaf(dz, xh, dw[i]);
-          db[i] += dz;
+          for (int i = 0; i < VEC; ++i) {
+            const float xh = (v[i] - st.x) * st.y;
+            const float dz = act_bwd<A.value>(e[i], fmaf(xh, ww[i], bb[i]));
+            dw[i] = fmaf(dz, xh, dw[i]);
+            db[i] += dz;
+          }
         }
-      }
+      });
     }
     __syncthreads();
 #pragma unroll
@@ -432,22 +490,46 @@ __global__ void __launch_bounds__(TH) pack_sums(const TI* __restrict__ x, const 
   }
 }
 
-// means [N][G] = (mean e, mean e xh) from the chunks' channel sums: one warp per (sequence, group)
-__global__ void __launch_bounds__(TH) pack_means(const float* __restrict__ part, int64_t MC, const int* __restrict__ off,
-                                                 const int64_t* __restrict__ cu, int64_t N, int64_t T, int C, int G,
-                                                 const float* __restrict__ w, float2* __restrict__ means) {
+// seq [2][N][C] = sums of part [2][MC][C] over the chunks of a sequence; 32 channels a block
+__global__ void __launch_bounds__(TH) pack_join(const float* __restrict__ part, int64_t MC, const int* __restrict__ off,
+                                                int64_t N, int C, float* __restrict__ seq) {
+  __shared__ double sm[2][TH / 32][32];
+  const int64_t n = blockIdx.x;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.y * 32 + tx;
+  double a = 0.0, b = 0.0;
+  if (c < C)
+    for (int r = off[n] + ty; r < off[n + 1]; r += TH / 32) {
+      a += (double)part[(size_t)r * C + c];
+      b += (double)part[((size_t)MC + r) * C + c];
+    }
+  sm[0][ty][tx] = a;
+  sm[1][ty][tx] = b;
+  __syncthreads();
+  if (ty == 0 && c < C) {
+#pragma unroll
+    for (int i = 1; i < TH / 32; ++i) {
+      a += sm[0][i][tx];
+      b += sm[1][i][tx];
+    }
+    seq[(size_t)n * C + c] = (float)a;
+    seq[(size_t)(N + n) * C + c] = (float)b;
+  }
+}
+
+// means [N][G] = (mean e, mean e xh) from the sequences' channel sums: one warp per (sequence, group)
+__global__ void __launch_bounds__(TH) pack_means(const float* __restrict__ seq, const int64_t* __restrict__ cu,
+                                                 int64_t N, int64_t T, int C, int G, const float* __restrict__ w,
+                                                 float2* __restrict__ means) {
   const int64_t id = (int64_t)blockIdx.x * (TH / 32) + (threadIdx.x >> 5);
   if (id >= N * G) return;
   const int64_t n = id / G;
   const int g = (int)(id - n * G), lane = threadIdx.x & 31, Cg = C / G;
   double s1 = 0.0, s2 = 0.0;
-  const int first = off[n], cnt = off[n + 1] - first;
-  for (int64_t j = lane; j < (int64_t)cnt * Cg; j += 32) {
-    const int64_t r = first + j / Cg;
-    const int ch = g * Cg + (int)(j % Cg);
+  for (int j = lane; j < Cg; j += 32) {
+    const int ch = g * Cg + j;
     const double ww = w ? (double)w[ch] : 1.0;
-    s2 += ww * (double)part[(size_t)r * C + ch];
-    s1 += ww * (double)part[((size_t)MC + r) * C + ch];
+    s2 += ww * (double)seq[(size_t)n * C + ch];
+    s1 += ww * (double)seq[(size_t)(N + n) * C + ch];
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
@@ -480,19 +562,21 @@ __global__ void __launch_bounds__(TH) pack_bwd(const TI* __restrict__ x, const T
     load_param<VEC>(w, ch, 1.f, ww);
     load_param<VEC>(b, ch, 0.f, bb);
     const size_t base = (size_t)t0 * C + ch;
+    with_act(act, [&](auto A) {
 #pragma unroll 4
-    for (int r = rl; r < rows; r += m.RP) {
-      float v[VEC], e[VEC];
-      Vec<TI, VEC>::load(x + base + (size_t)r * C, v);
-      Vec<TI, VEC>::load(dy + base + (size_t)r * C, e);
+      for (int r = rl; r < rows; r += m.RP) {
+        float v[VEC], e[VEC];
+        Vec<TI, VEC>::load(x + base + (size_t)r * C, v);
+        Vec<TI, VEC>::load(dy + base + (size_t)r * C, e);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float xh = (v[i] - st.x) * st.y;
-        const float dz = act_bwd(e[i], fmaf(xh, ww[i], bb[i]), act);
-        v[i] = st.y * (fmaf(dz, ww[i], -mm.x) - xh * mm.y);
+        for (int i = 0; i < VEC; ++i) {
+          const float xh = (v[i] - st.x) * st.y;
+          const float dz = act_bwd<A.value>(e[i], fmaf(xh, ww[i], bb[i]));
+          v[i] = st.y * (fmaf(dz, ww[i], -mm.x) - xh * mm.y);
+        }
+        Vec<TI, VEC>::store(dx + base + (size_t)r * C, v);
       }
-      Vec<TI, VEC>::store(dx + base + (size_t)r * C, v);
-    }
+    });
   }
 }
 
@@ -530,7 +614,7 @@ TokMap tok_map(int64_t Cg, int64_t G, int vec, int* nv) {
   return m;
 }
 
-// tokens in flight: about eight blocks on every SM
+// blocks along the tokens, per_sm on every SM
 int tok_blocks(int64_t T, int gy, int TP, int per_sm) {
   int64_t want = (int64_t)kNumSMs * per_sm / gy, most = (T + TP - 1) / TP;
   if (want < 1) want = 1;
@@ -538,8 +622,8 @@ int tok_blocks(int64_t T, int gy, int TP, int per_sm) {
 }
 
 int chunk_rows(int64_t T, int64_t C) {
-  // at least ~4 blocks per SM, at most 64 KiB of fp32 channels a block
-  int64_t r = T / (4 * kNumSMs);
+  // ~12 blocks per SM even out the last wave; at most 1 MiB of fp32 channels a block
+  int64_t r = T / (12 * kNumSMs);
   const int64_t most = 16384 / (C < 16384 ? C : 16384) * 16;
   r = r > most ? most : r;
   r = r < 16 ? 16 : r;
@@ -557,26 +641,44 @@ PackMap pack_map(int64_t T, int64_t C, int64_t G, int vec) {
   return m;
 }
 
-struct PackWork {
+// What the forward leaves for the backward: the chunk tables and the statistics.
+struct PackSaved {
   int* off;
   longlong2* tab;
-  double2* part;   // forward
-  float* sums;     // backward [2][MC][C]
-  float2* means;   // backward [N][G]
+  float2* stats;
 };
 
-size_t pack_layout(void* base, int64_t N, int64_t T, int64_t C, int64_t G, bool bwd, PackWork* out, int64_t* mc) {
+size_t pack_saved(void* base, int64_t N, int64_t T, int64_t C, int64_t G, PackSaved* out, int64_t* mc) {
   const int64_t R = chunk_rows(T, C), MC = (T + (R - 1) * N) / R;
   char* q = (char*)base;
   auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
+  PackSaved s;
+  s.off = (int*)take(4 * (N + 1));
+  s.tab = (longlong2*)take(16 * (size_t)MC);
+  s.stats = (float2*)take(8 * (size_t)N * G);
+  if (out) *out = s;
+  if (mc) *mc = MC;
+  return (size_t)(q - (char*)base);
+}
+
+struct PackWork {
+  double2* part;   // forward [MC][G]
+  float* sums;     // backward [2][MC][C]
+  float* seq;      // backward [2][N][C]
+  float2* means;   // backward [N][G]
+};
+
+size_t pack_work(void* base, int64_t N, int64_t T, int64_t C, int64_t G, bool bwd, PackWork* out) {
+  int64_t MC;
+  pack_saved(nullptr, N, T, C, G, nullptr, &MC);
+  char* q = (char*)base;
+  auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
   PackWork w;
-  w.off = (int*)take(4 * (N + 1));
-  w.tab = (longlong2*)take(16 * (size_t)MC);
   w.part = (double2*)take(bwd ? 0 : 16 * (size_t)MC * G);
   w.sums = (float*)take(bwd ? 8 * (size_t)MC * C : 0);
+  w.seq = (float*)take(bwd ? 8 * (size_t)N * C : 0);
   w.means = (float2*)take(bwd ? 8 * (size_t)N * G : 0);
   if (out) *out = w;
-  if (mc) *mc = MC;
   return (size_t)(q - (char*)base);
 }
 
@@ -615,7 +717,7 @@ struct Call {
   int act;
   const int64_t* cu;
   void* y;  // or dx
-  float2* stats;
+  void* saved;
   float *dw, *db;
   void* ws;
 };
@@ -623,12 +725,12 @@ struct Call {
 template <class TI, int VEC, int NV> int token_call(const Call& c, const TokMap& m, cudaStream_t st) {
   const int gy = (c.G + m.GB - 1) / m.GB;
   if (!c.dy) {
-    token_fwd<TI, VEC, NV><<<dim3(tok_blocks(c.T, gy, m.TP, 16), gy), TH, 0, st>>>(
+    token_fwd<TI, VEC, NV><<<dim3(tok_blocks(c.T, gy, m.TP, 32), gy), TH, 0, st>>>(
         (const TI*)c.x, c.T, c.C, c.G, m, c.w, c.b, c.eps, c.act, (TI*)c.y);
     SSLA_CHECK_LAUNCH("group_norm forward");
     return SSLA_OK;
   }
-  const int gx = tok_blocks(c.T, gy, m.TP, 4);
+  const int gx = tok_blocks(c.T, gy, m.TP, tok_resident(VEC * NV));  // one wave: the sums stay in registers
   token_bwd<TI, VEC, NV><<<dim3(gx, gy), TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.T, c.C, c.G, m, c.w, c.b, c.eps,
                                                       c.act, (TI*)c.y, (float*)c.ws);
   SSLA_CHECK_LAUNCH("group_norm backward");
@@ -654,41 +756,49 @@ template <class TI, int VEC> int token_vec(const Call& c, cudaStream_t st) {
 }
 
 template <class TI, int VEC> int pack_call(const Call& c, cudaStream_t st) {
+  PackSaved sv;
   PackWork w;
   int64_t MC;
-  pack_layout(c.ws, c.N, c.T, c.C, c.G, c.dy != nullptr, &w, &MC);
+  pack_saved(c.saved, c.N, c.T, c.C, c.G, &sv, &MC);
+  pack_work(c.ws, c.N, c.T, c.C, c.G, c.dy != nullptr, &w);
   const PackMap m = pack_map(c.T, c.C, c.G, VEC);
   const dim3 grid((unsigned)(MC > 0 ? MC : 1), (c.G + m.GB - 1) / m.GB);
   const unsigned ngrid = (unsigned)((c.N * c.G + TH / 32 - 1) / (TH / 32));
-  int rc = launch_pack_tables(c.cu, c.N, c.T, m.R, MC, 0, 0, w.off, nullptr, w.tab, nullptr, st);
-  if (rc) return rc;
   if (!c.dy) {
+    int rc = launch_pack_tables(c.cu, c.N, c.T, m.R, MC, 0, 0, sv.off, nullptr, sv.tab, nullptr, st);
+    if (rc) return rc;
     if (MC > 0) {
-      pack_stats<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, c.C, c.G, m, w.tab, w.part);
+      pack_stats<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, c.C, c.G, m, sv.tab, w.part);
       SSLA_CHECK_LAUNCH("group_norm statistics");
     }
     if (ngrid) {
-      pack_moments<<<ngrid, TH, 0, st>>>(w.part, w.off, c.cu, c.N, c.T, c.G, c.C / c.G, c.eps, c.stats);
+      pack_moments<<<ngrid, TH, 0, st>>>(w.part, sv.off, c.cu, c.N, c.T, c.G, c.C / c.G, c.eps, sv.stats);
       SSLA_CHECK_LAUNCH("group_norm moments");
     }
-    pack_fwd<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, c.T, c.C, c.G, m, w.tab, MC, c.cu, c.N, c.stats, c.w, c.b,
+    if (c.T == 0) return SSLA_OK;
+    pack_fwd<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, c.T, c.C, c.G, m, sv.tab, MC, c.cu, c.N, sv.stats, c.w, c.b,
                                            c.act, (TI*)c.y);
     SSLA_CHECK_LAUNCH("group_norm forward");
     return SSLA_OK;
   }
   if (MC > 0) {
-    pack_sums<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.C, c.G, m, w.tab, MC, c.stats, c.w, c.b,
+    pack_sums<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.C, c.G, m, sv.tab, MC, sv.stats, c.w, c.b,
                                             c.act, w.sums);
     SSLA_CHECK_LAUNCH("group_norm sums");
   }
-  column_sums<<<dim3((c.C + 31) / 32, 2), 1024, 0, st>>>(w.sums, MC, c.C, c.dw, c.db);
+  if (c.N > 0) {
+    pack_join<<<dim3((unsigned)c.N, (c.C + 31) / 32), TH, 0, st>>>(w.sums, MC, sv.off, c.N, c.C, w.seq);
+    SSLA_CHECK_LAUNCH("group_norm join");
+  }
+  column_sums<<<dim3((c.C + 31) / 32, 2), 1024, 0, st>>>(w.seq, c.N, c.C, c.dw, c.db);
   SSLA_CHECK_LAUNCH("group_norm column sums");
   if (ngrid) {
-    pack_means<<<ngrid, TH, 0, st>>>(w.sums, MC, w.off, c.cu, c.N, c.T, c.C, c.G, c.w, w.means);
+    pack_means<<<ngrid, TH, 0, st>>>(w.seq, c.cu, c.N, c.T, c.C, c.G, c.w, w.means);
     SSLA_CHECK_LAUNCH("group_norm means");
   }
-  pack_bwd<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.T, c.C, c.G, m, w.tab, MC, c.cu, c.N,
-                                         c.stats, w.means, c.w, c.b, c.act, (TI*)c.y);
+  if (c.T == 0) return SSLA_OK;
+  pack_bwd<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.T, c.C, c.G, m, sv.tab, MC, c.cu, c.N,
+                                         sv.stats, w.means, c.w, c.b, c.act, (TI*)c.y);
   SSLA_CHECK_LAUNCH("group_norm backward");
   return SSLA_OK;
 }
@@ -712,50 +822,61 @@ int dispatch(const Call& c, int dtype, cudaStream_t st) {
 using namespace ssla;
 using namespace ssla::gn;
 
+extern "C" size_t ssla_group_norm_act_saved_bytes(int64_t T, int64_t C, int64_t G, int64_t n_seqs) {
+  if (T < 0 || C < 1 || G < 1 || C % G || n_seqs < 0) return 0;
+  return pack_saved(nullptr, n_seqs, T, C, G, nullptr, nullptr);
+}
+
 extern "C" size_t ssla_group_norm_act_workspace_bytes(int64_t T, int64_t C, int64_t G, int packed, int64_t n_seqs,
                                                       int backward) {
   if (T < 0 || C < 1 || G < 1 || C % G || n_seqs < 0) return 0;
-  if (packed) return pack_layout(nullptr, n_seqs, T, C, G, backward != 0, nullptr, nullptr);
+  if (packed) return pack_work(nullptr, n_seqs, T, C, G, backward != 0, nullptr);
   return backward ? tok_part_bytes(T, C, G) : 0;
+}
+
+// Buffers of one call: the workspace, and with cu_seqlens what the forward saves.
+static int check_buffers(const char* name, int64_t T, int64_t C, int64_t G, bool packed, int64_t N, bool bwd,
+                         const void* saved, size_t saved_bytes, const void* ws, size_t ws_bytes) {
+  const size_t need = ssla_group_norm_act_workspace_bytes(T, C, G, packed, N, bwd);
+  const size_t keep = packed ? ssla_group_norm_act_saved_bytes(T, C, G, N) : 0;
+  if (ws_bytes < need || (need && !ws) || saved_bytes < keep || (keep && !saved)) {
+    set_error("%s: saved buffer of %zu bytes and workspace of %zu, %zu and %zu needed", name, saved_bytes, ws_bytes, keep,
+              need);
+    return SSLA_ERR_WORKSPACE;
+  }
+  SSLA_CHECK_ARG(aligned_to(ws, 16) && aligned_to(saved, 16), "%s: misaligned workspace or saved buffer", name);
+  return SSLA_OK;
 }
 
 extern "C" int ssla_group_norm_act_fwd(const void* x, int dtype, int64_t T, int64_t C, int64_t G, const float* w,
                                        const float* b, float eps, int act, const int64_t* cu_seqlens, int64_t n_seqs,
-                                       void* y, float* stats, void* workspace, size_t workspace_bytes,
-                                       ssla_stream_t stream) {
+                                       void* y, void* saved, size_t saved_bytes, void* workspace,
+                                       size_t workspace_bytes, ssla_stream_t stream) {
   const char* name = "ssla_group_norm_act_fwd";
   int rc = check(name, dtype, T, C, G, act, cu_seqlens != nullptr, n_seqs);
   if (rc) return rc;
   if (T == 0 && (!cu_seqlens || n_seqs == 0)) return SSLA_OK;
   SSLA_CHECK_ARG(T == 0 || (x && y), "%s: null pointer", name);
-  SSLA_CHECK_ARG(!cu_seqlens || n_seqs == 0 || stats, "%s: null stats", name);
-  const size_t need = ssla_group_norm_act_workspace_bytes(T, C, G, cu_seqlens != nullptr, n_seqs, 0);
-  if (workspace_bytes < need || (need && !workspace)) {
-    set_error("%s: workspace of %zu bytes < %zu needed", name, workspace_bytes, need);
-    return SSLA_ERR_WORKSPACE;
-  }
-  SSLA_CHECK_ARG(aligned_to(workspace, 16) && aligned_to(stats, 8), "%s: misaligned workspace or stats", name);
-  const Call c = {x, nullptr, T, n_seqs, (int)C, (int)G, w, b, eps, act, cu_seqlens, y, (float2*)stats, nullptr, nullptr,
-                  workspace};
+  if ((rc = check_buffers(name, T, C, G, cu_seqlens != nullptr, n_seqs, false, saved, saved_bytes, workspace,
+                          workspace_bytes)))
+    return rc;
+  const Call c = {x, nullptr, T, n_seqs, (int)C, (int)G, w, b, eps, act, cu_seqlens, y, saved, nullptr, nullptr, workspace};
   return dispatch(c, dtype, (cudaStream_t)stream);
 }
 
 extern "C" int ssla_group_norm_act_bwd(const void* x, const void* dy, int dtype, int64_t T, int64_t C, int64_t G,
                                        const float* w, const float* b, float eps, int act, const int64_t* cu_seqlens,
-                                       int64_t n_seqs, const float* stats, void* dx, float* dw, float* db,
-                                       void* workspace, size_t workspace_bytes, ssla_stream_t stream) {
+                                       int64_t n_seqs, const void* saved, size_t saved_bytes, void* dx, float* dw,
+                                       float* db, void* workspace, size_t workspace_bytes, ssla_stream_t stream) {
   const char* name = "ssla_group_norm_act_bwd";
   int rc = check(name, dtype, T, C, G, act, cu_seqlens != nullptr, n_seqs);
   if (rc) return rc;
   SSLA_CHECK_ARG(dw && db && (T == 0 || (x && dy && dx)), "%s: null pointer", name);
-  SSLA_CHECK_ARG(!cu_seqlens || n_seqs == 0 || stats, "%s: null stats", name);
-  const size_t need = ssla_group_norm_act_workspace_bytes(T, C, G, cu_seqlens != nullptr, n_seqs, 1);
-  if (workspace_bytes < need || (need && !workspace)) {
-    set_error("%s: workspace of %zu bytes < %zu needed", name, workspace_bytes, need);
-    return SSLA_ERR_WORKSPACE;
-  }
-  SSLA_CHECK_ARG(aligned_to(workspace, 16) && aligned_to(stats, 8), "%s: misaligned workspace or stats", name);
-  const Call c = {x, dy, T, n_seqs, (int)C, (int)G, w, b, eps, act, cu_seqlens, dx, (float2*)const_cast<float*>(stats),
+  if ((rc = check_buffers(name, T, C, G, cu_seqlens != nullptr, n_seqs, true, saved, saved_bytes, workspace,
+                          workspace_bytes)))
+    return rc;
+  // dy marks the backward for the dispatch, also where there are no rows
+  const Call c = {x, dy ? dy : dw, T, n_seqs, (int)C, (int)G, w, b, eps, act, cu_seqlens, dx, const_cast<void*>(saved),
                   dw, db, workspace};
   return dispatch(c, dtype, (cudaStream_t)stream);
 }

@@ -10,7 +10,8 @@ __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { 
 __global__ void __launch_bounds__(1024) tables_kernel(const int64_t* __restrict__ cu, int64_t N, int64_t T, int BT,
                                                       int64_t MC, int64_t len, int64_t MS, int* chunk_off, int* seg_off,
                                                       longlong2* chunk_tab, int4* seg_tab) {
-  __shared__ int wc[32], ws[32], run[2];
+  constexpr int KEPT = 1024;  // bounds of this many sequences stay in shared memory
+  __shared__ int wc[32], ws[32], run[2], kc[KEPT + 1], ks[KEPT + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) run[0] = run[1] = 0;
   __syncthreads();
@@ -65,12 +66,22 @@ __global__ void __launch_bounds__(1024) tables_kernel(const int64_t* __restrict_
     }
     return lo;
   };
+  const bool kept = N <= KEPT;
+  if (kept) {
+    for (int64_t n = tid; n <= N; n += 1024) {
+      kc[n] = chunk_off[n];
+      if (len) ks[n] = seg_off[n];
+    }
+    __syncthreads();
+  }
+  const int* oc = kept ? kc : chunk_off;
+  const int* os = kept ? ks : seg_off;
   const int total = chunk_off[N], segs = len ? seg_off[N] : 0;
   for (int64_t c = tid; c < MC; c += 1024) {
     longlong2 e = make_longlong2(0, -1);
     if (c < total) {
-      const int64_t n = owner(chunk_off, c);
-      const int64_t b = clamp64(cu[n], 0, T), t1 = clamp64(cu[n + 1], b, T), t0 = b + (c - chunk_off[n]) * BT;
+      const int64_t n = owner(oc, c);
+      const int64_t b = clamp64(cu[n], 0, T), t1 = clamp64(cu[n + 1], b, T), t0 = b + (c - oc[n]) * BT;
       const int64_t rows = t1 - t0 < BT ? t1 - t0 : BT;
       if (rows > 0) e = make_longlong2(t0, rows | (n << 32));
     }
@@ -79,9 +90,9 @@ __global__ void __launch_bounds__(1024) tables_kernel(const int64_t* __restrict_
   for (int64_t s = tid; s < MS; s += 1024) {
     int4 e = make_int4(0, 0, -1, 0);
     if (s < segs) {
-      const int n = (int)owner(seg_off, s);
-      const int first = chunk_off[n] + (int)((s - seg_off[n]) * len);
-      int cnt = chunk_off[n + 1] - first;
+      const int n = (int)owner(os, s);
+      const int first = oc[n] + (int)((s - os[n]) * len);
+      int cnt = oc[n + 1] - first;
       cnt = cnt < 0 ? 0 : (cnt > len ? (int)len : cnt);
       e = make_int4(first, cnt, n, 0);
     }

@@ -53,26 +53,30 @@ def _fwd(x, w, b, cu, T, C, G, eps, act):
     L = _lib.load()
     N = cu.numel() - 1 if cu is not None else 0
     y = torch.empty_like(x)
-    stats = torch.empty((N, G, 2), device=x.device, dtype=torch.float32) if cu is not None else None
-    nb = L.ssla_group_norm_act_workspace_bytes(T, C, G, int(cu is not None), N, 0) if cu is not None else 0
-    ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
+    saved = ws = None
+    sb = nb = 0
+    if cu is not None:
+        sb = L.ssla_group_norm_act_saved_bytes(T, C, G, N)
+        saved = torch.empty(sb, device=x.device, dtype=torch.uint8)
+        nb = L.ssla_group_norm_act_workspace_bytes(T, C, G, 1, N, 0)
+        ws = torch.empty(nb, device=x.device, dtype=torch.uint8)
     with _lib.on_device(x.device):
         _lib.check(
             L.ssla_group_norm_act_fwd(
                 x.data_ptr(), _lib.dtype_code(x), T, C, G, _lib.ptr(w), _lib.ptr(b), float(eps), act, _lib.ptr(cu), N,
-                y.data_ptr(), _lib.ptr(stats), _lib.ptr(ws), nb, _lib.raw_stream(x.device),
+                y.data_ptr(), _lib.ptr(saved), sb, _lib.ptr(ws), nb, _lib.raw_stream(x.device),
             ),
             "group_norm_act forward",
         )
-    return y, stats
+    return y, saved
 
 
 class GroupNormActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, num_groups, weight, bias, cu_seqlens, eps, activation):
         x, w, b, cu, T, C = _inputs(x, num_groups, weight, bias, cu_seqlens, activation)
-        y, stats = _fwd(x, w, b, cu, T, C, num_groups, eps, _ACT[activation])
-        ctx.save_for_backward(x, w, b, cu, stats)
+        y, saved = _fwd(x, w, b, cu, T, C, num_groups, eps, _ACT[activation])
+        ctx.save_for_backward(x, w, b, cu, saved)
         ctx.args = (num_groups, eps, _ACT[activation], T, C)
         ctx.dtypes = [p.dtype if p is not None else None for p in (weight, bias)]
         return y
@@ -80,7 +84,7 @@ class GroupNormActFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, w, b, cu, stats = ctx.saved_tensors
+        x, w, b, cu, saved = ctx.saved_tensors
         G, eps, act, T, C = ctx.args
         L = _lib.load()
         N = cu.numel() - 1 if cu is not None else 0
@@ -93,8 +97,8 @@ class GroupNormActFunction(torch.autograd.Function):
             _lib.check(
                 L.ssla_group_norm_act_bwd(
                     x.data_ptr(), dy.data_ptr(), _lib.dtype_code(x), T, C, G, _lib.ptr(w), _lib.ptr(b), float(eps),
-                    act, _lib.ptr(cu), N, _lib.ptr(stats), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(),
-                    nb, _lib.raw_stream(x.device),
+                    act, _lib.ptr(cu), N, _lib.ptr(saved), saved.numel() if saved is not None else 0, dx.data_ptr(),
+                    dw.data_ptr(), db.data_ptr(), ws.data_ptr(), nb, _lib.raw_stream(x.device),
                 ),
                 "group_norm_act backward",
             )

@@ -135,8 +135,10 @@ int ssla_chunk_gla_fwd_noalloc(const void* q, const void* k, const void* v, cons
  * is 0 in fp32 either way.
  * The chunked forward fills `states` (ssla_gated_delta_rule_states_bytes) for the backward; both
  * take scratch of ssla_gated_delta_rule_workspace_bytes (backward = 0 / 1).  states and workspace
- * are 16-byte aligned. */
-size_t ssla_gated_delta_rule_states_bytes(int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V);
+ * are 16-byte aligned.  has_h0, has_ht: whether the forward was given h0 and ht (bf16 calls with
+ * neither keep the states in 16 bits between the kernels). */
+size_t ssla_gated_delta_rule_states_bytes(int dtype, int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K,
+                                          int64_t V, int has_h0, int has_ht);
 size_t ssla_gated_delta_rule_workspace_bytes(int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
                                              int backward);
 int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, const void* v, const void* g, const void* beta,
@@ -147,9 +149,10 @@ int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, const void* v,
 int ssla_chunk_gated_delta_rule_bwd(const void* q, const void* k, const void* v, const void* g, const void* beta,
                                     int dtype, int dtype_g, int dtype_beta, const int64_t* cu_seqlens, int64_t n_seqs,
                                     int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V, float scale,
-                                    const void* states, size_t states_bytes, const void* dout, const float* dht,
-                                    void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dh0, void* workspace,
-                                    size_t workspace_bytes, ssla_stream_t stream);
+                                    int has_h0, int has_ht, const void* states, size_t states_bytes,
+                                    const void* dout, const float* dht, void* dq, void* dk, void* dv, void* dg,
+                                    void* dbeta, float* dh0, void* workspace, size_t workspace_bytes,
+                                    ssla_stream_t stream);
 /* The same forward token by token (streaming, serving): the state stays in registers. */
 int ssla_recurrent_gated_delta_rule_fwd(const void* q, const void* k, const void* v, const void* g, const void* beta,
                                         int dtype, int dtype_g, int dtype_beta, const int64_t* cu_seqlens,

@@ -42,11 +42,11 @@ SIGNATURES = {
         [p, p, p, p, i32, i32, p, i64, i64, i64, i64, i64, f32, p, sz, p, p, p, p, p, p, p, p, sz, p],
     ),
     "ssla_chunk_gla_fwd_noalloc": (i32, [p, p, p, p, i32, i32, p, i64, i64, i64, i64, i64, f32, p, p, p, p]),
-    "ssla_gated_delta_rule_states_bytes": (sz, [i64] * 6),
+    "ssla_gated_delta_rule_states_bytes": (sz, [i32] + [i64] * 6 + [i32] * 2),
     "ssla_gated_delta_rule_workspace_bytes": (sz, [i64] * 6 + [i32]),
     "ssla_chunk_gated_delta_rule_fwd": (i32, [p] * 5 + [i32] * 3 + [p] + [i64] * 6 + [f32] + [p] * 4 + [sz, p, sz, p]),
     "ssla_chunk_gated_delta_rule_bwd": (
-        i32, [p] * 5 + [i32] * 3 + [p] + [i64] * 6 + [f32, p, sz] + [p] * 9 + [sz, p]),
+        i32, [p] * 5 + [i32] * 3 + [p] + [i64] * 6 + [f32, i32, i32, p, sz] + [p] * 9 + [sz, p]),
     "ssla_recurrent_gated_delta_rule_fwd": (i32, [p] * 5 + [i32] * 3 + [p] + [i64] * 6 + [f32] + [p] * 4),
     "ssla_segment_offsets_sorted": (i32, [p, i64, i64, p, p]),
     "ssla_segment_csr_workspace_bytes": (sz, [i64, i64]),

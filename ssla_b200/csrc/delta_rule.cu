@@ -3,100 +3,19 @@
 //   prep        per (chunk, value head): T, PM = Kl^T W, B = Kl^T T beta V, exp(gC)
 //   chain       S' = exp(gC) S - PM S + B along every sequence: the one sequential part
 //   output      per (chunk, value head): O from the start state
-#include "delta_rule.cuh"
+#include "delta_rule_16.cuh"
+#include "delta_rule_inverse.cuh"
 #include "pack_tables.cuh"
 
 namespace ssla {
 namespace delta {
 namespace {
 
-// ------------------------------------------------------------------ (I + A)^-1 of a 64 x 64 tile
-// sA strictly lower triangular -> sT, upper triangle zero; sY is scratch (>= 2048 floats).
-// Diagonal 16 x 16 blocks by substitution (one thread a column), then pairs of blocks twice as
-// large: the block below the diagonal is -T22 A21 T11.
-__device__ __forceinline__ void unit_lower_inverse(const float* sA, float* sT, float* sY) {
-  const int tid = threadIdx.x;
-  for (int i = tid; i < BT * BT; i += THREADS) {
-    const int r = i >> 6, c = i & 63;
-    if ((r >> 4) != (c >> 4)) sT[r * LDC + c] = 0.f;
-  }
-  if (tid < 64) {
-    const int b = (tid >> 4) * 16, c = tid & 15;
-    float x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float acc = i == c ? 1.f : 0.f;
-#pragma unroll
-      for (int j = 0; j < i; ++j) acc = fmaf(-sA[(b + i) * LDC + b + j], x[j], acc);
-      x[i] = acc;
-    }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sT[(b + i) * LDC + b + c] = x[i];
-  }
-  __syncthreads();
-  {  // 16 -> 32, two pairs, 128 threads each: thread = (row, 2 columns)
-    const int p = tid >> 7, u = tid & 127, r = u >> 3, c = (u & 7) * 2, d = 32 * p;
-    float x = 0.f, y = 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float a = sA[(d + 16 + r) * LDC + d + j];
-      x = fmaf(a, sT[(d + j) * LDC + d + c], x);
-      y = fmaf(a, sT[(d + j) * LDC + d + c + 1], y);
-    }
-    sY[p * 256 + r * 16 + c] = x;
-    sY[p * 256 + r * 16 + c + 1] = y;
-    __syncthreads();
-    x = y = 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float a = -sT[(d + 16 + r) * LDC + d + 16 + j];
-      x = fmaf(a, sY[p * 256 + j * 16 + c], x);
-      y = fmaf(a, sY[p * 256 + j * 16 + c + 1], y);
-    }
-    sT[(d + 16 + r) * LDC + d + c] = x;
-    sT[(d + 16 + r) * LDC + d + c + 1] = y;
-  }
-  __syncthreads();
-  {  // 32 -> 64: thread = 2 rows x 2 columns
-    const int r = (tid >> 4) * 2, c = (tid & 15) * 2;
-    float x[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) {
-      const float a0 = sA[(32 + r) * LDC + j], a1 = sA[(33 + r) * LDC + j];
-      const float b0 = sT[j * LDC + c], b1 = sT[j * LDC + c + 1];
-      x[0][0] = fmaf(a0, b0, x[0][0]);
-      x[0][1] = fmaf(a0, b1, x[0][1]);
-      x[1][0] = fmaf(a1, b0, x[1][0]);
-      x[1][1] = fmaf(a1, b1, x[1][1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sY[(r + i) * 33 + c + j] = x[i][j];
-        x[i][j] = 0.f;
-      }
-    __syncthreads();
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) {
-      const float a0 = -sT[(32 + r) * LDC + 32 + j], a1 = -sT[(33 + r) * LDC + 32 + j];
-      const float b0 = sY[j * 33 + c], b1 = sY[j * 33 + c + 1];
-      x[0][0] = fmaf(a0, b0, x[0][0]);
-      x[0][1] = fmaf(a0, b1, x[0][1]);
-      x[1][0] = fmaf(a1, b0, x[1][0]);
-      x[1][1] = fmaf(a1, b1, x[1][1]);
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) sT[(32 + r + i) * LDC + c + j] = x[i][j];
-  }
-  __syncthreads();
-}
-
 // ------------------------------------------------------------------ prep
-template <class TI, int KP> struct PrepSmem {
-  static constexpr int LDK = KTile<TI, KP>::LD, LDV = 72;
+using TI = float;  // 16-bit tokens: delta_rule_16.cu
+
+template <int KP> struct PrepSmem {
+  static constexpr int LDK = KP + 8, LDV = 72;
   TI k[BT * LDK];
   TI v[BT * LDV];
   float a[BT * LDC];
@@ -106,12 +25,12 @@ template <class TI, int KP> struct PrepSmem {
   Gates gates;
 };
 
-template <class TI, int KP, bool SP>
+template <int KP>
 __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong2* __restrict__ tab, int VP,
                                                           float* __restrict__ decay, float* __restrict__ tinv,
                                                           float* __restrict__ pm, float* __restrict__ bout) {
-  using S = PrepSmem<TI, KP>;
-  constexpr bool X = Io16<TI>::exact;
+  using S = PrepSmem<KP>;
+  constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDV = S::LDV;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -206,14 +125,14 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
 struct ChainArgs {
   const float* pm;        // [step * HV + hv][KP][KP]
   const float* b;         // [step * HV + hv][KP][VP]
-  float* s;               // start state of every step ([..][KP][VP]), may be b itself; null: not kept
+  float* s;               // start state of every step ([..][KP][VP], two bf16 planes if planes); null: not kept
   const float* decay;     // per (step, hv); null: S' = PM S + B (composed maps)
   const int* off;         // steps of list n: off[n] .. off[n+1] - 1 ...
   const int4* seg;        // ... or of list n: seg[n].x, seg[n].y steps (seg[n].z < 0: none)
   const float* init;      // [n * HV + hv][K][V] unpadded (padded: [KP][VP])
   float* last;            // likewise
   float* mseg;            // composing: [n * HV + hv][KP][KP] for the columns from VP on, start from I
-  bool init_padded, last_padded, reverse, compose, round;
+  bool init_padded, last_padded, reverse, compose, planes;
   int HV, K, V, VP, slices;
 };
 
@@ -300,8 +219,10 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
       for (int r = 0; r < 4; ++r) bc[j][r] = bn[j][r];
     if (a.s && !ident)
       each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-        *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) =
-            a.round ? make_float2(tf32(x), tf32(y)) : make_float2(x, y);
+        if (a.planes)
+          h16::put_at<2>((h16::bf*)a.s + (2 * it * KP + r) * a.VP + c0 + c, KP * a.VP, x, y);
+        else
+          *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
       });
     cp_wait<0>();
     __syncthreads();  // map i and the state are there, step i - 1 is read
@@ -370,8 +291,8 @@ int chain(ChainArgs a, int KP, int vs, bool trans, bool split, int64_t lists, cu
 }
 
 // ------------------------------------------------------------------ output
-template <class TI, int KP, int VB> struct OutSmem {
-  static constexpr int LDK = KTile<TI, KP>::LD, LDV = VB + 8, LDX = VB + 4;
+template <int KP, int VB> struct OutSmem {
+  static constexpr int LDK = KP + 8, LDV = VB + 8, LDX = VB + 4;
   TI k[BT * LDK];
   TI q[BT * LDK];
   TI v[BT * LDV];
@@ -382,12 +303,12 @@ template <class TI, int KP, int VB> struct OutSmem {
   Gates gates;
 };
 
-template <class TI, int KP, int VB>
+template <int KP, int VB>
 __device__ __forceinline__ void output_chunk(const Args& a, const longlong2* __restrict__ tab, int VP,
                                              const float* __restrict__ tinv, const float* __restrict__ states,
                                              TI* __restrict__ o) {
-  using S = OutSmem<TI, KP, VB>;
-  constexpr bool X = Io16<TI>::exact, SP = OutSplit<TI>::v;
+  using S = OutSmem<KP, VB>;
+  constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDV = S::LDV, LDX = S::LDX, NT = VB / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -465,31 +386,29 @@ __device__ __forceinline__ void output_chunk(const Args& a, const longlong2* __r
   }
 }
 
-template <class TI, int KP, int VB>
+template <int KP, int VB>
 __global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlong2* __restrict__ tab, int VP,
                                                             const float* __restrict__ tinv,
                                                             const float* __restrict__ states, TI* __restrict__ o) {
-  output_chunk<TI, KP, VB>(a, tab, VP, tinv, states, o);
+  output_chunk<KP, VB>(a, tab, VP, tinv, states, o);
   zero_uncovered(o, a, (int64_t)a.HV * a.V);
 }
 
-template <class TI, int KP>
-int run_fwd(const Args& a, const Plan& p, const Saved& sv, const Work& w, int VP, const float* h0, void* o, float* ht,
-            bool split, cudaStream_t st) {
-  const int64_t items = p.MC * a.HV;
-  if (items > 0) {
-    const size_t smem = sizeof(PrepSmem<TI, KP>);
-    auto* prep = split ? prep_kernel<TI, KP, true> : prep_kernel<TI, KP, OutSplit<TI>::v>;
-    cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    prep<<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, sv.tinv, sv.pm, sv.s);
-    SSLA_CHECK_LAUNCH("gated_delta_rule prep");
-  }
-  int rc = run_chain(p, sv, w, sv.s, h0, ht, a.N, a.HV, a.K, a.V, false, split, !OutSplit<TI>::v, st);
-  if (rc || a.T == 0) return rc;
+template <int KP>
+int prep32(const Args& a, const Saved& sv, int VP, float* inc, int64_t items, cudaStream_t st) {
+  const size_t smem = sizeof(PrepSmem<KP>);
+  cudaFuncSetAttribute(prep_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  prep_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, sv.tinv, sv.pm, inc);
+  SSLA_CHECK_LAUNCH("gated_delta_rule prep");
+  return SSLA_OK;
+}
+
+template <int KP>
+int output32(const Args& a, const Saved& sv, int VP, void* o, int64_t items, cudaStream_t st) {
   constexpr int VB = KP == 64 ? 64 : 32;
-  const size_t smem = sizeof(OutSmem<TI, KP, VB>);
-  cudaFuncSetAttribute(output_kernel<TI, KP, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  output_kernel<TI, KP, VB><<<(unsigned)(items > 0 ? items : 1), THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.s, (TI*)o);
+  const size_t smem = sizeof(OutSmem<KP, VB>);
+  cudaFuncSetAttribute(output_kernel<KP, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  output_kernel<KP, VB><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.s, (TI*)o);
   SSLA_CHECK_LAUNCH("gated_delta_rule output");
   return SSLA_OK;
 }
@@ -541,24 +460,24 @@ Args make_args(const void* q, const void* k, const void* v, const void* g, const
 }
 
 int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const float* init, float* last, int64_t N,
-              int HV, int K, int V, bool reverse, bool split, bool round, cudaStream_t st) {
+              int HV, int K, int V, bool reverse, bool exact, bool planes, cudaStream_t st) {
   ChainArgs c = {};
   c.HV = HV;
   c.K = K;
   c.V = V;
   c.VP = pad_v(V);
   c.reverse = reverse;
-  c.round = round;
+  c.planes = planes;
   const int KP = pad_k(K);
   c.pm = sv.pm;
-  c.b = s;
+  c.b = w.inc;
   c.s = s;
   c.decay = sv.decay;
   if (!p.len) {
     c.off = sv.chunk_off;
     c.init = init;
     c.last = last;
-    return chain(c, KP, p.vs, reverse, split, N, st);
+    return chain(c, KP, p.vs, reverse, exact, N, st);
   }
   // compose the maps of every segment, run along the segments, run inside them
   ChainArgs d = c;
@@ -568,7 +487,7 @@ int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const flo
   d.mseg = w.mseg;
   d.last = w.bseg;
   d.last_padded = true;
-  int rc = chain(d, KP, p.vs_seg, reverse, split, p.MS, st);
+  int rc = chain(d, KP, p.vs_seg, reverse, exact, p.MS, st);
   if (rc) return rc;
   d = c;
   d.pm = w.mseg;
@@ -577,12 +496,12 @@ int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const flo
   d.off = sv.seg_off;
   d.init = init;
   d.last = last;
-  d.round = false;
-  if ((rc = chain(d, KP, 16, false, split, N, st))) return rc;
+  d.planes = false;
+  if ((rc = chain(d, KP, 16, false, exact, N, st))) return rc;
   c.seg = sv.seg_tab;
   c.init = w.bseg;
   c.init_padded = true;
-  return chain(c, KP, p.vs_seg, reverse, split, p.MS, st);
+  return chain(c, KP, p.vs_seg, reverse, exact, p.MS, st);
 }
 
 }  // namespace delta
@@ -591,10 +510,11 @@ int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const flo
 using namespace ssla;
 using namespace ssla::delta;
 
-extern "C" size_t ssla_gated_delta_rule_states_bytes(int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K,
-                                                     int64_t V) {
+extern "C" size_t ssla_gated_delta_rule_states_bytes(int dtype, int64_t n_seqs, int64_t T, int64_t H, int64_t HV,
+                                                     int64_t K, int64_t V, int has_h0, int has_ht) {
   if (n_seqs < 0 || T < 0 || H < 0 || HV < 0 || K < 1 || V < 1) return 0;
-  return saved_layout(nullptr, make_plan(n_seqs, T, HV, K, V), n_seqs, HV, pad_k(K), pad_v(V), nullptr);
+  return saved_layout(nullptr, make_plan(n_seqs, T, HV, K, V), dtype, exact_states(dtype, has_h0, has_ht), n_seqs, HV,
+                      pad_k(K), pad_v(V), nullptr);
 }
 
 extern "C" size_t ssla_gated_delta_rule_workspace_bytes(int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K,
@@ -617,9 +537,10 @@ extern "C" int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, con
   SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "%s: null pointer", name);
   const Plan p = make_plan(n_seqs, T, HV, K, V);
   const int KP = pad_k(K), VP = pad_v(V);
+  const bool exact = exact_states(dtype, h0, ht);
   Saved sv;
   Work w;
-  const size_t need = saved_layout(states, p, n_seqs, HV, KP, VP, &sv);
+  const size_t need = saved_layout(states, p, dtype, exact, n_seqs, HV, KP, VP, &sv);
   const size_t need_w = work_layout(workspace, p, T, H, HV, K, KP, VP, false, &w);
   if (states_bytes < need || workspace_bytes < need_w || (need_w && !workspace)) {
     set_error("%s: states of %zu bytes and workspace of %zu, %zu and %zu needed", name, states_bytes, workspace_bytes,
@@ -632,9 +553,17 @@ extern "C" int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, con
                           sv.seg_tab, st);
   if (rc) return rc;
   const Args a = make_args(q, k, v, g, beta, dtype, dtype_g, dtype_beta, cu_seqlens, n_seqs, T, H, HV, K, V, scale);
-  const bool split = state_split(dtype, h0, ht);
-  return SSLA_DISPATCH_DTYPE(dtype, T_, [&] {
-    return KP == 64 ? run_fwd<T_, 64>(a, p, sv, w, VP, h0, o, ht, split, st)
-                    : run_fwd<T_, 128>(a, p, sv, w, VP, h0, o, ht, split, st);
-  });
+  const int64_t items = p.MC * HV, blocks = items > 0 ? items : 1;
+  const bool f32 = dtype == SSLA_F32;
+  if (items > 0) {
+    rc = !f32      ? prep16(dtype, a, sv, KP, VP, exact, w.inc, items, st)
+         : KP == 64 ? prep32<64>(a, sv, VP, w.inc, items, st)
+                    : prep32<128>(a, sv, VP, w.inc, items, st);
+    if (rc) return rc;
+  }
+  rc = run_chain(p, sv, w, sv.s, h0, ht, n_seqs, (int)HV, (int)K, (int)V, false, exact, !f32, st);
+  if (rc || T == 0) return rc;
+  return !f32       ? output16(dtype, a, sv, KP, VP, exact, o, blocks, st)
+         : KP == 64 ? output32<64>(a, sv, VP, o, blocks, st)
+                    : output32<128>(a, sv, VP, o, blocks, st);
 }

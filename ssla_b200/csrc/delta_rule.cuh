@@ -44,10 +44,17 @@ struct Plan {
 };
 Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V);
 
-// What the forward leaves for the backward (caller's `states` buffer), all padded to KP x VP:
+// Whether the states leave in fp32, so that everything behind them keeps fp32 accuracy; else their
+// only readers are bf16 outputs.  (h0 given: its gradient may be asked for.)
+inline bool exact_states(int dtype, bool h0, bool ht) { return dtype != SSLA_BF16 || h0 || ht; }
+// bf16 planes of T for 16-bit tokens (delta_rule_16.cuh)
+inline int t_planes(bool exact) { return exact ? 3 : 2; }
+
+// What the forward leaves for the backward (caller's `states` buffer), states padded to KP x VP:
 //   chunk_off [N+1], seg_off [N+1] (device), chunk_tab [MC] {first token, rows | seq << 32},
-//   seg_tab [MS] {first chunk, chunks, seq}; per (chunk, value head) item: decay = exp(gC),
-//   tinv [64,64] = T, pm [KP,KP] and s [KP,VP] = state at the chunk's start (B before the scan).
+//   seg_tab [MS] {first chunk, chunks, seq}; per (chunk, value head) item: decay = exp(gC);
+//   tinv: T, fp32 [64,64], or for 16-bit tokens planes of T and T^T in fragment order;
+//   pm [KP,KP]; s [KP,VP] = state at the chunk's start, fp32, or for 16-bit tokens two bf16 planes.
 struct Saved {
   int* chunk_off;
   int* seg_off;
@@ -59,7 +66,8 @@ struct Saved {
   float* s;
 };
 
-inline size_t saved_layout(void* base, const Plan& p, int64_t N, int64_t HV, int KP, int VP, Saved* out) {
+inline size_t saved_layout(void* base, const Plan& p, int dtype, bool exact, int64_t N, int64_t HV, int KP, int VP,
+                           Saved* out) {
   char* q = (char*)base;
   const size_t items = (size_t)p.MC * HV;
   auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
@@ -69,16 +77,18 @@ inline size_t saved_layout(void* base, const Plan& p, int64_t N, int64_t HV, int
   s.chunk_tab = (longlong2*)take(16 * (size_t)p.MC);
   s.seg_tab = (int4*)take(16 * (size_t)p.MS);
   s.decay = (float*)take(4 * items);
-  s.tinv = (float*)take(4 * items * BT * BT);
+  s.tinv = (float*)take((dtype == SSLA_F32 ? 4 : 4 * t_planes(exact)) * items * BT * BT);
   s.pm = (float*)take(4 * items * KP * KP);
   s.s = (float*)take(4 * items * KP * VP);
   if (out) *out = s;
   return (size_t)(q - (char*)base);
 }
 
-// Scratch of one call: the composed maps of the segments; the backward's adjoint states and, when
-// value heads share key heads, fp32 dq and dk of every value head.
+// Scratch of one call: the increments of the chunk maps (B or dB); the composed maps of the segments;
+// for the backward the adjoint states (laid out as s) and, when value heads share key heads, fp32 dq
+// and dk of every value head.
 struct Work {
+  float* inc;   // [MC*HV, KP, VP]
   float* mseg;  // [MS*HV, KP, KP]
   float* bseg;  // [MS*HV, KP, VP]
   float* ds;    // [MC*HV, KP, VP]
@@ -90,10 +100,11 @@ inline size_t work_layout(void* base, const Plan& p, int64_t T, int64_t H, int64
   char* q = (char*)base;
   auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
   Work w;
-  const size_t segs = p.len ? (size_t)p.MS * HV : 0;
+  const size_t segs = p.len ? (size_t)p.MS * HV : 0, states = 4 * (size_t)p.MC * HV * KP * VP;
+  w.inc = (float*)take(states);
   w.mseg = (float*)take(4 * segs * KP * KP);
   w.bseg = (float*)take(4 * segs * KP * VP);
-  w.ds = (float*)take(bwd ? 4 * (size_t)p.MC * HV * KP * VP : 0);
+  w.ds = (float*)take(bwd ? states : 0);
   w.dqk = (float*)take(bwd && HV != H ? 8 * (size_t)T * HV * K : 0);
   if (out) *out = w;
   return (size_t)(q - (char*)base);
@@ -323,18 +334,6 @@ __device__ __forceinline__ void load_gates(Gates& s, const Args& a, int64_t t0, 
   if (lane == 0) s.whole = expf((float)all);
 }
 
-template <class TI> struct Io16 { static constexpr bool exact = true; };
-template <> struct Io16<float> { static constexpr bool exact = false; };
-// Products whose results leave in bf16 only need less than bf16's own rounding (2^-8): one TF32
-// product (2^-11 per operand).  fp16 and fp32 results need the split.
-template <class TI> struct OutSplit { static constexpr bool v = true; };
-template <> struct OutSplit<__nv_bfloat16> { static constexpr bool v = false; };
-// The states themselves: split unless every output that depends on them leaves in bf16, that is
-// bf16 tokens without a final state or a gradient of the initial one.
-inline bool state_split(int dtype, const void* h0, const void* ht) { return dtype != SSLA_BF16 || h0 || ht; }
-
-template <class TI, int KP> struct KTile { static constexpr int LD = KP + 8; };
-
 __device__ __forceinline__ bool locate(const longlong2* tab, int64_t MC, int64_t chunk, int64_t& t0, int& rows) {
   if (chunk >= MC) return false;
   const longlong2 e = tab[chunk];
@@ -354,18 +353,47 @@ __device__ __forceinline__ void zero_uncovered(TO* out, const Args& a, int64_t n
     out[i < head ? i : e * n + (i - head)] = TO(0.f);
 }
 
+struct Grads {
+  const void* dout;
+  void *dq, *dk, *dv, *dg, *dbeta;
+  float* dqk;  // [2, T, HV, K] instead of dq, dk where value heads share key heads; else null
+};
+template <class TI>
+__device__ __forceinline__ void zero_gradients(const Args& a, TI* dq, TI* dk, TI* dv, void* dg, void* dbeta, float* dqk) {
+  if (dqk) {
+    zero_uncovered(dqk, a, (int64_t)a.HV * a.K);
+    zero_uncovered(dqk + (size_t)a.T * a.HV * a.K, a, (int64_t)a.HV * a.K);
+  } else {
+    zero_uncovered(dq, a, (int64_t)a.H * a.K);
+    zero_uncovered(dk, a, (int64_t)a.H * a.K);
+  }
+  zero_uncovered(dv, a, (int64_t)a.HV * a.V);
+  if (a.dt_g == SSLA_F32) zero_uncovered((float*)dg, a, a.HV);
+  else zero_uncovered((__half*)dg, a, a.HV);  // 0 has the same bits in both 16-bit types
+  if (a.dt_b == SSLA_F32) zero_uncovered((float*)dbeta, a, a.HV);
+  else zero_uncovered((__half*)dbeta, a, a.HV);
+}
+
 // delta_rule.cu
 int check_args(const char* name, int dtype, int dtype_g, int dtype_b, int64_t N, int64_t T, int64_t H, int64_t HV,
                int64_t K, int64_t V);
 Args make_args(const void* q, const void* k, const void* v, const void* g, const void* beta, int dtype, int dtype_g,
                int dtype_b, const int64_t* cu, int64_t N, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,
                float scale);
-// The affine chunk maps along every sequence: forward S' = decay S - PM S + B (s: B in, start states
-// out), reverse the adjoint with PM^T (s: dB in, adjoint of every chunk's end state out).
-// split: products at fp32 accuracy; round: the states kept for the per-chunk kernels are rounded to
-// TF32, which is all that their single products read.
+// The affine chunk maps along every sequence, from their increments w.inc: forward S' = decay S - PM S + B
+// (s: start states), reverse the adjoint with PM^T (s: adjoint of every chunk's end state).  exact:
+// products at fp32 accuracy; planes: s in two bf16 planes instead of fp32.
 int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const float* init, float* last, int64_t N,
-              int HV, int K, int V, bool reverse, bool split, bool round, cudaStream_t st);
+              int HV, int K, int V, bool reverse, bool exact, bool planes, cudaStream_t st);
+// delta_rule_16.cu, delta_rule_16_bwd.cu: the per-chunk kernels of 16-bit tokens
+int prep16(int dtype, const Args& a, const Saved& sv, int KP, int VP, bool exact, float* inc, int64_t items,
+           cudaStream_t st);
+int output16(int dtype, const Args& a, const Saved& sv, int KP, int VP, bool exact, void* o, int64_t items,
+             cudaStream_t st);
+int adjoint16(int dtype, const Args& a, const Saved& sv, int KP, int VP, int planes, const void* dout, float* inc,
+              int64_t items, cudaStream_t st);
+int backward16(int dtype, const Args& a, const Saved& sv, int KP, int VP, int planes, const void* ds, const Grads& g,
+               int64_t items, cudaStream_t st);
 
 }  // namespace delta
 }  // namespace ssla

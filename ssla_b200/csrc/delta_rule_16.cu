@@ -1,0 +1,337 @@
+// Chunked gated delta rule for bf16 and fp16 tokens: prep and output kernels on bf16 planes
+// (delta_rule_16.cuh; the formulas are in delta_rule.cuh).  The chain between them is delta_rule.cu's.
+#include "delta_rule_16.cuh"
+#include "delta_rule_inverse.cuh"
+
+namespace ssla {
+namespace delta {
+namespace {
+
+using namespace h16;
+
+// ------------------------------------------------------------------ prep
+// NI planes of intermediate results: 3 where the states leave in fp32, else 2.
+template <class TI, int KP, int NI> struct Prep16 {
+  static constexpr int NT = Planes<TI>::n, LDK = KP + 8;
+  bf k[NT * BT * LDK];
+  bf v[NT * BT * LDT];
+  union {
+    float a[BT * LDC];     // A; once inverted
+    bf tc[NI * BT * LDT];  // planes of T diag(..)
+  };
+  float t[BT * LDC];
+  bf y[(NI > 2 ? NI : 2) * BT * LDT];  // scratch of the inverse, then planes of a panel
+  float col[BT];
+  Gates gates;
+};
+
+// Planes of T and of its transpose in fragment order.
+template <int NI> __device__ __forceinline__ void write_t(const float* t, bf* out) {
+  for (int i = threadIdx.x; i < 2 * 16 * 32; i += THREADS) {
+    const int lane = i & 31, kb = (i >> 5) & 3, mb = (i >> 7) & 3, tr = i >> 9;
+    const int r = 16 * mb + (lane >> 2), c = 16 * kb + 2 * (lane & 3);
+    uint32_t w[NI][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int rr = r + (j & 1) * 8, cc = c + (j >> 1) * 8;
+      float x = tr ? t[cc * LDC + rr] : t[rr * LDC + cc];
+      float y = tr ? t[(cc + 1) * LDC + rr] : t[rr * LDC + cc + 1];
+#pragma unroll
+      for (int p = 0; p < NI; ++p) {
+        w[p][j] = pack(x, y);
+        rest(w[p][j], x, y);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < NI; ++p)
+      reinterpret_cast<uint4*>(out)[((tr * NI + p) * 16 + mb * 4 + kb) * 32 + lane] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+  }
+}
+
+template <class TI, int KP, int NI>
+__global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 1024 ? 3 : sizeof(Prep16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
+    prep16_kernel(Args a, const longlong2* __restrict__ tab, int VP, float* __restrict__ decay, bf* __restrict__ tinv,
+                  float* __restrict__ pm, float* __restrict__ bout) {
+  using S = Prep16<TI, KP, NI>;
+  constexpr int N = S::NT, LDK = S::LDK, PLK = BT * LDK, PLT = BT * LDT;
+  extern __shared__ __align__(16) unsigned char raw[];
+  S& s = *reinterpret_cast<S*>(raw);
+  const int64_t chunk = blockIdx.x / a.HV;
+  const int hv = (int)(blockIdx.x - chunk * a.HV), h = hv / a.R;
+  const size_t item = blockIdx.x;
+  int64_t t0;
+  int rows;
+  if (!locate(tab, a.MC, chunk, t0, rows)) return;
+  const int warp = threadIdx.x >> 5;
+  load_tokens<TI, LDK, KP, THREADS>(s.k, (const TI*)a.k + ((size_t)t0 * a.H + h) * a.K, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  auto load_v = [&](int v0) {
+    load_tokens<TI, LDT, 64, THREADS>(s.v, (const TI*)a.v + ((size_t)t0 * a.HV + hv) * a.V + v0, (size_t)a.HV * a.V,
+                                      rows, a.V - v0, a.vec_v);
+    cp_commit();
+  };
+  load_v(0);
+  if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
+  cp_wait<0>();
+  __syncthreads();
+  if (threadIdx.x == 0) decay[item] = s.gates.whole;
+  const int m0 = (warp >> 1) * 16, n0 = (warp & 1) * 32;
+  {
+    float acc[1][4][4];
+    zero(acc);
+    if (n0 <= m0) mm(acc, RowA<LDK, PLK, N>(s.k), ColB<LDK, PLK, N>(s.k), m0, n0, 0, KP);
+    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
+      const float b = s.gates.beta[i];
+      *reinterpret_cast<float2*>(s.a + i * LDC + j) =
+          make_float2(i > j ? b * s.gates.fade(i, j) * x : 0.f, i > j + 1 ? b * s.gates.fade(i, j + 1) * y : 0.f);
+    });
+  }
+  __syncthreads();
+  unit_lower_inverse(s.a, s.t, reinterpret_cast<float*>(s.y));
+  write_t<NI>(s.t, tinv + item * (2 * NI * BT * BT));
+  auto scale_t = [&](bool w) {  // tc = T diag(beta [exp(gc)])
+    for (int i = threadIdx.x; i < BT * BT / 2; i += THREADS) {
+      const int r = i >> 5, c = (i & 31) * 2;
+      const float2 x = pair(s.t + r * LDC + c), b = pair(s.gates.beta + c), e = pair(s.gates.start + c);
+      put<NI, PLT>(s.tc + r * LDT + c, x.x * b.x * (w ? e.x : 1.f), x.y * b.y * (w ? e.y : 1.f));
+    }
+  };
+  scale_t(true);
+  __syncthreads();
+  const int panels = KP / 64 + VP / 64;
+  for (int p = 0; p < panels; ++p) {
+    const bool w = p < KP / 64;
+    const int c0 = (w ? p : p - KP / 64) * 64;
+    if (!w && (c0 == 0 || VP > 64)) {
+      if (p > KP / 64) load_v(c0);
+      if (c0 == 0) scale_t(false);
+      cp_wait<0>();
+      __syncthreads();
+    }
+    {
+      float acc[1][4][4];
+      zero(acc);
+      const RowA<LDT, PLT, NI> t(s.tc);
+      if (w) mm(acc, t, RowB<LDK, PLK, N>(s.k + c0), m0, n0, 0, m0 + 16);
+      else mm(acc, t, RowB<LDT, PLT, N>(s.v), m0, n0, 0, m0 + 16);
+      each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
+        const float l = s.gates.left[i];
+        put<NI, PLT>(s.y + i * LDT + j, x * l, y * l);
+      });
+    }
+    __syncthreads();
+    {
+      constexpr int MT = KP / 64;
+      float acc[MT][4][4];
+      zero(acc);
+      const int mk = (warp >> 1) * 16 * MT;
+      mm(acc, ColA<LDK, PLK, N>(s.k), RowB<LDT, PLT, NI>(s.y), mk, n0, 0, BT);
+      float* out = w ? pm + item * KP * KP : bout + item * KP * VP;
+      const int ld = w ? KP : VP;
+      each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
+        *reinterpret_cast<float2*>(out + (size_t)m * ld + c0 + n) = w ? stage2<(NI > 2)>(x, y) : make_float2(x, y);
+      });
+    }
+    __syncthreads();  // the readers of v, tc and y are done
+  }
+}
+
+// ------------------------------------------------------------------ output
+// Four warps, 16 rows each over all columns: the scores P stay in registers as left operand.
+constexpr int TH4 = 128;
+
+template <class TI, int KP, int VB> struct Out16 {
+  static constexpr int N = Planes<TI>::n, LDK = KP + 8, LDX = VB + 8;
+  bf k[N * BT * LDK];
+  bf q[N * BT * LDK];
+  bf t[2 * BT * BT];  // fragment order
+  bf s[2 * KP * LDX];
+  bf x[2 * BT * LDX];
+  Gates gates;
+};
+
+template <class TI, int KP, int VB>
+__device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* __restrict__ tab, int VP, int tplanes,
+                                               const bf* __restrict__ tinv, const bf* __restrict__ states,
+                                               TI* __restrict__ o) {
+  using S = Out16<TI, KP, VB>;
+  constexpr int N = S::N, LDK = S::LDK, LDX = S::LDX, PLK = BT * LDK, PLX = BT * LDX, NT = VB / 8;
+  extern __shared__ __align__(16) unsigned char raw[];
+  S& s = *reinterpret_cast<S*>(raw);
+  const int64_t chunk = blockIdx.x / a.HV;
+  const int hv = (int)(blockIdx.x - chunk * a.HV), h = hv / a.R;
+  const size_t item = blockIdx.x;
+  int64_t t0;
+  int rows;
+  if (!locate(tab, a.MC, chunk, t0, rows)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m0 = warp * 16;
+  const size_t qk = ((size_t)t0 * a.H + h) * a.K;
+  load_tokens<TI, LDK, KP, TH4>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  load_tokens<TI, LDK, KP, TH4>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  cp_commit();
+  copy16<TH4>(s.t, tinv + item * (2 * (size_t)tplanes * BT * BT), 2 * FRAG_PLANE);
+  const bf* st = states + item * (2 * KP * VP);
+  load_planes<LDX, KP, VB, TH4>(s.s, st, VP);
+  cp_commit();
+  if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
+  cp_wait<1>();
+  __syncthreads();
+  uint32_t pf[4][2][4];  // planes of the warp's rows of P, by blocks of 16 columns
+  const int i0 = m0 + (lane >> 2);
+  {
+    const RowA<LDK, PLK, N> qa(s.q);
+    const ColB<LDK, PLK, N> kb(s.k);
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (b <= warp) {
+        float c[1][2][4];
+        zero(c);
+        mm(c, qa, kb, m0, 16 * b, 0, KP);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = 16 * b + 8 * j + 2 * (lane & 3);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int i = i0 + 8 * r;
+            float x = i >= col ? fade16(s.gates, i, col) * c[0][j][2 * r] : 0.f;
+            float y = i > col ? fade16(s.gates, i, col + 1) * c[0][j][2 * r + 1] : 0.f;
+            const uint32_t w = pack(x, y);
+            rest(w, x, y);
+            pf[b][0][2 * j + r] = w;
+            pf[b][1][2 * j + r] = pack(x, y);
+          }
+        }
+      }
+  }
+  const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]};
+  const float ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]};
+  const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
+  const TI* gv = (const TI*)a.v + vo;
+  const bool even = a.V % 2 == 0 && (reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(o)) % 4 == 0;
+  for (int v0 = 0; v0 < a.V; v0 += VB) {
+    if (v0) {
+      __syncthreads();  // readers of the previous panel are done
+      load_planes<LDX, KP, VB, TH4>(s.s, st + v0, VP);
+      cp_commit();
+    }
+    float xv[1][NT][4];
+    each_pair(xv, m0, 0, [&](int i, int n, float& x, float& y) {
+      const int c = v0 + n;
+      x = y = 0.f;
+      if (i < rows) {
+        const TI* p = gv + i * vstride + c;
+        if (even) {
+          if (c < a.V) {
+            const float2 z = pair(p);
+            x = z.x;
+            y = z.y;
+          }
+        } else {
+          if (c < a.V) x = ldf(p);
+          if (c + 1 < a.V) y = ldf(p + 1);
+        }
+      }
+    });
+    cp_wait<0>();
+    __syncthreads();
+    float aq[1][NT][4], ak[1][NT][4];
+    zero(aq);
+    zero(ak);
+    const RowB<LDX, KP * LDX, 2> sb(s.s);
+    mm(ak, RowA<LDK, PLK, N>(s.k), sb, m0, 0, 0, KP);
+    mm(aq, RowA<LDK, PLK, N>(s.q), sb, m0, 0, 0, KP);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        put<2, PLX>(s.x + (i0 + 8 * r) * LDX + 8 * j + 2 * (lane & 3),
+                    be[r] * (xv[0][j][2 * r] - ee[r] * ak[0][j][2 * r]),
+                    be[r] * (xv[0][j][2 * r + 1] - ee[r] * ak[0][j][2 * r + 1]));
+    __syncthreads();
+    zero(ak);
+    const RowB<LDX, PLX, 2> xb(s.x);
+    mm(ak, FragA<2>(s.t), xb, m0, 0, 0, m0 + 16);
+    __syncthreads();
+    each_pair(ak, m0, 0, [&](int i, int n, float x, float y) { put<2, PLX>(s.x + i * LDX + n, x, y); });
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) aq[0][j][r] *= ee[r >> 1];
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (b <= warp) {
+#pragma unroll
+        for (int j = 0; j < NT; j += 2) {
+          uint32_t f0[4], f1[4];
+          xb.load(f0, 16 * b, 8 * j, 0);
+          xb.load(f1, 16 * b, 8 * j, 1);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            mma16(aq[0][j + u], pf[b][1], f0[2 * u], f0[2 * u + 1]);
+            mma16(aq[0][j + u], pf[b][0], f1[2 * u], f1[2 * u + 1]);
+            mma16(aq[0][j + u], pf[b][0], f0[2 * u], f0[2 * u + 1]);
+          }
+        }
+      }
+    each_pair(aq, m0, 0, [&](int i, int n, float x, float y) {
+      const int c = v0 + n;
+      if (i < rows && c < a.V) {
+        TI* p = o + vo + i * vstride + c;
+        if (even) {
+          store2(p, x * a.scale, y * a.scale);
+        } else {
+          stf(p, x * a.scale);
+          if (c + 1 < a.V) stf(p + 1, y * a.scale);
+        }
+      }
+    });
+  }
+}
+
+template <class TI, int KP, int VB>
+__global__ void __launch_bounds__(TH4, sizeof(Out16<TI, KP, VB>) <= 75 * 1024 ? 3 : 2)
+    output16_kernel(Args a, const longlong2* __restrict__ tab, int VP, int tplanes, const bf* __restrict__ tinv,
+                    const bf* __restrict__ states, TI* __restrict__ o) {
+  output16_chunk<TI, KP, VB>(a, tab, VP, tplanes, tinv, states, o);
+  zero_uncovered(o, a, (int64_t)a.HV * a.V);
+}
+
+template <class TI, int KP, int NI>
+int prep(const Args& a, const Saved& sv, int VP, float* b, int64_t items, cudaStream_t st) {
+  const size_t smem = sizeof(Prep16<TI, KP, NI>);
+  cudaFuncSetAttribute(prep16_kernel<TI, KP, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  prep16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, (bf*)sv.tinv, sv.pm, b);
+  SSLA_CHECK_LAUNCH("gated_delta_rule prep");
+  return SSLA_OK;
+}
+
+template <class TI, int KP>
+int output(const Args& a, const Saved& sv, int VP, bool exact, void* o, int64_t items, cudaStream_t st) {
+  constexpr int VB = KP == 64 ? 64 : 32;
+  const size_t smem = sizeof(Out16<TI, KP, VB>);
+  cudaFuncSetAttribute(output16_kernel<TI, KP, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  output16_kernel<TI, KP, VB><<<(unsigned)items, TH4, smem, st>>>(a, sv.chunk_tab, VP, exact ? 3 : 2, (const bf*)sv.tinv,
+                                                                 (const bf*)sv.s, (TI*)o);
+  SSLA_CHECK_LAUNCH("gated_delta_rule output");
+  return SSLA_OK;
+}
+
+}  // namespace
+
+int prep16(int dtype, const Args& a, const Saved& sv, int KP, int VP, bool exact, float* b, int64_t items,
+           cudaStream_t st) {
+  if (dtype == SSLA_F16)
+    return KP == 64 ? prep<__half, 64, 3>(a, sv, VP, b, items, st) : prep<__half, 128, 3>(a, sv, VP, b, items, st);
+  if (exact) return KP == 64 ? prep<bf, 64, 3>(a, sv, VP, b, items, st) : prep<bf, 128, 3>(a, sv, VP, b, items, st);
+  return KP == 64 ? prep<bf, 64, 2>(a, sv, VP, b, items, st) : prep<bf, 128, 2>(a, sv, VP, b, items, st);
+}
+
+int output16(int dtype, const Args& a, const Saved& sv, int KP, int VP, bool exact, void* o, int64_t items,
+             cudaStream_t st) {
+  if (dtype == SSLA_F16)
+    return KP == 64 ? output<__half, 64>(a, sv, VP, exact, o, items, st) : output<__half, 128>(a, sv, VP, exact, o, items, st);
+  return KP == 64 ? output<bf, 64>(a, sv, VP, exact, o, items, st) : output<bf, 128>(a, sv, VP, exact, o, items, st);
+}
+
+}  // namespace delta
+}  // namespace ssla

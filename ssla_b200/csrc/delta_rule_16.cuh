@@ -1,0 +1,216 @@
+// Products of the per-chunk kernels for 16-bit tokens (delta_rule_16.cu, delta_rule_16_bwd.cu).
+//
+// Every operand is a sum of bf16 planes: bf16 tokens are one plane, fp16 tokens two (exact),
+// intermediate results x = p0 + p1 (+ p2), each plane the bf16 rounding of what the planes before
+// leave, so two planes hold 16 bits and three 24.  A product keeps the plane pairs (i, j) with
+// i + j < max(planes): 2 MMAs for token x 2 planes, 3 for 2 x 2, 3 for token x 3, 6 for 3 x 3.  The
+// planes lie in shared memory as 16-bit tiles with rows 8 elements longer than the matrix (16-byte
+// rows at odd multiples of 16: ldmatrix without bank conflicts), and ldmatrix with or without
+// transposition reads either orientation of a tile as either operand, four 8x8 blocks an
+// instruction.  Against TF32 products (11-bit operands of 4 bytes, one 32-bit load for every
+// operand register) the same tensor time carries 16 bits and a third of the instructions: the
+// output kernel of 8 x 2048 tokens, 4 heads of 64, went from 41 to 17 us.
+#pragma once
+#include "delta_rule.cuh"
+
+namespace ssla {
+namespace delta {
+namespace h16 {
+
+using bf = __nv_bfloat16;
+constexpr int LDT = BT + 8;  // rows of [64, 64] tiles
+
+template <class TI> struct Planes;  // of a token tile
+template <> struct Planes<__nv_bfloat16> { static constexpr int n = 1; };
+template <> struct Planes<__half> { static constexpr int n = 2; };
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Left operand, 16 x 16 blocks at (m, k).  RowA: stored [m][k].  ColA: stored [k][m].
+template <int LD, int PLANE, int N> struct RowA {
+  static constexpr int n = N;
+  uint32_t at;
+  __device__ __forceinline__ RowA(const bf* p) {
+    const int l = threadIdx.x & 31;
+    at = smem_u32(p + (l & 15) * LD + (l >> 4) * 8);
+  }
+  __device__ __forceinline__ void load(uint32_t (&r)[4], int m, int k, int p) const {
+    ldsm4(r, at + 2 * (p * PLANE + m * LD + k));
+  }
+};
+template <int LD, int PLANE, int N> struct ColA {
+  static constexpr int n = N;
+  uint32_t at;
+  __device__ __forceinline__ ColA(const bf* p) {
+    const int l = threadIdx.x & 31;
+    at = smem_u32(p + ((l & 7) + (l >> 4) * 8) * LD + ((l >> 3) & 1) * 8);
+  }
+  __device__ __forceinline__ void load(uint32_t (&r)[4], int m, int k, int p) const {
+    ldsm4t(r, at + 2 * (p * PLANE + k * LD + m));
+  }
+};
+// Fragments in order: [plane][m / 16][k / 16][lane] of 16 bytes (a [64, 64] matrix).
+template <int N> struct FragA {
+  static constexpr int n = N;
+  const uint4* at;
+  __device__ __forceinline__ FragA(const void* p) : at((const uint4*)p + (threadIdx.x & 31)) {}
+  __device__ __forceinline__ void load(uint32_t (&r)[4], int m, int k, int p) const {
+    const uint4 x = at[((p * 4 + (m >> 4)) * 4 + (k >> 4)) * 32];
+    r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
+  }
+};
+// Right operand, 16 x 16 blocks at (k, n).  RowB: stored [k][n].  ColB: stored [n][k].
+template <int LD, int PLANE, int N> struct RowB {
+  static constexpr int n = N;
+  uint32_t at;
+  __device__ __forceinline__ RowB(const bf* p) {
+    const int l = threadIdx.x & 31;
+    at = smem_u32(p + ((l & 7) + ((l >> 3) & 1) * 8) * LD + (l >> 4) * 8);
+  }
+  __device__ __forceinline__ void load(uint32_t (&r)[4], int k, int c, int p) const {
+    ldsm4t(r, at + 2 * (p * PLANE + k * LD + c));
+  }
+};
+template <int LD, int PLANE, int N> struct ColB {
+  static constexpr int n = N;
+  uint32_t at;
+  __device__ __forceinline__ ColB(const bf* p) {
+    const int l = threadIdx.x & 31;
+    at = smem_u32(p + ((l & 7) + (l >> 4) * 8) * LD + ((l >> 3) & 1) * 8);
+  }
+  __device__ __forceinline__ void load(uint32_t (&r)[4], int k, int c, int p) const {
+    ldsm4(r, at + 2 * (p * PLANE + c * LD + k));
+  }
+};
+
+// acc += A B over k in [k0, k1) (multiples of 16), columns n0 .. n0 + 8 NT
+template <int MT, int NT, class A, class B>
+__device__ __forceinline__ void mm(float (&acc)[MT][NT][4], const A& a, const B& b, int m0, int n0, int k0, int k1) {
+  static_assert(NT % 2 == 0, "columns come in pairs of tiles");
+  constexpr int MOST = A::n > B::n ? A::n : B::n;
+#pragma unroll 4
+  for (int k = k0; k < k1; k += 16) {
+    uint32_t fa[MT][A::n][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int p = 0; p < A::n; ++p) a.load(fa[i][p], m0 + 16 * i, k, p);
+#pragma unroll
+    for (int j = 0; j < NT; j += 2) {
+      uint32_t fb[B::n][4];
+#pragma unroll
+      for (int p = 0; p < B::n; ++p) b.load(fb[p], k, n0 + 8 * j, p);
+#pragma unroll
+      for (int s = MOST - 1; s >= 0; --s)  // small products first
+#pragma unroll
+        for (int p = 0; p <= s; ++p)
+          if (p < A::n && s - p < B::n)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              mma16(acc[i][j], fa[i][p], fb[s - p][0], fb[s - p][1]);
+              mma16(acc[i][j + 1], fa[i][p], fb[s - p][2], fb[s - p][3]);
+            }
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t pack(float x, float y) {  // x in the low half
+  const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void store2(__nv_bfloat16* p, float x, float y) {
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
+}
+__device__ __forceinline__ void store2(__half* p, float x, float y) {
+  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(x, y);
+}
+// what the planes so far leave of x, y
+__device__ __forceinline__ void rest(uint32_t w, float& x, float& y) {
+  x -= __uint_as_float(w << 16);
+  y -= __uint_as_float(w & 0xffff0000u);
+}
+// N planes of the pair (x, y) at p, plane elements apart
+template <int N> __device__ __forceinline__ void put_at(bf* p, size_t plane, float x, float y) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t w = pack(x, y);
+    *reinterpret_cast<uint32_t*>(p + i * plane) = w;
+    if (i + 1 < N) rest(w, x, y);
+  }
+}
+template <int N, int PLANE> __device__ __forceinline__ void put(bf* p, float x, float y) { put_at<N>(p, PLANE, x, y); }
+
+// ------------------------------------------------------------------ token tiles
+// dst[planes][64][LD] = rows of src (COLS columns, zeros behind); asynchronous for bf16.
+template <class TI, int LD, int COLS, int NTH>
+__device__ __forceinline__ void load_tokens(bf* dst, const TI* src, size_t stride, int rows, int cols, bool vec) {
+  constexpr int PR = COLS / 8, PLANE = BT * LD;
+  if constexpr (Planes<TI>::n == 1) {
+    if (vec) {
+      for (int i = threadIdx.x; i < BT * PR; i += NTH) {
+        const int r = i / PR, c = (i % PR) * 8;
+        if (r < rows && c < cols) cp16(dst + r * LD + c, src + r * stride + c);
+        else *reinterpret_cast<uint4*>(dst + r * LD + c) = make_uint4(0, 0, 0, 0);
+      }
+      return;
+    }
+  }
+  for (int i = threadIdx.x; i < BT * COLS / 2; i += NTH) {
+    const int r = i / (COLS / 2), c = (i % (COLS / 2)) * 2;
+    float x = 0.f, y = 0.f;
+    if (r < rows) {
+      const TI* p = src + r * stride + c;
+      if (vec) {  // even columns, 4-byte aligned
+        if (c < cols) {
+          const float2 z = pair(p);
+          x = z.x;
+          y = z.y;
+        }
+      } else {
+        if (c < cols) x = ldf(p);
+        if (c + 1 < cols) y = ldf(p + 1);
+      }
+    }
+    put<Planes<TI>::n, PLANE>(dst + r * LD + c, x, y);
+  }
+}
+// planes of a state panel: dst[2][ROWS][LD], src [2][ROWS][stride] (16-byte aligned)
+template <int LD, int ROWS, int COLS, int NTH>
+__device__ __forceinline__ void load_planes(bf* dst, const bf* src, int stride) {
+  constexpr int PR = COLS / 8;
+  for (int i = threadIdx.x; i < 2 * ROWS * PR; i += NTH) {
+    const int r = i / PR, c = (i % PR) * 8;
+    cp16(dst + r * LD + c, src + (size_t)r * stride + c);
+  }
+}
+template <int NTH> __device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) {
+  for (int i = threadIdx.x * 16; i < bytes; i += NTH * 16) cp16((char*)dst + i, (const char*)src + i);
+}
+
+constexpr int FRAG_PLANE = 4 * 4 * 32 * 16;  // bytes of one plane of a [64, 64] matrix in fragment order
+
+// exp of an in-chunk difference on the special-function unit (about 2^-22; the results leave in 16 bits)
+__device__ __forceinline__ float fade16(const Gates& s, int i, int j) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.4426950408889634f * ((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]))));
+  return r;
+}
+
+}  // namespace h16
+}  // namespace delta
+}  // namespace ssla

@@ -16,8 +16,10 @@ namespace ssla {
 namespace delta {
 namespace {
 
-template <class TI, int KP> struct AdjSmem {
-  static constexpr int LDK = KTile<TI, KP>::LD, LDW = KP + 4, LDO = 72;
+using TI = float;  // 16-bit tokens: delta_rule_16_bwd.cu
+
+template <int KP> struct AdjSmem {
+  static constexpr int LDK = KP + 8, LDW = KP + 4, LDO = 72;
   TI k[BT * LDK];
   TI q[BT * LDK];
   TI d[BT * LDO];
@@ -28,12 +30,12 @@ template <class TI, int KP> struct AdjSmem {
 };
 
 // dB of every (chunk, value head) into ds.
-template <class TI, int KP, bool SP>
-__global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<TI, KP>) <= 113 * 1024 ? 2 : 1)
+template <int KP>
+__global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2 : 1)
     adjoint_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
                    const TI* __restrict__ dout, float* __restrict__ ds) {
-  using S = AdjSmem<TI, KP>;
-  constexpr bool X = Io16<TI>::exact;
+  using S = AdjSmem<KP>;
+  constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDW = S::LDW, LDO = S::LDO, NK = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -109,9 +111,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<TI, KP>) <= 113 * 1024
   }
 }
 
-template <class TI, int KP> struct BwdSmem {
+template <int KP> struct BwdSmem {
   // p and t, s and e are read both along rows and down columns: one of the two conflicts either way
-  static constexpr int VB = 32, LDK = KTile<TI, KP>::LD, LDO = VB + 8, LDX = VB + 8, LDS = VB + 4, LDP = BT + 4;
+  static constexpr int VB = 32, LDK = KP + 8, LDO = VB + 8, LDX = VB + 8, LDS = VB + 4, LDP = BT + 4;
   TI k[BT * LDK];
   TI q[BT * LDK];
   TI d[BT * LDO];
@@ -126,15 +128,15 @@ template <class TI, int KP> struct BwdSmem {
   Gates gates;
 };
 
-template <class TI, int KP>
+template <int KP>
 __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* __restrict__ tab, int VP,
                                                const float* __restrict__ tinv, const float* __restrict__ states,
                                                const float* __restrict__ ds, const TI* __restrict__ dout,
                                                TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv,
                                                void* __restrict__ dg, void* __restrict__ dbeta,
                                                float* __restrict__ dqk) {
-  using S = BwdSmem<TI, KP>;
-  constexpr bool X = Io16<TI>::exact, SP = OutSplit<TI>::v;
+  using S = BwdSmem<KP>;
+  constexpr bool X = false, SP = true;
   constexpr int VB = S::VB, LDK = S::LDK, LDO = S::LDO, LDX = S::LDX, LDS = S::LDS, LDP = S::LDP, NT = VB / 16, NK = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -391,34 +393,22 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   if (2 * lane + 1 < rows) st_any(dg, a.dt_g, at + a.HV, suf - gc[0] + sum);
 }
 
-template <class TI, int KP>
-__global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<TI, KP>) <= 113 * 1024 ? 2 : 1)
+template <int KP>
+__global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<KP>) <= 113 * 1024 ? 2 : 1)
     backward_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
                     const float* __restrict__ states, const float* __restrict__ ds, const TI* __restrict__ dout,
                     TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv, void* __restrict__ dg,
                     void* __restrict__ dbeta, float* __restrict__ dqk) {
-  backward_chunk<TI, KP>(a, tab, VP, tinv, states, ds, dout, dq, dk, dv, dg, dbeta, dqk);
-  const size_t TK = (size_t)a.T * a.HV * a.K;
-  if (dqk) {
-    zero_uncovered(dqk, a, (int64_t)a.HV * a.K);
-    zero_uncovered(dqk + TK, a, (int64_t)a.HV * a.K);
-  } else {
-    zero_uncovered(dq, a, (int64_t)a.H * a.K);
-    zero_uncovered(dk, a, (int64_t)a.H * a.K);
-  }
-  zero_uncovered(dv, a, (int64_t)a.HV * a.V);
-  if (a.dt_g == SSLA_F32) zero_uncovered((float*)dg, a, a.HV);
-  else zero_uncovered((__half*)dg, a, a.HV);  // 0 has the same bits in both 16-bit types
-  if (a.dt_b == SSLA_F32) zero_uncovered((float*)dbeta, a, a.HV);
-  else zero_uncovered((__half*)dbeta, a, a.HV);
+  backward_chunk<KP>(a, tab, VP, tinv, states, ds, dout, dq, dk, dv, dg, dbeta, dqk);
+  zero_gradients(a, dq, dk, dv, dg, dbeta, dqk);
 }
 
 // dq, dk [T, H, K] = sums over the value heads of a key head, in their order.  One warp a row of K.
-template <class TI>
+template <class TO>
 __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ dqk, int64_t TH, int R, int K,
-                                                        TI* __restrict__ dq, TI* __restrict__ dk) {
+                                                        TO* __restrict__ dq, TO* __restrict__ dk) {
   const float* p = dqk + (blockIdx.y ? (size_t)TH * R * K : 0);
-  TI* out = blockIdx.y ? dk : dq;
+  TO* out = blockIdx.y ? dk : dq;
   const int lane = threadIdx.x & 31;
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < TH; row += (int64_t)gridDim.x * 8) {
     const float* src = p + (size_t)row * R * K;
@@ -430,7 +420,7 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict_
           x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         const float v[4] = {x.x, x.y, x.z, x.w};
-        Vec<TI, 4>::store(out + (size_t)row * K + c, v);
+        Vec<TO, 4>::store(out + (size_t)row * K + c, v);
       }
     } else {
       for (int c = lane; c < K; c += 32) {
@@ -442,40 +432,30 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict_
   }
 }
 
-template <class TI, int KP, bool SP>
-int run_adjoint(const Args& a, const Saved& sv, int VP, const void* dout, float* ds, int64_t items, cudaStream_t st) {
-  const size_t smem = sizeof(AdjSmem<TI, KP>);
-  cudaFuncSetAttribute(adjoint_kernel<TI, KP, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  adjoint_kernel<TI, KP, SP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, (const TI*)dout, ds);
+template <int KP>
+int adjoint32(const Args& a, const Saved& sv, int VP, const void* dout, float* inc, int64_t items, cudaStream_t st) {
+  const size_t smem = sizeof(AdjSmem<KP>);
+  cudaFuncSetAttribute(adjoint_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  adjoint_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, (const TI*)dout, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule adjoint");
   return SSLA_OK;
 }
 
-template <class TI, int KP>
-int run_bwd(const Args& a, const Plan& p, const Saved& sv, const Work& w, int VP, const void* dout, const float* dht,
-            void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dh0, cudaStream_t st) {
-  const int64_t items = p.MC * a.HV;
-  int rc = SSLA_OK;
-  if (items > 0) {
-    // dh0 leaves in fp32: its increments take the split even for bf16 tokens
-    rc = OutSplit<TI>::v || dh0 ? run_adjoint<TI, KP, true>(a, sv, VP, dout, w.ds, items, st)
-                                : run_adjoint<TI, KP, OutSplit<TI>::v>(a, sv, VP, dout, w.ds, items, st);
-    if (rc) return rc;
-  }
-  rc = run_chain(p, sv, w, w.ds, dht, dh0, a.N, a.HV, a.K, a.V, true, OutSplit<TI>::v || dh0, !OutSplit<TI>::v, st);
-  if (rc || a.T == 0) return rc;
-  float* dqk = a.R > 1 ? w.dqk : nullptr;
-  const size_t smem = sizeof(BwdSmem<TI, KP>);
-  cudaFuncSetAttribute(backward_kernel<TI, KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  backward_kernel<TI, KP><<<(unsigned)(items > 0 ? items : 1), THREADS, smem, st>>>(
-      a, sv.chunk_tab, VP, sv.tinv, sv.s, w.ds, (const TI*)dout, (TI*)dq, (TI*)dk, (TI*)dv, dg, dbeta, dqk);
+template <int KP>
+int backward32(const Args& a, const Saved& sv, int VP, const float* ds, const Grads& g, int64_t items, cudaStream_t st) {
+  const size_t smem = sizeof(BwdSmem<KP>);
+  cudaFuncSetAttribute(backward_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  backward_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.s, ds, (const TI*)g.dout,
+                                                             (TI*)g.dq, (TI*)g.dk, (TI*)g.dv, g.dg, g.dbeta, g.dqk);
   SSLA_CHECK_LAUNCH("gated_delta_rule backward");
-  if (dqk) {
-    const int64_t blocks = (a.T * a.H + 7) / 8;
-    sum_heads_kernel<TI><<<dim3((unsigned)(blocks < 16 * kNumSMs ? blocks : 16 * kNumSMs), 2), 256, 0, st>>>(
-        dqk, a.T * a.H, a.R, a.K, (TI*)dq, (TI*)dk);
-    SSLA_CHECK_LAUNCH("gated_delta_rule sum_heads");
-  }
+  return SSLA_OK;
+}
+
+template <class TO> int sum_heads(const Args& a, const Grads& g, cudaStream_t st) {
+  const int64_t blocks = (a.T * a.H + 7) / 8;
+  sum_heads_kernel<TO><<<dim3((unsigned)(blocks < 16 * kNumSMs ? blocks : 16 * kNumSMs), 2), 256, 0, st>>>(
+      g.dqk, a.T * a.H, a.R, a.K, (TO*)g.dq, (TO*)g.dk);
+  SSLA_CHECK_LAUNCH("gated_delta_rule sum_heads");
   return SSLA_OK;
 }
 
@@ -489,8 +469,8 @@ using namespace ssla::delta;
 extern "C" int ssla_chunk_gated_delta_rule_bwd(const void* q, const void* k, const void* v, const void* g,
                                                const void* beta, int dtype, int dtype_g, int dtype_beta,
                                                const int64_t* cu_seqlens, int64_t n_seqs, int64_t T, int64_t H,
-                                               int64_t HV, int64_t K, int64_t V, float scale, const void* states,
-                                               size_t states_bytes, const void* dout, const float* dht, void* dq,
+                                               int64_t HV, int64_t K, int64_t V, float scale, int has_h0, int has_ht,
+                                               const void* states, size_t states_bytes, const void* dout, const float* dht, void* dq,
                                                void* dk, void* dv, void* dg, void* dbeta, float* dh0, void* workspace,
                                                size_t workspace_bytes, ssla_stream_t stream) {
   const char* name = "ssla_chunk_gated_delta_rule_bwd";
@@ -499,11 +479,13 @@ extern "C" int ssla_chunk_gated_delta_rule_bwd(const void* q, const void* k, con
   if (HV == 0) return SSLA_OK;
   SSLA_CHECK_ARG(cu_seqlens && states, "%s: null pointer", name);
   SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && dout && dq && dk && dv && dg && dbeta), "%s: null pointer", name);
+  const bool exact = exact_states(dtype, has_h0, has_ht);  // as in the forward
+  SSLA_CHECK_ARG(!dh0 || has_h0, "%s: dh0 without an initial state", name);
   const Plan p = make_plan(n_seqs, T, HV, K, V);
   const int KP = pad_k(K), VP = pad_v(V);
   Saved sv;
   Work w;
-  const size_t need = saved_layout(const_cast<void*>(states), p, n_seqs, HV, KP, VP, &sv);
+  const size_t need = saved_layout(const_cast<void*>(states), p, dtype, exact, n_seqs, HV, KP, VP, &sv);
   const size_t need_w = work_layout(workspace, p, T, H, HV, K, KP, VP, true, &w);
   if (states_bytes < need || workspace_bytes < need_w || (need_w && !workspace)) {
     set_error("%s: states of %zu bytes and workspace of %zu, %zu and %zu needed", name, states_bytes, workspace_bytes,
@@ -513,8 +495,20 @@ extern "C" int ssla_chunk_gated_delta_rule_bwd(const void* q, const void* k, con
   SSLA_CHECK_ARG(aligned_to(states, 16) && aligned_to(workspace, 16), "%s: states and workspace must be 16-byte aligned", name);
   cudaStream_t st = (cudaStream_t)stream;
   const Args a = make_args(q, k, v, g, beta, dtype, dtype_g, dtype_beta, cu_seqlens, n_seqs, T, H, HV, K, V, scale);
-  return SSLA_DISPATCH_DTYPE(dtype, T_, [&] {
-    return KP == 64 ? run_bwd<T_, 64>(a, p, sv, w, VP, dout, dht, dq, dk, dv, dg, dbeta, dh0, st)
-                    : run_bwd<T_, 128>(a, p, sv, w, VP, dout, dht, dq, dk, dv, dg, dbeta, dh0, st);
-  });
+  const int64_t items = p.MC * HV, blocks = items > 0 ? items : 1;
+  const bool f32 = dtype == SSLA_F32;
+  if (items > 0) {
+    rc = !f32       ? adjoint16(dtype, a, sv, KP, VP, t_planes(exact), dout, w.inc, items, st)
+         : KP == 64 ? adjoint32<64>(a, sv, VP, dout, w.inc, items, st)
+                    : adjoint32<128>(a, sv, VP, dout, w.inc, items, st);
+    if (rc) return rc;
+  }
+  rc = run_chain(p, sv, w, w.ds, dht, dh0, n_seqs, (int)HV, (int)K, (int)V, true, exact, !f32, st);
+  if (rc || T == 0) return rc;
+  const Grads gr = {dout, dq, dk, dv, dg, dbeta, a.R > 1 ? w.dqk : nullptr};
+  rc = !f32       ? backward16(dtype, a, sv, KP, VP, t_planes(exact), w.ds, gr, blocks, st)
+       : KP == 64 ? backward32<64>(a, sv, VP, w.ds, gr, blocks, st)
+                  : backward32<128>(a, sv, VP, w.ds, gr, blocks, st);
+  if (rc || !gr.dqk) return rc;
+  return SSLA_DISPATCH_DTYPE(dtype, T_, [&] { return sum_heads<T_>(a, gr, st); });
 }

@@ -82,7 +82,8 @@ def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
     dev = q.device
     o = torch.empty_like(v)
     ht = torch.empty((N, HV, K, V), device=dev, dtype=torch.float32) if output_final_state else None
-    nb = L.ssla_gated_delta_rule_states_bytes(N, T, H, HV, K, V)
+    nb = L.ssla_gated_delta_rule_states_bytes(_lib.dtype_code(q), N, T, H, HV, K, V, h0 is not None,
+                                              output_final_state)
     states = torch.empty(nb, device=dev, dtype=torch.uint8)
     wb = L.ssla_gated_delta_rule_workspace_bytes(N, T, H, HV, K, V, 0)
     ws = torch.empty(wb, device=dev, dtype=torch.uint8)
@@ -97,7 +98,7 @@ def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
     return o, ht, states
 
 
-def chunk_bwd(q, k, v, g, beta, cu, scale, has_h0, states, do, dht):
+def chunk_bwd(q, k, v, g, beta, cu, scale, has_h0, has_ht, states, do, dht):
     T, H, K = q.shape
     HV, V = v.shape[1:]
     N = cu.numel() - 1
@@ -112,7 +113,7 @@ def chunk_bwd(q, k, v, g, beta, cu, scale, has_h0, states, do, dht):
     with _lib.on_device(dev):
         _lib.check(
             L.ssla_chunk_gated_delta_rule_bwd(
-                *tensor_args(q, k, v, g, beta, cu, scale), states.data_ptr(), states.numel(), do.data_ptr(),
+                *tensor_args(q, k, v, g, beta, cu, scale), has_h0, has_ht, states.data_ptr(), states.numel(), do.data_ptr(),
                 _lib.ptr(dht), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
                 _lib.ptr(dh0), ws.data_ptr(), wb, _lib.raw_stream(q.device),
             ),
@@ -128,14 +129,14 @@ class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
         o, ht, states = chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
         ctx.save_for_backward(q, k, v, g, beta, cu, states)
         ctx.scale = scale
-        ctx.has_h0 = h0 is not None
+        ctx.has_h0, ctx.has_ht = h0 is not None, bool(output_final_state)
         return o, ht
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do, dht):
         q, k, v, g, beta, cu, states = ctx.saved_tensors
-        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, ctx.has_h0, states, do, dht)
+        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, ctx.has_h0, ctx.has_ht, states, do, dht)
         return dq, dk, dv, dg, dbeta, None, None, dh0, None
 
 

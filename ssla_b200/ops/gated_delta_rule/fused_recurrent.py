@@ -50,7 +50,7 @@ class FusedRecurrentGatedDeltaRuleFunction(torch.autograd.Function):
     def backward(ctx, do, dht):
         q, k, v, g, beta, cu, h0 = ctx.saved_tensors
         states = chunk_fwd(q, k, v, g, beta, cu, ctx.scale, h0, False)[2]
-        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, h0 is not None, states, do, dht)
+        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, h0 is not None, False, states, do, dht)
         return dq, dk, dv, dg, dbeta, None, None, dh0, None
 
 

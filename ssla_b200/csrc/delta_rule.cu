@@ -6,6 +6,7 @@
 #include "delta_rule_16.cuh"
 #include "delta_rule_inverse.cuh"
 #include "pack_tables.cuh"
+#include <stdlib.h>
 
 namespace ssla {
 namespace delta {
@@ -22,13 +23,15 @@ template <int KP> struct PrepSmem {
   float t[BT * LDC];
   float y[BT * 68];
   float col[BT];
+  unsigned red[THREADS / 32];
   Gates gates;
 };
 
 template <int KP>
 __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong2* __restrict__ tab, int VP,
                                                           float* __restrict__ decay, float* __restrict__ tinv,
-                                                          float* __restrict__ pm, float* __restrict__ bout) {
+                                                          __half* __restrict__ pm, float* __restrict__ pscale,
+                                                          float* __restrict__ inc) {
   using S = PrepSmem<KP>;
   constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDV = S::LDV;
@@ -109,149 +112,188 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
       const int mk = (warp >> 1) * 16 * MT;
       warp_mma<X, !SP, SP>(acc, mk, n0, 0, BT, [&](int m, int j) { return column<LDK>(sk + j * LDK + m); },
                            [&](int j, int n) { return column<68>(s.y + j * 68 + n); });
-      float* out = w ? pm + item * KP * KP : bout + item * KP * VP;
-      const int ld = w ? KP : VP;
-      each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
-        *reinterpret_cast<float2*>(out + (size_t)m * ld + c0 + n) = w ? stage2<SP>(x, y) : make_float2(x, y);
-      });
+      if (w)
+        store_pm<KP, 2>(acc, mk, c0, n0, s.red, pm + item * (2 * KP * (KP + 8)), pscale + item * (KP / 64));
+      else
+        each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
+          *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, c0 + n)) = make_float2(x, y);
+        });
     }
   }
 }
 
 // ------------------------------------------------------------------ chain
-// One CTA carries VS columns of one state along its list of steps; every warp owns 16 of the KP
-// rows in the accumulator layout.  A step needs one exchange of the state through shared memory
-// (it is the right operand) and streams the step's [KP, KP] map through two cp.async buffers.
+// One CTA carries VS columns of one state along its sequence's chunks; every warp owns 16 of the KP
+// rows in the accumulator layout (fp32).  The one product of a step, PM S, runs on fp16 planes (NP =
+// 2: hi + lo, 22 bits, three MMAs; NP = 1: 11 bits, for states whose only readers are bf16 outputs):
+// prep leaves PM in planes scaled by a power of two, and every warp scales its 16 rows of S by one
+// of its own before it shares them, so that 16 rows of the contraction have one scale, undone when
+// their MMA's result is added.  A step streams PM and its slice of B through a ring of cp.async
+// buffers, laid out in memory as in shared memory, and has one barrier.
+// What bounds it: the chain of one step (barrier, MMAs, rescaling) and, for 128 x 128, the 70 KB a
+// step from L2.  TF32 products of an fp32 PM took 750 instructions a warp and step against 190: the
+// 512 chunks of a 32768-token prompt, 8 heads of 128, 0.93 ms.
+template <int KP, int VS, int NP> struct ChainSmem {
+  static constexpr int LDP = KP + 8, LDS = VS == 8 ? 8 : VS + 8;  // ldmatrix without conflicts
+  static constexpr int PM = 2 * NP * KP * LDP, B = 4 * KP * VS, STAGE = PM + B + 16;      // bytes; decay, pscale
+  static constexpr int S = 2 * NP * KP * LDS, STATE = 2 * (S + 4 * (KP / 16)), MOST = 227 * 1024 - 1024;
+  static constexpr int fit = (MOST - STATE) / STAGE, stages = fit > 4 ? 4 : fit, bytes = STATE + stages * STAGE;
+  static_assert(stages >= 2 && STATE % 16 == 0 && STAGE % 16 == 0, "a step is loaded while another runs");
+};
+
 struct ChainArgs {
-  const float* pm;        // [step * HV + hv][KP][KP]
-  const float* b;         // [step * HV + hv][KP][VP]
-  float* s;               // start state of every step ([..][KP][VP], two bf16 planes if planes); null: not kept
-  const float* decay;     // per (step, hv); null: S' = PM S + B (composed maps)
-  const int* off;         // steps of list n: off[n] .. off[n+1] - 1 ...
-  const int4* seg;        // ... or of list n: seg[n].x, seg[n].y steps (seg[n].z < 0: none)
-  const float* init;      // [n * HV + hv][K][V] unpadded (padded: [KP][VP])
-  float* last;            // likewise
-  float* mseg;            // composing: [n * HV + hv][KP][KP] for the columns from VP on, start from I
-  bool init_padded, last_padded, reverse, compose, planes;
+  const __half* pm;     // [item][NP][KP][KP + 8]
+  const float* pscale;  // [item][KP / 64]
+  const float* inc;     // [item][VP / 8][KP][8]
+  const float* decay;   // [item]
+  float* s;             // start (reverse: end) state of every chunk [item][KP][VP], in two bf16 planes if planes
+  const int* off;       // chunks of sequence n: off[n] .. off[n + 1] - 1; item = chunk * HV + head
+  const float* init;    // [N * HV][K][V] or null
+  float* last;          // likewise
+  bool reverse, planes;
   int HV, K, V, VP, slices;
 };
 
-template <int KP, int VS, bool TRANS, bool SP>
+__device__ __forceinline__ void mma16h(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int KP, int VS, bool TRANS, int NP>
 __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
-  constexpr int NTH = KP * 2, NT = VS / 8, LDP = KP + (TRANS ? 4 : 8), LDS = VS + 4;
+  using M = ChainSmem<KP, VS, NP>;
+  constexpr int NTH = KP * 2, NT = VS / 8, LDP = M::LDP, LDS = M::LDS, ST = M::stages, NB = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
-  float* sp = reinterpret_cast<float*>(raw);
-  float* ss = sp + 2 * KP * LDP;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int64_t lh = blockIdx.x / a.slices;
-  int c0 = (int)(blockIdx.x - lh * a.slices) * VS;
-  const int64_t list = lh / a.HV;
-  const int hv = (int)(lh - list * a.HV);
-  int first, count;
-  if (a.seg) {
-    const int4 e = a.seg[list];
-    if (e.z < 0) return;
-    first = e.x;
-    count = e.y;
-  } else {
-    first = a.off[list];
-    count = a.off[list + 1] - first;
-  }
-  const bool ident = a.compose && c0 >= a.VP;  // columns of the map itself
-  if (ident) c0 -= a.VP;
-  const int m0 = warp * 16;
-  float S[1][NT][4];
-  auto at = [&](int i) { return (int64_t)first + (a.reverse ? count - 1 - i : i); };
-  auto load_map = [&](int i) {
-    const float* src = a.pm + ((size_t)at(i) * a.HV + hv) * KP * KP;
-    float* dst = sp + (i & 1) * KP * LDP;
-    for (int j = threadIdx.x; j < KP * KP / 4; j += NTH) {
-      const int r = j / (KP / 4), c = (j - r * (KP / 4)) * 4;
-      cp16(dst + r * LDP + c, src + (size_t)r * KP + c);
+  unsigned char* const ring = raw + M::STATE;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, m0 = warp * 16;
+  const unsigned lh = blockIdx.x / (unsigned)a.slices;
+  const int c0 = (int)(blockIdx.x - lh * a.slices) * VS;
+  const int list = (int)(lh / (unsigned)a.HV), hv = (int)(lh - (unsigned)list * a.HV);
+  const int first = a.off[list], count = a.off[list + 1] - first;
+  auto at = [&](int i) { return (size_t)(first + (a.reverse ? count - 1 - i : i)) * a.HV + hv; };
+  auto load = [&](int i) {  // one cp.async group per step, empty behind the last
+    if (i < count) {
+      const size_t it = at(i);
+      unsigned char* dst = ring + (i % ST) * M::STAGE;
+      const unsigned char* src = (const unsigned char*)a.pm + it * M::PM;
+#pragma unroll 4
+      for (int j = threadIdx.x * 16; j < M::PM; j += NTH * 16) cp16(dst + j, src + j);
+      src = (const unsigned char*)(a.inc + it * KP * a.VP + (size_t)c0 * KP);
+#pragma unroll
+      for (int j = threadIdx.x * 16; j < M::B; j += NTH * 16) cp16(dst + M::PM + j, src + j);
+      if (threadIdx.x <= KP / 64)
+        cp4(dst + M::PM + M::B + 4 * threadIdx.x,
+            threadIdx.x ? a.pscale + it * (KP / 64) + threadIdx.x - 1 : a.decay + it);
     }
+    cp_commit();
   };
-  if (count > 0) load_map(0);
-  cp_commit();
-  // start state
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) load(i);
+  float S[1][NT][4];
   each_pair(S, m0, 0, [&](int r, int c, float& x, float& y) {
     x = y = 0.f;
     const int cc = c0 + c;
-    if (ident) {
-      x = r == cc ? 1.f : 0.f;
-      y = r == cc + 1 ? 1.f : 0.f;
-    } else if (a.init && a.init_padded) {
-      const float2 z = *reinterpret_cast<const float2*>(a.init + ((size_t)lh * KP + r) * a.VP + cc);
-      x = z.x;
-      y = z.y;
-    } else if (a.init && r < a.K) {
+    if (a.init && r < a.K) {
       const float* p = a.init + ((size_t)lh * a.K + r) * a.V + cc;
       if (cc < a.V) x = p[0];
       if (cc + 1 < a.V) y = p[1];
     }
   });
-  float bn[NT][4];
-  auto load_b = [&](int i) {
-    const float* p = a.b + (((size_t)at(i) * a.HV + hv) * KP + m0) * a.VP + c0;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const float2 u = *reinterpret_cast<const float2*>(p + (size_t)g * a.VP + 8 * j + 2 * t);
-      const float2 w = *reinterpret_cast<const float2*>(p + (size_t)(g + 8) * a.VP + 8 * j + 2 * t);
-      bn[j][0] = u.x;
-      bn[j][1] = u.y;
-      bn[j][2] = w.x;
-      bn[j][3] = w.y;
-    }
-  };
-  float bc[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) bc[j][0] = bc[j][1] = bc[j][2] = bc[j][3] = bn[j][0] = bn[j][1] = bn[j][2] = bn[j][3] = 0.f;
-  if (!ident && count > 0) load_b(0);
+  // lane addresses of ldmatrix: the map's rows (its transpose: columns), the state's rows
+  const uint32_t a_at = TRANS ? ((lane & 7) + (lane >> 4) * 8) * LDP + ((lane >> 3) & 1) * 8 + m0
+                              : (m0 + (lane & 15)) * LDP + (lane >> 4) * 8;
+  const uint32_t b_at = VS == 8 ? (lane & 15) * LDS + (NP > 1 ? (lane >> 4) * (KP * LDS) : 0)
+                                : ((lane & 7) + ((lane >> 3) & 1) * 8) * LDS + (lane >> 4) * 8;
   for (int i = 0; i < count; ++i) {
-    const size_t it = (size_t)at(i) * a.HV + hv;
-    float* sc = ss + (i & 1) * KP * LDS;
-    each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-      *reinterpret_cast<float2*>(sc + r * LDS + c) = stage2<SP>(x, y);
-    });
-    const float d = a.decay ? a.decay[it] : 0.f;
+    const size_t it = at(i);
+    __half* sc = reinterpret_cast<__half*>(raw + (i & 1) * (M::STATE / 2));
+    float* un = reinterpret_cast<float*>(raw + (i & 1) * (M::STATE / 2) + M::S);
+    unsigned most = 0;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) bc[j][r] = bn[j][r];
-    if (a.s && !ident)
+      for (int r = 0; r < 4; ++r) most = max(most, finite_bits(S[0][j][r]));
+    const float scale = plane_scale(__reduce_max_sync(0xffffffffu, most));
+    if (lane == 0) un[warp] = plane_unscale(scale);
+    each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
+      put_half<NP>(sc + r * LDS + c, KP * LDS, x * scale, y * scale);
+    });
+    cp_wait<ST - 2>();
+    __syncthreads();  // step i's map and state are there, step i - 1 is read
+    load(i + ST - 1);
+    if (a.s)
       each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
         if (a.planes)
-          h16::put_at<2>((h16::bf*)a.s + (2 * it * KP + r) * a.VP + c0 + c, KP * a.VP, x, y);
+          h16::put_at<2>((h16::bf*)a.s + (2 * it * KP + r) * a.VP + c0 + c, (size_t)KP * a.VP, x, y);
         else
           *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
       });
-    cp_wait<0>();
-    __syncthreads();  // map i and the state are there, step i - 1 is read
-    if (i + 1 < count) {
-      load_map(i + 1);
-      if (!ident) load_b(i + 1);
+    const unsigned char* stage = ring + (i % ST) * M::STAGE;
+    const float* ps = reinterpret_cast<const float*>(stage + M::PM + M::B) + 1;
+    const float d = ps[-1];
+    const uint32_t pa = h16::smem_u32(stage) + 2 * a_at, pb = h16::smem_u32(sc) + 2 * b_at;
+    float acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) {
+      uint32_t fa[NP][4];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const uint32_t q = pa + 2 * (p * KP * LDP + (TRANS ? kb * 16 * LDP : kb * 16));
+        if (TRANS) h16::ldsm4t(fa[p], q);
+        else h16::ldsm4(fa[p], q);
+      }
+      uint32_t fb[NP][NT][2];
+      if (VS == 8) {  // both planes of the one column tile at once (one plane: the upper half is unused)
+        uint32_t r[4];
+        h16::ldsm4t(r, pb + 2 * kb * 16 * LDS);
+        fb[0][0][0] = r[0];
+        fb[0][0][1] = r[1];
+        fb[NP - 1][0][0] = r[NP > 1 ? 2 : 0];
+        fb[NP - 1][0][1] = r[NP > 1 ? 3 : 1];
+      } else {
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int j = 0; j < NT; j += 2) {
+            uint32_t r[4];
+            h16::ldsm4t(r, pb + 2 * (p * KP * LDS + kb * 16 * LDS + 8 * j));
+            fb[p][j][0] = r[0];
+            fb[p][j][1] = r[1];
+            fb[p][j + (NT > 1)][0] = r[2];
+            fb[p][j + (NT > 1)][1] = r[3];
+          }
+      }
+      const float f = TRANS ? un[kb] : un[kb] * ps[kb / 4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        if (NP > 1) {
+          mma16h(part, fa[NP - 1], fb[0][j][0], fb[0][j][1]);
+          mma16h(part, fa[0], fb[NP - 1][j][0], fb[NP - 1][j][1]);
+        }
+        mma16h(part, fa[0], fb[0][j][0], fb[0][j][1]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(f, part[r], acc[j][r]);
+      }
     }
-    cp_commit();
-    const float* pc = sp + (i & 1) * KP * LDP;
-    float acc[1][NT][4];
-    zero(acc);
-    warp_mma<!SP, !SP, SP>(acc, m0, 0, 0, KP,
-                           [&](int m, int k) { return TRANS ? column<LDP>(pc + k * LDP + m) : pair(pc + m * LDP + k); },
-                           [&](int k, int n) { return column<LDS>(sc + k * LDS + n); });
+    const float* bc = reinterpret_cast<const float*>(stage + M::PM);
+    const float f = TRANS ? ps[m0 / 64] : 1.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        S[0][j][r] = a.decay ? fmaf(d, S[0][j][r], bc[j][r] - acc[0][j][r]) : acc[0][j][r] + bc[j][r];
+      for (int r = 0; r < 2; ++r) {
+        const float2 b = pair(bc + (j * KP + m0 + g + 8 * r) * 8 + 2 * t);
+        float &x = S[0][j][2 * r], &y = S[0][j][2 * r + 1];
+        x = fmaf(d, x, b.x - f * acc[j][2 * r]);
+        y = fmaf(d, y, b.y - f * acc[j][2 * r + 1]);
+      }
   }
-  if (ident) {
-    each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-      *reinterpret_cast<float2*>(a.mseg + ((size_t)lh * KP + r) * KP + c0 + c) = make_float2(x, y);
-    });
-  } else if (a.last && a.last_padded) {
-    each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-      *reinterpret_cast<float2*>(a.last + ((size_t)lh * KP + r) * a.VP + c0 + c) = make_float2(x, y);
-    });
-  } else if (a.last) {
+  cp_wait<0>();
+  if (a.last)
     each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
       const int cc = c0 + c;
       if (r < a.K) {
@@ -260,34 +302,27 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
         if (cc + 1 < a.V) p[1] = y;
       }
     });
-  }
 }
 
-template <int KP, int VS, bool TRANS, bool SP> int launch_chain(const ChainArgs& a, int64_t lists, cudaStream_t st) {
-  constexpr size_t smem = 4 * (2 * KP * (KP + (TRANS ? 4 : 8)) + 2 * KP * (VS + 4));
-  cudaFuncSetAttribute(chain_kernel<KP, VS, TRANS, SP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  const int64_t grid = lists * a.HV * a.slices;
+template <int KP, int VS, bool TRANS, int NP> int launch_chain(const ChainArgs& a, int64_t N, cudaStream_t st) {
+  constexpr int smem = ChainSmem<KP, VS, NP>::bytes;
+  cudaFuncSetAttribute(chain_kernel<KP, VS, TRANS, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int64_t grid = N * a.HV * a.slices;
   if (grid == 0) return SSLA_OK;
-  chain_kernel<KP, VS, TRANS, SP><<<(unsigned)grid, KP * 2, smem, st>>>(a);
+  chain_kernel<KP, VS, TRANS, NP><<<(unsigned)grid, KP * 2, smem, st>>>(a);
   SSLA_CHECK_LAUNCH("gated_delta_rule chain");
   return SSLA_OK;
 }
 
-template <int KP, int VS> int chain_vs(const ChainArgs& a, bool trans, bool split, int64_t lists, cudaStream_t st) {
-  if (split) return trans ? launch_chain<KP, VS, true, true>(a, lists, st) : launch_chain<KP, VS, false, true>(a, lists, st);
-  return trans ? launch_chain<KP, VS, true, false>(a, lists, st) : launch_chain<KP, VS, false, false>(a, lists, st);
+template <int KP, int VS> int chain_vs(const ChainArgs& a, bool exact, int64_t N, cudaStream_t st) {
+  if (exact) return a.reverse ? launch_chain<KP, VS, true, 2>(a, N, st) : launch_chain<KP, VS, false, 2>(a, N, st);
+  return a.reverse ? launch_chain<KP, VS, true, 1>(a, N, st) : launch_chain<KP, VS, false, 1>(a, N, st);
 }
 
-template <int KP> int chain_kp(const ChainArgs& a, int vs, bool trans, bool split, int64_t lists, cudaStream_t st) {
-  if (vs == 8) return chain_vs<KP, 8>(a, trans, split, lists, st);
-  if (vs == 16) return chain_vs<KP, 16>(a, trans, split, lists, st);
-  if (vs == 32) return chain_vs<KP, 32>(a, trans, split, lists, st);
-  return chain_vs<KP, 64>(a, trans, split, lists, st);
-}
-
-int chain(ChainArgs a, int KP, int vs, bool trans, bool split, int64_t lists, cudaStream_t st) {
-  a.slices = (a.VP + (a.compose ? KP : 0)) / vs;
-  return KP == 64 ? chain_kp<64>(a, vs, trans, split, lists, st) : chain_kp<128>(a, vs, trans, split, lists, st);
+template <int KP> int chain_kp(const ChainArgs& a, int vs, bool exact, int64_t N, cudaStream_t st) {
+  if (vs == 8) return chain_vs<KP, 8>(a, exact, N, st);
+  if (vs == 16) return chain_vs<KP, 16>(a, exact, N, st);
+  return chain_vs<KP, 32>(a, exact, N, st);
 }
 
 // ------------------------------------------------------------------ output
@@ -398,7 +433,7 @@ template <int KP>
 int prep32(const Args& a, const Saved& sv, int VP, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(PrepSmem<KP>);
   cudaFuncSetAttribute(prep_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  prep_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, sv.tinv, sv.pm, inc);
+  prep_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, sv.tinv, sv.pm, sv.pscale, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
 }
@@ -418,13 +453,12 @@ int output32(const Args& a, const Saved& sv, int VP, void* o, int64_t items, cud
 Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V) {
   Plan p;
   p.MC = max_chunks(N, T);
-  const int VP = pad_v(V), KP = pad_k(K);
-  (void)KP;
+  const int VP = pad_v(V);
   p.vs = 8;
-  p.vs_seg = 16;
-  while (p.vs < 64 && N * HV * (VP / p.vs) >= 4 * kNumSMs) p.vs *= 2;
-  p.len = 0;
-  p.MS = 0;
+  int64_t want = 2 * kNumSMs;
+  if (getenv("PW")) want = atoi(getenv("PW"));
+  while (p.vs < 32 && N * HV * (VP / p.vs) >= want) p.vs *= 2;
+  if (getenv("PVS")) p.vs = atoi(getenv("PVS"));
   return p;
 }
 
@@ -462,46 +496,22 @@ Args make_args(const void* q, const void* k, const void* v, const void* g, const
 int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const float* init, float* last, int64_t N,
               int HV, int K, int V, bool reverse, bool exact, bool planes, cudaStream_t st) {
   ChainArgs c = {};
+  c.pm = sv.pm;
+  c.pscale = sv.pscale;
+  c.inc = w.inc;
+  c.decay = sv.decay;
+  c.s = s;
+  c.off = sv.chunk_off;
+  c.init = init;
+  c.last = last;
+  c.reverse = reverse;
+  c.planes = planes;
   c.HV = HV;
   c.K = K;
   c.V = V;
   c.VP = pad_v(V);
-  c.reverse = reverse;
-  c.planes = planes;
-  const int KP = pad_k(K);
-  c.pm = sv.pm;
-  c.b = w.inc;
-  c.s = s;
-  c.decay = sv.decay;
-  if (!p.len) {
-    c.off = sv.chunk_off;
-    c.init = init;
-    c.last = last;
-    return chain(c, KP, p.vs, reverse, exact, N, st);
-  }
-  // compose the maps of every segment, run along the segments, run inside them
-  ChainArgs d = c;
-  d.s = nullptr;
-  d.seg = sv.seg_tab;
-  d.compose = true;
-  d.mseg = w.mseg;
-  d.last = w.bseg;
-  d.last_padded = true;
-  int rc = chain(d, KP, p.vs_seg, reverse, exact, p.MS, st);
-  if (rc) return rc;
-  d = c;
-  d.pm = w.mseg;
-  d.b = d.s = w.bseg;
-  d.decay = nullptr;
-  d.off = sv.seg_off;
-  d.init = init;
-  d.last = last;
-  d.planes = false;
-  if ((rc = chain(d, KP, 16, false, exact, N, st))) return rc;
-  c.seg = sv.seg_tab;
-  c.init = w.bseg;
-  c.init_padded = true;
-  return chain(c, KP, p.vs_seg, reverse, exact, p.MS, st);
+  c.slices = c.VP / p.vs;
+  return pad_k(K) == 64 ? chain_kp<64>(c, p.vs, exact, N, st) : chain_kp<128>(c, p.vs, exact, N, st);
 }
 
 }  // namespace delta
@@ -549,8 +559,7 @@ extern "C" int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, con
   }
   SSLA_CHECK_ARG(aligned_to(states, 16) && aligned_to(workspace, 16), "%s: states and workspace must be 16-byte aligned", name);
   cudaStream_t st = (cudaStream_t)stream;
-  rc = launch_pack_tables(cu_seqlens, n_seqs, T, BT, p.MC, p.len, p.MS, sv.chunk_off, sv.seg_off, sv.chunk_tab,
-                          sv.seg_tab, st);
+  rc = launch_pack_tables(cu_seqlens, n_seqs, T, BT, p.MC, sv.chunk_off, sv.chunk_tab, st);
   if (rc) return rc;
   const Args a = make_args(q, k, v, g, beta, dtype, dtype_g, dtype_beta, cu_seqlens, n_seqs, T, H, HV, K, V, scale);
   const int64_t items = p.MC * HV, blocks = items > 0 ? items : 1;

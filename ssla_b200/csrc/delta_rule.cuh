@@ -33,14 +33,9 @@ inline int64_t max_chunks(int64_t N, int64_t T) { return (T + (BT - 1) * N) / BT
 inline int pad_k(int64_t K) { return K <= 64 ? 64 : 128; }
 inline int pad_v(int64_t V) { return (int)((V + 63) / 64 * 64); }
 
-// Segments: runs of `len` chunks of one sequence whose maps are composed first when there are too
-// few (sequence, head, column) chains to fill the GPU; len = 0 leaves sequences whole.
 struct Plan {
-  int64_t MC;    // upper bound of chunks
-  int64_t len;   // chunks per segment (0: no segments)
-  int64_t MS;    // upper bound of segments
-  int vs;        // state columns per chain
-  int vs_seg;    // the same inside segments
+  int64_t MC;  // upper bound of chunks
+  int vs;      // state columns per chain
 };
 Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V);
 
@@ -51,20 +46,21 @@ inline bool exact_states(int dtype, bool h0, bool ht) { return dtype != SSLA_BF1
 inline int t_planes(bool exact) { return exact ? 3 : 2; }
 
 // What the forward leaves for the backward (caller's `states` buffer), states padded to KP x VP:
-//   chunk_off [N+1], seg_off [N+1] (device), chunk_tab [MC] {first token, rows | seq << 32},
-//   seg_tab [MS] {first chunk, chunks, seq}; per (chunk, value head) item: decay = exp(gC);
-//   tinv: T, fp32 [64,64], or for 16-bit tokens planes of T and T^T in fragment order;
-//   pm [KP,KP]; s [KP,VP] = state at the chunk's start, fp32, or for 16-bit tokens two bf16 planes.
+//   chunk_off [N+1] (device), chunk_tab [MC] {first token, rows | seq << 32}; per (chunk, value
+//   head) item: decay = exp(gC); tinv: T, fp32 [64,64], or for 16-bit tokens planes of T and T^T in
+//   fragment order; pm: fp16 planes of PM as the chain reads them (ChainTile), its 64-column panels
+//   scaled by powers of two, pscale [KP/64] = what undoes it; s [KP,VP] = state at the chunk's
+//   start, fp32, or for 16-bit tokens two bf16 planes.
 struct Saved {
   int* chunk_off;
-  int* seg_off;
   longlong2* chunk_tab;
-  int4* seg_tab;
   float* decay;
   float* tinv;
-  float* pm;
+  __half* pm;
+  float* pscale;
   float* s;
 };
+inline int pm_planes(bool exact) { return exact ? 2 : 1; }
 
 inline size_t saved_layout(void* base, const Plan& p, int dtype, bool exact, int64_t N, int64_t HV, int KP, int VP,
                            Saved* out) {
@@ -73,26 +69,23 @@ inline size_t saved_layout(void* base, const Plan& p, int dtype, bool exact, int
   auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
   Saved s;
   s.chunk_off = (int*)take(4 * (N + 1));
-  s.seg_off = (int*)take(4 * (N + 1));
   s.chunk_tab = (longlong2*)take(16 * (size_t)p.MC);
-  s.seg_tab = (int4*)take(16 * (size_t)p.MS);
   s.decay = (float*)take(4 * items);
   s.tinv = (float*)take((dtype == SSLA_F32 ? 4 : 4 * t_planes(exact)) * items * BT * BT);
-  s.pm = (float*)take(4 * items * KP * KP);
+  s.pm = (__half*)take(2 * (size_t)pm_planes(exact) * items * KP * (KP + 8));
+  s.pscale = (float*)take(4 * items * (KP / 64));
   s.s = (float*)take(4 * items * KP * VP);
   if (out) *out = s;
   return (size_t)(q - (char*)base);
 }
 
-// Scratch of one call: the increments of the chunk maps (B or dB); the composed maps of the segments;
-// for the backward the adjoint states (laid out as s) and, when value heads share key heads, fp32 dq
-// and dk of every value head.
+// Scratch of one call: the increments of the chunk maps (B or dB) by slices of 8 columns; for the
+// backward the adjoint states (laid out as s) and, when value heads share key heads, fp32 dq and dk
+// of every value head.
 struct Work {
-  float* inc;   // [MC*HV, KP, VP]
-  float* mseg;  // [MS*HV, KP, KP]
-  float* bseg;  // [MS*HV, KP, VP]
-  float* ds;    // [MC*HV, KP, VP]
-  float* dqk;   // [2, T, HV, K]
+  float* inc;  // [MC*HV][VP/8][KP][8]
+  float* ds;   // [MC*HV, KP, VP]
+  float* dqk;  // [2, T, HV, K]
 };
 
 inline size_t work_layout(void* base, const Plan& p, int64_t T, int64_t H, int64_t HV, int64_t K, int KP, int VP,
@@ -100,14 +93,16 @@ inline size_t work_layout(void* base, const Plan& p, int64_t T, int64_t H, int64
   char* q = (char*)base;
   auto take = [&](size_t n) { char* r = q; q += align256(n); return (void*)r; };
   Work w;
-  const size_t segs = p.len ? (size_t)p.MS * HV : 0, states = 4 * (size_t)p.MC * HV * KP * VP;
+  const size_t states = 4 * (size_t)p.MC * HV * KP * VP;
   w.inc = (float*)take(states);
-  w.mseg = (float*)take(4 * segs * KP * KP);
-  w.bseg = (float*)take(4 * segs * KP * VP);
   w.ds = (float*)take(bwd ? states : 0);
   w.dqk = (float*)take(bwd && HV != H ? 8 * (size_t)T * HV * K : 0);
   if (out) *out = w;
   return (size_t)(q - (char*)base);
+}
+// (row, col) of an item's increments
+__device__ __forceinline__ float* inc_at(float* inc, size_t item, int KP, int VP, int row, int col) {
+  return inc + item * KP * VP + ((size_t)(col >> 3) * KP + row) * 8 + (col & 7);
 }
 
 // One call's tensors and sizes (device pointers), shared by the kernels.
@@ -174,7 +169,7 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], cons
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-template <bool AX, bool BX, bool SPLIT, int MT, int NT, class FA, class FB>
+template <bool AX, bool BX, bool SPLIT, int UNROLL = 2, int MT, int NT, class FA, class FB>
 __device__ __forceinline__ void warp_mma(float (&acc)[MT][NT][4], int m0, int n0, int k0, int k1, FA fa, FB fb) {
   constexpr bool SMALL = SPLIT && !(AX && BX);
   const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
@@ -184,7 +179,7 @@ __device__ __forceinline__ void warp_mma(float (&acc)[MT][NT][4], int m0, int n0
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) small[i][j][0] = small[i][j][1] = small[i][j][2] = small[i][j][3] = 0.f;
-#pragma unroll 2
+#pragma unroll UNROLL
   for (int k = k0; k < k1; k += 8) {
     uint32_t ah[MT][4], al[MT][4];
 #pragma unroll
@@ -248,9 +243,58 @@ __device__ __forceinline__ void each_pair(float (&acc)[MT][NT][4], int m0, int n
     }
 }
 
+// ------------------------------------------------------------------ scaled fp16 planes
+// fp32 values as hi + lo in fp16 (22 bits) need a common power of two that brings the largest near
+// 2^14: everything down to 2^-28 of it then keeps all its bits.  Bits of that scale from the largest
+// magnitude's bits (finite values only: an infinity must not shrink its neighbours), and its inverse.
+__device__ __forceinline__ unsigned finite_bits(float x) {
+  const unsigned b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ float plane_scale(unsigned most) {
+  const unsigned e = most >> 23;  // biased exponent of the largest
+  return __uint_as_float((e < 20u ? 247u : 267u - e) << 23);  // 2^(13 - exponent), at most 2^120
+}
+__device__ __forceinline__ float plane_unscale(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
+template <int N> __device__ __forceinline__ void put_half(__half* p, size_t plane, float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  *reinterpret_cast<__half2*>(p) = h;
+  if (N > 1) {
+    const float2 z = __half22float2(h);
+    *reinterpret_cast<__half2*>(p + plane) = __floats2half2_rn(x - z.x, y - z.y);
+  }
+}
+// A block's panel of PM (64 columns from c0, the accumulators of all its warps) into planes.
+// red: 8 words of shared memory; ends with the block's barrier passed.
+template <int KP, int NPL, int MT>
+__device__ __forceinline__ void store_pm(float (&acc)[MT][4][4], int mk, int c0, int n0, unsigned* red, __half* pm,
+                                         float* pscale) {
+  unsigned most = 0;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) most = max(most, finite_bits(acc[i][j][r]));
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) most = max(most, red[w]);
+  const float sc = plane_scale(most);
+  if (threadIdx.x == 0) pscale[c0 / 64] = plane_unscale(sc);
+  each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
+    put_half<NPL>(pm + m * (KP + 8) + c0 + n, (size_t)KP * (KP + 8), x * sc, y * sc);
+  });
+}
+
 // ------------------------------------------------------------------ copies into shared memory
 __device__ __forceinline__ void cp16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
                : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

@@ -21,7 +21,7 @@ template <class TI, int KP, int NI> struct Prep16 {
   };
   float t[BT * LDC];
   bf y[(NI > 2 ? NI : 2) * BT * LDT];  // scratch of the inverse, then planes of a panel
-  float col[BT];
+  unsigned red[THREADS / 32];
   Gates gates;
 };
 
@@ -51,7 +51,7 @@ template <int NI> __device__ __forceinline__ void write_t(const float* t, bf* ou
 template <class TI, int KP, int NI>
 __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 1024 ? 3 : sizeof(Prep16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
     prep16_kernel(Args a, const longlong2* __restrict__ tab, int VP, float* __restrict__ decay, bf* __restrict__ tinv,
-                  float* __restrict__ pm, float* __restrict__ bout) {
+                  __half* __restrict__ pm, float* __restrict__ pscale, float* __restrict__ inc) {
   using S = Prep16<TI, KP, NI>;
   constexpr int N = S::NT, LDK = S::LDK, PLK = BT * LDK, PLT = BT * LDT;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -125,11 +125,13 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
       zero(acc);
       const int mk = (warp >> 1) * 16 * MT;
       mm(acc, ColA<LDK, PLK, N>(s.k), RowB<LDT, PLT, NI>(s.y), mk, n0, 0, BT);
-      float* out = w ? pm + item * KP * KP : bout + item * KP * VP;
-      const int ld = w ? KP : VP;
-      each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
-        *reinterpret_cast<float2*>(out + (size_t)m * ld + c0 + n) = w ? stage2<(NI > 2)>(x, y) : make_float2(x, y);
-      });
+      constexpr int NPL = NI > 2 ? 2 : 1;
+      if (w)
+        store_pm<KP, NPL>(acc, mk, c0, n0, s.red, pm + item * (NPL * KP * (KP + 8)), pscale + item * (KP / 64));
+      else
+        each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
+          *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, c0 + n)) = make_float2(x, y);
+        });
     }
     __syncthreads();  // the readers of v, tc and y are done
   }
@@ -300,7 +302,8 @@ template <class TI, int KP, int NI>
 int prep(const Args& a, const Saved& sv, int VP, float* b, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Prep16<TI, KP, NI>);
   cudaFuncSetAttribute(prep16_kernel<TI, KP, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  prep16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, (bf*)sv.tinv, sv.pm, b);
+  prep16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, (bf*)sv.tinv, sv.pm, sv.pscale,
+                                                                  b);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
 }

@@ -23,7 +23,7 @@ template <class TI, int KP, int NI> struct Adj16 {
 template <class TI, int KP, int NI>
 __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
     adjoint16_kernel(Args a, const longlong2* __restrict__ tab, int VP, const bf* __restrict__ tinv,
-                     const TI* __restrict__ dout, float* __restrict__ db) {
+                     const TI* __restrict__ dout, float* __restrict__ inc) {
   using S = Adj16<TI, KP, NI>;
   constexpr int N = S::N, LDK = S::LDK, PLK = BT * LDK, PLT = BT * LDT, NK = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 10
     zero(o);
     mm(o, ColA<LDK, PLK, NI>(s.w), RowB<LDT, PLT, N>(s.d), mk, n0, 0, BT);
     each_pair(o, mk, n0, [&](int m, int n, float x, float y) {
-      *reinterpret_cast<float2*>(db + (item * KP + m) * VP + v0 + n) = make_float2(x, y);
+      *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, v0 + n)) = make_float2(x, y);
     });
   }
 }
@@ -435,11 +435,11 @@ __global__ void __launch_bounds__(Bwd16<TI, KP>::NTH, sizeof(Bwd16<TI, KP>) <= 1
 }
 
 template <class TI, int KP, int NI>
-int adjoint(const Args& a, const Saved& sv, int VP, const void* dout, float* db, int64_t items, cudaStream_t st) {
+int adjoint(const Args& a, const Saved& sv, int VP, const void* dout, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Adj16<TI, KP, NI>);
   cudaFuncSetAttribute(adjoint16_kernel<TI, KP, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   adjoint16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, (const bf*)sv.tinv,
-                                                                      (const TI*)dout, db);
+                                                                      (const TI*)dout, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule adjoint");
   return SSLA_OK;
 }
@@ -458,14 +458,14 @@ int backward(const Args& a, const Saved& sv, int VP, int tplanes, const bf* ds, 
 
 }  // namespace
 
-int adjoint16(int dtype, const Args& a, const Saved& sv, int KP, int VP, int planes, const void* dout, float* db,
+int adjoint16(int dtype, const Args& a, const Saved& sv, int KP, int VP, int planes, const void* dout, float* inc,
               int64_t items, cudaStream_t st) {
   if (dtype == SSLA_F16)
-    return KP == 64 ? adjoint<__half, 64, 3>(a, sv, VP, dout, db, items, st)
-                    : adjoint<__half, 128, 3>(a, sv, VP, dout, db, items, st);
+    return KP == 64 ? adjoint<__half, 64, 3>(a, sv, VP, dout, inc, items, st)
+                    : adjoint<__half, 128, 3>(a, sv, VP, dout, inc, items, st);
   if (planes == 3)
-    return KP == 64 ? adjoint<bf, 64, 3>(a, sv, VP, dout, db, items, st) : adjoint<bf, 128, 3>(a, sv, VP, dout, db, items, st);
-  return KP == 64 ? adjoint<bf, 64, 2>(a, sv, VP, dout, db, items, st) : adjoint<bf, 128, 2>(a, sv, VP, dout, db, items, st);
+    return KP == 64 ? adjoint<bf, 64, 3>(a, sv, VP, dout, inc, items, st) : adjoint<bf, 128, 3>(a, sv, VP, dout, inc, items, st);
+  return KP == 64 ? adjoint<bf, 64, 2>(a, sv, VP, dout, inc, items, st) : adjoint<bf, 128, 2>(a, sv, VP, dout, inc, items, st);
 }
 
 int backward16(int dtype, const Args& a, const Saved& sv, int KP, int VP, int planes, const void* ds, const Grads& g,

@@ -29,11 +29,11 @@ template <int KP> struct AdjSmem {
   Gates gates;
 };
 
-// dB of every (chunk, value head) into ds.
+// dB of every (chunk, value head).
 template <int KP>
 __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2 : 1)
     adjoint_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
-                   const TI* __restrict__ dout, float* __restrict__ ds) {
+                   const TI* __restrict__ dout, float* __restrict__ inc) {
   using S = AdjSmem<KP>;
   constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDW = S::LDW, LDO = S::LDO, NK = KP / 16;
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2
     warp_mma<!SP, X, SP>(db, mk, n0, 0, BT, [&](int m, int j) { return column<LDW>(s.w + j * LDW + m); },
                          [&](int j, int n) { return column<LDO>(s.d + j * LDO + n); });
     each_pair(db, mk, n0, [&](int m, int n, float x, float y) {
-      *reinterpret_cast<float2*>(ds + (item * KP + m) * VP + v0 + n) = make_float2(x, y);
+      *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, v0 + n)) = make_float2(x, y);
     });
   }
 }

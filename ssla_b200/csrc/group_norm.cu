@@ -765,7 +765,7 @@ template <class TI, int VEC> int pack_call(const Call& c, cudaStream_t st) {
   const dim3 grid((unsigned)(MC > 0 ? MC : 1), (c.G + m.GB - 1) / m.GB);
   const unsigned ngrid = (unsigned)((c.N * c.G + TH / 32 - 1) / (TH / 32));
   if (!c.dy) {
-    int rc = launch_pack_tables(c.cu, c.N, c.T, m.R, MC, 0, 0, sv.off, nullptr, sv.tab, nullptr, st);
+    int rc = launch_pack_tables(c.cu, c.N, c.T, m.R, MC, sv.off, sv.tab, st);
     if (rc) return rc;
     if (MC > 0) {
       pack_stats<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, c.C, c.G, m, sv.tab, w.part);

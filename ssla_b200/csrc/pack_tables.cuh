@@ -5,9 +5,8 @@
 namespace ssla {
 // Sequences are cut into chunks of `rows` tokens: chunk_off[n] (n <= N) is the first chunk of
 // sequence n, chunk_tab[c] = {first token, tokens | sequence << 32} or {0, -1} behind the last one;
-// MC >= (T + (rows - 1) N) / rows entries.  With len > 0 also runs of len chunks: seg_off [N + 1],
-// seg_tab [MS] = {first chunk, chunks, sequence or -1, 0}.  Offsets are clamped into [0, T] and the
-// lists into their bounds, so malformed cu_seqlens cannot lead outside the buffers.
-int launch_pack_tables(const int64_t* cu, int64_t N, int64_t T, int rows, int64_t MC, int64_t len, int64_t MS,
-                       int* chunk_off, int* seg_off, longlong2* chunk_tab, int4* seg_tab, cudaStream_t st);
+// MC >= (T + (rows - 1) N) / rows entries.  Offsets are clamped into [0, T] and the lists into their
+// bounds, so malformed cu_seqlens cannot lead outside the buffers.
+int launch_pack_tables(const int64_t* cu, int64_t N, int64_t T, int rows, int64_t MC, int* chunk_off,
+                       longlong2* chunk_tab, cudaStream_t st);
 }  // namespace ssla

@@ -6,7 +6,7 @@
 #include "delta_rule_16.cuh"
 #include "delta_rule_inverse.cuh"
 #include "pack_tables.cuh"
-#include <stdlib.h>
+#include "tc_util.cuh"
 
 namespace ssla {
 namespace delta {
@@ -29,8 +29,7 @@ template <int KP> struct PrepSmem {
 
 template <int KP>
 __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong2* __restrict__ tab, int VP,
-                                                          float* __restrict__ decay, float* __restrict__ tinv,
-                                                          __half* __restrict__ pm, float* __restrict__ pscale,
+                                                          float* __restrict__ tinv, unsigned char* __restrict__ pm,
                                                           float* __restrict__ inc) {
   using S = PrepSmem<KP>;
   constexpr bool X = false, SP = true;
@@ -43,6 +42,7 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
   int64_t t0;
   int rows;
   if (!locate(tab, a.MC, chunk, t0, rows)) return;
+  unsigned char* const record = pm + item * pm_bytes(KP, 2);
   const int warp = threadIdx.x >> 5;
   load_rows<TI, LDK, KP>(s.k, (const TI*)a.k + ((size_t)t0 * a.H + h) * a.K, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   auto load_v = [&](int v0) {
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
   if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
   cp_wait<0>();
   __syncthreads();
-  if (threadIdx.x == 0) decay[item] = s.gates.whole;
+  if (threadIdx.x == 0) *reinterpret_cast<float*>(record) = s.gates.whole;
   const TI* sk = s.k;
   const int m0 = (warp >> 1) * 16, n0 = (warp & 1) * 32;
   {
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
       warp_mma<X, !SP, SP>(acc, mk, n0, 0, BT, [&](int m, int j) { return column<LDK>(sk + j * LDK + m); },
                            [&](int j, int n) { return column<68>(s.y + j * 68 + n); });
       if (w)
-        store_pm<KP, 2>(acc, mk, c0, n0, s.red, pm + item * (2 * KP * (KP + 8)), pscale + item * (KP / 64));
+        store_pm<KP, 2>(acc, mk, c0, n0, s.red, record);
       else
         each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
           *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, c0 + n)) = make_float2(x, y);
@@ -128,31 +128,36 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
 // 2: hi + lo, 22 bits, three MMAs; NP = 1: 11 bits, for states whose only readers are bf16 outputs):
 // prep leaves PM in planes scaled by a power of two, and every warp scales its 16 rows of S by one
 // of its own before it shares them, so that 16 rows of the contraction have one scale, undone when
-// their MMA's result is added.  A step streams PM and its slice of B through a ring of cp.async
-// buffers, laid out in memory as in shared memory, and has one barrier.
-// What bounds it: the chain of one step (barrier, MMAs, rescaling) and, for 128 x 128, the 70 KB a
-// step from L2.  TF32 products of an fp32 PM took 750 instructions a warp and step against 190: the
-// 512 chunks of a 32768-token prompt, 8 heads of 128, 0.93 ms.
+// their MMA's result is added.  A step streams the chunk's record and its slice of B through a ring
+// of bulk copies (one thread issues them; the memory has the layout of shared memory), and has one
+// barrier.  A wait that gives up makes the rest of the chain NaN.
+// What bounds it: the dependent chain of a step (barrier, MMAs, rescaling).
 template <int KP, int VS, int NP> struct ChainSmem {
   static constexpr int LDP = KP + 8, LDS = VS == 8 ? 8 : VS + 8;  // ldmatrix without conflicts
-  static constexpr int PM = 2 * NP * KP * LDP, B = 4 * KP * VS, STAGE = PM + B + 16;      // bytes; decay, pscale
+  static constexpr int PM = pm_bytes(KP, NP), B = 4 * KP * VS, STAGE = PM + B;  // bytes
   static constexpr int S = 2 * NP * KP * LDS, STATE = 2 * (S + 4 * (KP / 16)), MOST = 227 * 1024 - 1024;
-  static constexpr int fit = (MOST - STATE) / STAGE, stages = fit > 4 ? 4 : fit, bytes = STATE + stages * STAGE;
-  static_assert(stages >= 2 && STATE % 16 == 0 && STAGE % 16 == 0, "a step is loaded while another runs");
+  static constexpr int fit = (MOST - STATE - 64) / STAGE, stages = fit > 4 ? 4 : fit, bytes = STATE + 64 + stages * STAGE;
+  static_assert(stages >= 2 && STATE % 32 == 0 && STAGE % 16 == 0, "a step is loaded while another runs");
 };
 
 struct ChainArgs {
-  const __half* pm;     // [item][NP][KP][KP + 8]
-  const float* pscale;  // [item][KP / 64]
-  const float* inc;     // [item][VP / 8][KP][8]
-  const float* decay;   // [item]
-  float* s;             // start (reverse: end) state of every chunk [item][KP][VP], in two bf16 planes if planes
-  const int* off;       // chunks of sequence n: off[n] .. off[n + 1] - 1; item = chunk * HV + head
-  const float* init;    // [N * HV][K][V] or null
-  float* last;          // likewise
+  const unsigned char* pm;  // [item] records
+  const float* inc;         // [item][VP / 8][KP][8]
+  float* s;          // start (reverse: end) state of every chunk [item][KP][VP], in two bf16 planes if planes
+  const int* off;    // chunks of sequence n: off[n] .. off[n + 1] - 1; item = chunk * HV + head
+  const float* init; // [N * HV][K][V] or null
+  float* last;       // likewise
   bool reverse, planes;
   int HV, K, V, VP, slices;
 };
+
+// 16-byte aligned addresses, bytes a multiple of 16; completes on the mbarrier
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* mbar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   h16::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(h16::smem_u32(mbar))
+               : "memory");
+}
 
 __device__ __forceinline__ void mma16h(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -165,32 +170,30 @@ template <int KP, int VS, bool TRANS, int NP>
 __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
   using M = ChainSmem<KP, VS, NP>;
   constexpr int NTH = KP * 2, NT = VS / 8, LDP = M::LDP, LDS = M::LDS, ST = M::stages, NB = KP / 16;
-  extern __shared__ __align__(16) unsigned char raw[];
-  unsigned char* const ring = raw + M::STATE;
+  extern __shared__ __align__(128) unsigned char raw[];
+  uint64_t* const full = reinterpret_cast<uint64_t*>(raw + M::STATE);
+  unsigned char* const ring = raw + M::STATE + 64;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, m0 = warp * 16;
   const unsigned lh = blockIdx.x / (unsigned)a.slices;
   const int c0 = (int)(blockIdx.x - lh * a.slices) * VS;
   const int list = (int)(lh / (unsigned)a.HV), hv = (int)(lh - (unsigned)list * a.HV);
   const int first = a.off[list], count = a.off[list + 1] - first;
   auto at = [&](int i) { return (size_t)(first + (a.reverse ? count - 1 - i : i)) * a.HV + hv; };
-  auto load = [&](int i) {  // one cp.async group per step, empty behind the last
-    if (i < count) {
-      const size_t it = at(i);
-      unsigned char* dst = ring + (i % ST) * M::STAGE;
-      const unsigned char* src = (const unsigned char*)a.pm + it * M::PM;
-#pragma unroll 4
-      for (int j = threadIdx.x * 16; j < M::PM; j += NTH * 16) cp16(dst + j, src + j);
-      src = (const unsigned char*)(a.inc + it * KP * a.VP + (size_t)c0 * KP);
-#pragma unroll
-      for (int j = threadIdx.x * 16; j < M::B; j += NTH * 16) cp16(dst + M::PM + j, src + j);
-      if (threadIdx.x <= KP / 64)
-        cp4(dst + M::PM + M::B + 4 * threadIdx.x,
-            threadIdx.x ? a.pscale + it * (KP / 64) + threadIdx.x - 1 : a.decay + it);
-    }
-    cp_commit();
+  auto load = [&](int i) {  // thread 0
+    const size_t it = at(i);
+    unsigned char* dst = ring + (i % ST) * M::STAGE;
+    tc::mbar_arrive_expect_tx(full + i % ST, M::STAGE);
+    bulk_load(dst, a.pm + it * M::PM, M::PM, full + i % ST);
+    bulk_load(dst + M::PM, a.inc + it * KP * a.VP + (size_t)c0 * KP, M::B, full + i % ST);
   };
-#pragma unroll
-  for (int i = 0; i < ST - 1; ++i) load(i);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) tc::mbar_init(full + i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int i = 0; i < ST - 1 && i < count; ++i) load(i);
+  }
+  __syncthreads();
+  bool good = true;
+  int bad_at = 0;
   float S[1][NT][4];
   each_pair(S, m0, 0, [&](int r, int c, float& x, float& y) {
     x = y = 0.f;
@@ -220,20 +223,15 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
     each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
       put_half<NP>(sc + r * LDS + c, KP * LDS, x * scale, y * scale);
     });
-    cp_wait<ST - 2>();
-    __syncthreads();  // step i's map and state are there, step i - 1 is read
-    load(i + ST - 1);
-    if (a.s)
-      each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-        if (a.planes)
-          h16::put_at<2>((h16::bf*)a.s + (2 * it * KP + r) * a.VP + c0 + c, (size_t)KP * a.VP, x, y);
-        else
-          *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
-      });
+    if (good && !tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20)) {
+      good = false;
+      bad_at = i;
+    }
+    __syncthreads();  // the state is there, step i - 1 is read
     const unsigned char* stage = ring + (i % ST) * M::STAGE;
-    const float* ps = reinterpret_cast<const float*>(stage + M::PM + M::B) + 1;
-    const float d = ps[-1];
-    const uint32_t pa = h16::smem_u32(stage) + 2 * a_at, pb = h16::smem_u32(sc) + 2 * b_at;
+    const float* ps = reinterpret_cast<const float*>(stage) + 1;
+    const float d = good ? ps[-1] : __int_as_float(0x7fffffff);
+    const uint32_t pa = h16::smem_u32(stage + 16) + 2 * a_at, pb = h16::smem_u32(sc) + 2 * b_at;
     float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
@@ -280,6 +278,14 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
         for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(f, part[r], acc[j][r]);
       }
     }
+    if (threadIdx.x == 0 && good && i + ST - 1 < count) load(i + ST - 1);
+    if (a.s)
+      each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
+        if (a.planes)
+          h16::put_at<2>((h16::bf*)a.s + (2 * it * KP + r) * a.VP + c0 + c, (size_t)KP * a.VP, x, y);
+        else
+          *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
+      });
     const float* bc = reinterpret_cast<const float*>(stage + M::PM);
     const float f = TRANS ? ps[m0 / 64] : 1.f;
 #pragma unroll
@@ -292,7 +298,8 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
         y = fmaf(d, y, b.y - f * acc[j][2 * r + 1]);
       }
   }
-  cp_wait<0>();
+  if (!good && threadIdx.x == 0)  // let the copies under way end before the block's memory goes
+    for (int i = bad_at; i < bad_at + ST && i < count; ++i) tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20);
   if (a.last)
     each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
       const int cc = c0 + c;
@@ -433,7 +440,7 @@ template <int KP>
 int prep32(const Args& a, const Saved& sv, int VP, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(PrepSmem<KP>);
   cudaFuncSetAttribute(prep_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  prep_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, sv.tinv, sv.pm, sv.pscale, inc);
+  prep_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.pm, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
 }
@@ -454,11 +461,12 @@ Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V) {
   Plan p;
   p.MC = max_chunks(N, T);
   const int VP = pad_v(V);
+  // Columns of a chain: 8 while that leaves few blocks (a step is its own latency: 512 steps of 128 x
+  // 128 take 0.51 ms with 8 columns on 128 SMs, 1.0 ms with 16 on 64), up to 32 while at least two
+  // blocks per SM remain (the map is read once per block: 112 chains of 128 x 128 take 198 us with 8
+  // columns, 121 us with 32).
   p.vs = 8;
-  int64_t want = 2 * kNumSMs;
-  if (getenv("PW")) want = atoi(getenv("PW"));
-  while (p.vs < 32 && N * HV * (VP / p.vs) >= want) p.vs *= 2;
-  if (getenv("PVS")) p.vs = atoi(getenv("PVS"));
+  while (p.vs < 32 && N * HV * (VP / (2 * p.vs)) >= 2 * kNumSMs) p.vs *= 2;
   return p;
 }
 
@@ -497,9 +505,7 @@ int run_chain(const Plan& p, const Saved& sv, const Work& w, float* s, const flo
               int HV, int K, int V, bool reverse, bool exact, bool planes, cudaStream_t st) {
   ChainArgs c = {};
   c.pm = sv.pm;
-  c.pscale = sv.pscale;
   c.inc = w.inc;
-  c.decay = sv.decay;
   c.s = s;
   c.off = sv.chunk_off;
   c.init = init;

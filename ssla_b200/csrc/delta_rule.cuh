@@ -47,20 +47,20 @@ inline int t_planes(bool exact) { return exact ? 3 : 2; }
 
 // What the forward leaves for the backward (caller's `states` buffer), states padded to KP x VP:
 //   chunk_off [N+1] (device), chunk_tab [MC] {first token, rows | seq << 32}; per (chunk, value
-//   head) item: decay = exp(gC); tinv: T, fp32 [64,64], or for 16-bit tokens planes of T and T^T in
-//   fragment order; pm: fp16 planes of PM as the chain reads them (ChainTile), its 64-column panels
-//   scaled by powers of two, pscale [KP/64] = what undoes it; s [KP,VP] = state at the chunk's
+//   head) item: tinv: T, fp32 [64,64], or for 16-bit tokens planes of T and T^T in fragment order;
+//   pm: the record of pm_bytes that a step of the chain copies; s [KP,VP] = state at the chunk's
 //   start, fp32, or for 16-bit tokens two bf16 planes.
 struct Saved {
   int* chunk_off;
   longlong2* chunk_tab;
-  float* decay;
   float* tinv;
-  __half* pm;
-  float* pscale;
+  unsigned char* pm;
   float* s;
 };
-inline int pm_planes(bool exact) { return exact ? 2 : 1; }
+// A chunk map's record: fp32 exp(gC) and, per 64-column panel of PM, what undoes its scale (16 bytes);
+// then one or two fp16 planes [KP][KP + 8] of the scaled PM.
+__host__ __device__ constexpr int pm_planes(bool exact) { return exact ? 2 : 1; }
+__host__ __device__ constexpr int pm_bytes(int KP, int planes) { return 16 + 2 * planes * KP * (KP + 8); }
 
 inline size_t saved_layout(void* base, const Plan& p, int dtype, bool exact, int64_t N, int64_t HV, int KP, int VP,
                            Saved* out) {
@@ -70,10 +70,8 @@ inline size_t saved_layout(void* base, const Plan& p, int dtype, bool exact, int
   Saved s;
   s.chunk_off = (int*)take(4 * (N + 1));
   s.chunk_tab = (longlong2*)take(16 * (size_t)p.MC);
-  s.decay = (float*)take(4 * items);
   s.tinv = (float*)take((dtype == SSLA_F32 ? 4 : 4 * t_planes(exact)) * items * BT * BT);
-  s.pm = (__half*)take(2 * (size_t)pm_planes(exact) * items * KP * (KP + 8));
-  s.pscale = (float*)take(4 * items * (KP / 64));
+  s.pm = (unsigned char*)take(items * pm_bytes(KP, pm_planes(exact)));
   s.s = (float*)take(4 * items * KP * VP);
   if (out) *out = s;
   return (size_t)(q - (char*)base);
@@ -267,8 +265,9 @@ template <int N> __device__ __forceinline__ void put_half(__half* p, size_t plan
 // A block's panel of PM (64 columns from c0, the accumulators of all its warps) into planes.
 // red: 8 words of shared memory; ends with the block's barrier passed.
 template <int KP, int NPL, int MT>
-__device__ __forceinline__ void store_pm(float (&acc)[MT][4][4], int mk, int c0, int n0, unsigned* red, __half* pm,
-                                         float* pscale) {
+__device__ __forceinline__ void store_pm(float (&acc)[MT][4][4], int mk, int c0, int n0, unsigned* red,
+                                         unsigned char* record) {
+  __half* const pm = reinterpret_cast<__half*>(record + 16);
   unsigned most = 0;
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -282,7 +281,7 @@ __device__ __forceinline__ void store_pm(float (&acc)[MT][4][4], int mk, int c0,
 #pragma unroll
   for (int w = 0; w < THREADS / 32; ++w) most = max(most, red[w]);
   const float sc = plane_scale(most);
-  if (threadIdx.x == 0) pscale[c0 / 64] = plane_unscale(sc);
+  if (threadIdx.x == 0) reinterpret_cast<float*>(record)[1 + c0 / 64] = plane_unscale(sc);
   each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
     put_half<NPL>(pm + m * (KP + 8) + c0 + n, (size_t)KP * (KP + 8), x * sc, y * sc);
   });
@@ -291,10 +290,6 @@ __device__ __forceinline__ void store_pm(float (&acc)[MT][4][4], int mk, int c0,
 // ------------------------------------------------------------------ copies into shared memory
 __device__ __forceinline__ void cp16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
-}
-__device__ __forceinline__ void cp4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
                : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

@@ -50,8 +50,8 @@ template <int NI> __device__ __forceinline__ void write_t(const float* t, bf* ou
 
 template <class TI, int KP, int NI>
 __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 1024 ? 3 : sizeof(Prep16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
-    prep16_kernel(Args a, const longlong2* __restrict__ tab, int VP, float* __restrict__ decay, bf* __restrict__ tinv,
-                  __half* __restrict__ pm, float* __restrict__ pscale, float* __restrict__ inc) {
+    prep16_kernel(Args a, const longlong2* __restrict__ tab, int VP, bf* __restrict__ tinv, unsigned char* __restrict__ pm,
+                  float* __restrict__ inc) {
   using S = Prep16<TI, KP, NI>;
   constexpr int N = S::NT, LDK = S::LDK, PLK = BT * LDK, PLT = BT * LDT;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -62,6 +62,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
   int64_t t0;
   int rows;
   if (!locate(tab, a.MC, chunk, t0, rows)) return;
+  constexpr int NPL = pm_planes(NI > 2);
+  unsigned char* const record = pm + item * pm_bytes(KP, NPL);
   const int warp = threadIdx.x >> 5;
   load_tokens<TI, LDK, KP, THREADS>(s.k, (const TI*)a.k + ((size_t)t0 * a.H + h) * a.K, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   auto load_v = [&](int v0) {
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
   if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
   cp_wait<0>();
   __syncthreads();
-  if (threadIdx.x == 0) decay[item] = s.gates.whole;
+  if (threadIdx.x == 0) *reinterpret_cast<float*>(record) = s.gates.whole;
   const int m0 = (warp >> 1) * 16, n0 = (warp & 1) * 32;
   {
     float acc[1][4][4];
@@ -125,9 +127,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
       zero(acc);
       const int mk = (warp >> 1) * 16 * MT;
       mm(acc, ColA<LDK, PLK, N>(s.k), RowB<LDT, PLT, NI>(s.y), mk, n0, 0, BT);
-      constexpr int NPL = NI > 2 ? 2 : 1;
       if (w)
-        store_pm<KP, NPL>(acc, mk, c0, n0, s.red, pm + item * (NPL * KP * (KP + 8)), pscale + item * (KP / 64));
+        store_pm<KP, NPL>(acc, mk, c0, n0, s.red, record);
       else
         each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
           *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, c0 + n)) = make_float2(x, y);
@@ -138,25 +139,24 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
 }
 
 // ------------------------------------------------------------------ output
-// Four warps, 16 rows each over all columns: the scores P stay in registers as left operand.
-constexpr int TH4 = 128;
-
-template <class TI, int KP, int VB> struct Out16 {
-  static constexpr int N = Planes<TI>::n, LDK = KP + 8, LDX = VB + 8;
+// 4 row groups of 16 x CG column groups of warps; panels of 64 value columns.
+template <class TI, int KP> struct Out16 {
+  static constexpr int N = Planes<TI>::n, LDK = KP + 8, CG = KP / 32, NTH = 128 * CG;
   bf k[N * BT * LDK];
   bf q[N * BT * LDK];
-  bf t[2 * BT * BT];  // fragment order
-  bf s[2 * KP * LDX];
-  bf x[2 * BT * LDX];
+  bf p[2 * BT * LDT];
+  bf s[2 * KP * LDT];
+  bf x[2 * BT * LDT];  // beta X, then U
   Gates gates;
+  static constexpr int resident(size_t bytes) { return bytes <= 75 * 1024 ? 3 : bytes <= 113 * 1024 ? 2 : 1; }
 };
 
-template <class TI, int KP, int VB>
+template <class TI, int KP>
 __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* __restrict__ tab, int VP, int tplanes,
                                                const bf* __restrict__ tinv, const bf* __restrict__ states,
                                                TI* __restrict__ o) {
-  using S = Out16<TI, KP, VB>;
-  constexpr int N = S::N, LDK = S::LDK, LDX = S::LDX, PLK = BT * LDK, PLX = BT * LDX, NT = VB / 8;
+  using S = Out16<TI, KP>;
+  constexpr int N = S::N, LDK = S::LDK, CG = S::CG, NTH = S::NTH, PLK = BT * LDK, PLT = BT * LDT, NT = 8 / CG;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
   const int64_t chunk = blockIdx.x / a.HV;
@@ -165,58 +165,42 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
   int64_t t0;
   int rows;
   if (!locate(tab, a.MC, chunk, t0, rows)) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, m0 = warp * 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cg = warp & (CG - 1), m0 = (warp / CG) * 16, n0 = cg * (64 / CG), i0 = m0 + (lane >> 2);
   const size_t qk = ((size_t)t0 * a.H + h) * a.K;
-  load_tokens<TI, LDK, KP, TH4>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
-  load_tokens<TI, LDK, KP, TH4>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  load_tokens<TI, LDK, KP, NTH>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
+  load_tokens<TI, LDK, KP, NTH>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   cp_commit();
-  copy16<TH4>(s.t, tinv + item * (2 * (size_t)tplanes * BT * BT), 2 * FRAG_PLANE);
   const bf* st = states + item * (2 * KP * VP);
-  load_planes<LDX, KP, VB, TH4>(s.s, st, VP);
+  load_planes<LDT, KP, 64, NTH>(s.s, st, VP);
   cp_commit();
   if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
   cp_wait<1>();
   __syncthreads();
-  uint32_t pf[4][2][4];  // planes of the warp's rows of P, by blocks of 16 columns
-  const int i0 = m0 + (lane >> 2);
   {
-    const RowA<LDK, PLK, N> qa(s.q);
-    const ColB<LDK, PLK, N> kb(s.k);
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (b <= warp) {
-        float c[1][2][4];
-        zero(c);
-        mm(c, qa, kb, m0, 16 * b, 0, KP);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int col = 16 * b + 8 * j + 2 * (lane & 3);
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int i = i0 + 8 * r;
-            float x = i >= col ? fade16(s.gates, i, col) * c[0][j][2 * r] : 0.f;
-            float y = i > col ? fade16(s.gates, i, col + 1) * c[0][j][2 * r + 1] : 0.f;
-            const uint32_t w = pack(x, y);
-            rest(w, x, y);
-            pf[b][0][2 * j + r] = w;
-            pf[b][1][2 * j + r] = pack(x, y);
-          }
-        }
-      }
+    float acc[1][NT][4];
+    zero(acc);
+    if (n0 <= m0 + 15) mm(acc, RowA<LDK, PLK, N>(s.q), ColB<LDK, PLK, N>(s.k), m0, n0, 0, KP);
+    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
+      put<2, PLT>(s.p + i * LDT + j, i >= j ? fade16(s.gates, i, j) * x : 0.f, i > j ? fade16(s.gates, i, j + 1) * y : 0.f);
+    });
   }
+  const FragA<2> t_a(tinv + item * (2 * (size_t)tplanes * BT * BT));
+  const RowB<LDT, KP * LDT, 2> s_b(s.s);
+  const RowB<LDT, PLT, 2> x_b(s.x);
   const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]};
   const float ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]};
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
   const TI* gv = (const TI*)a.v + vo;
   const bool even = a.V % 2 == 0 && (reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(o)) % 4 == 0;
-  for (int v0 = 0; v0 < a.V; v0 += VB) {
+  for (int v0 = 0; v0 < a.V; v0 += 64) {
     if (v0) {
       __syncthreads();  // readers of the previous panel are done
-      load_planes<LDX, KP, VB, TH4>(s.s, st + v0, VP);
+      load_planes<LDT, KP, 64, NTH>(s.s, st + v0, VP);
       cp_commit();
     }
     float xv[1][NT][4];
-    each_pair(xv, m0, 0, [&](int i, int n, float& x, float& y) {
+    each_pair(xv, m0, n0, [&](int i, int n, float& x, float& y) {
       const int c = v0 + n;
       x = y = 0.f;
       if (i < rows) {
@@ -238,44 +222,27 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
     float aq[1][NT][4], ak[1][NT][4];
     zero(aq);
     zero(ak);
-    const RowB<LDX, KP * LDX, 2> sb(s.s);
-    mm(ak, RowA<LDK, PLK, N>(s.k), sb, m0, 0, 0, KP);
-    mm(aq, RowA<LDK, PLK, N>(s.q), sb, m0, 0, 0, KP);
+    mm(ak, RowA<LDK, PLK, N>(s.k), s_b, m0, n0, 0, KP);
+    mm(aq, RowA<LDK, PLK, N>(s.q), s_b, m0, n0, 0, KP);
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        put<2, PLX>(s.x + (i0 + 8 * r) * LDX + 8 * j + 2 * (lane & 3),
+        put<2, PLT>(s.x + (i0 + 8 * r) * LDT + n0 + 8 * j + 2 * (lane & 3),
                     be[r] * (xv[0][j][2 * r] - ee[r] * ak[0][j][2 * r]),
                     be[r] * (xv[0][j][2 * r + 1] - ee[r] * ak[0][j][2 * r + 1]));
     __syncthreads();
     zero(ak);
-    const RowB<LDX, PLX, 2> xb(s.x);
-    mm(ak, FragA<2>(s.t), xb, m0, 0, 0, m0 + 16);
+    mm(ak, t_a, x_b, m0, n0, 0, m0 + 16);  // U
     __syncthreads();
-    each_pair(ak, m0, 0, [&](int i, int n, float x, float y) { put<2, PLX>(s.x + i * LDX + n, x, y); });
+    each_pair(ak, m0, n0, [&](int i, int n, float x, float y) { put<2, PLT>(s.x + i * LDT + n, x, y); });
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) aq[0][j][r] *= ee[r >> 1];
     __syncthreads();
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-      if (b <= warp) {
-#pragma unroll
-        for (int j = 0; j < NT; j += 2) {
-          uint32_t f0[4], f1[4];
-          xb.load(f0, 16 * b, 8 * j, 0);
-          xb.load(f1, 16 * b, 8 * j, 1);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            mma16(aq[0][j + u], pf[b][1], f0[2 * u], f0[2 * u + 1]);
-            mma16(aq[0][j + u], pf[b][0], f1[2 * u], f1[2 * u + 1]);
-            mma16(aq[0][j + u], pf[b][0], f0[2 * u], f0[2 * u + 1]);
-          }
-        }
-      }
-    each_pair(aq, m0, 0, [&](int i, int n, float x, float y) {
+    mm(aq, RowA<LDT, PLT, 2>(s.p), x_b, m0, n0, 0, m0 + 16);
+    each_pair(aq, m0, n0, [&](int i, int n, float x, float y) {
       const int c = v0 + n;
       if (i < rows && c < a.V) {
         TI* p = o + vo + i * vstride + c;
@@ -290,11 +257,11 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
   }
 }
 
-template <class TI, int KP, int VB>
-__global__ void __launch_bounds__(TH4, sizeof(Out16<TI, KP, VB>) <= 75 * 1024 ? 3 : 2)
+template <class TI, int KP>
+__global__ void __launch_bounds__(Out16<TI, KP>::NTH, Out16<TI, KP>::resident(sizeof(Out16<TI, KP>)))
     output16_kernel(Args a, const longlong2* __restrict__ tab, int VP, int tplanes, const bf* __restrict__ tinv,
                     const bf* __restrict__ states, TI* __restrict__ o) {
-  output16_chunk<TI, KP, VB>(a, tab, VP, tplanes, tinv, states, o);
+  output16_chunk<TI, KP>(a, tab, VP, tplanes, tinv, states, o);
   zero_uncovered(o, a, (int64_t)a.HV * a.V);
 }
 
@@ -302,19 +269,17 @@ template <class TI, int KP, int NI>
 int prep(const Args& a, const Saved& sv, int VP, float* b, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Prep16<TI, KP, NI>);
   cudaFuncSetAttribute(prep16_kernel<TI, KP, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  prep16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.decay, (bf*)sv.tinv, sv.pm, sv.pscale,
-                                                                  b);
+  prep16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, (bf*)sv.tinv, sv.pm, b);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
 }
 
 template <class TI, int KP>
 int output(const Args& a, const Saved& sv, int VP, bool exact, void* o, int64_t items, cudaStream_t st) {
-  constexpr int VB = KP == 64 ? 64 : 32;
-  const size_t smem = sizeof(Out16<TI, KP, VB>);
-  cudaFuncSetAttribute(output16_kernel<TI, KP, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  output16_kernel<TI, KP, VB><<<(unsigned)items, TH4, smem, st>>>(a, sv.chunk_tab, VP, exact ? 3 : 2, (const bf*)sv.tinv,
-                                                                 (const bf*)sv.s, (TI*)o);
+  const size_t smem = sizeof(Out16<TI, KP>);
+  cudaFuncSetAttribute(output16_kernel<TI, KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  output16_kernel<TI, KP><<<(unsigned)items, Out16<TI, KP>::NTH, smem, st>>>(
+      a, sv.chunk_tab, VP, t_planes(exact), (const bf*)sv.tinv, (const bf*)sv.s, (TI*)o);
   SSLA_CHECK_LAUNCH("gated_delta_rule output");
   return SSLA_OK;
 }

@@ -63,10 +63,12 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
     if (n0 <= m0)
       warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sk + m * LDK + k); },
                          [&](int k, int n) { return pair(sk + n * LDK + k); });
+    fade_scores<true, false>(acc, s.gates, m0, n0);
+    const int i0 = m0 + ((threadIdx.x & 31) >> 2);
+    const float b0 = s.gates.beta[i0], b1 = s.gates.beta[i0 + 8];
     each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
-      const float b = s.gates.beta[i];
-      s.a[i * LDC + j] = i > j ? b * s.gates.fade(i, j) * x : 0.f;
-      s.a[i * LDC + j + 1] = i > j + 1 ? b * s.gates.fade(i, j + 1) * y : 0.f;
+      const float b = i == i0 ? b0 : b1;
+      *reinterpret_cast<float2*>(s.a + i * LDC + j) = make_float2(b * x, b * y);
     });
   }
   __syncthreads();
@@ -385,9 +387,9 @@ __device__ __forceinline__ void output_chunk(const Args& a, const longlong2* __r
       if (p0 <= m0)
         warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
                            [&](int k, int n) { return pair(sk + n * LDK + k); });
+      fade_scores<false, false>(acc, s.gates, m0, p0);
       each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
-        *reinterpret_cast<float2*>(s.p + i * LDC + j) =
-            stage2<SP>(i >= j ? s.gates.fade(i, j) * x : 0.f, i > j ? s.gates.fade(i, j + 1) * y : 0.f);
+        *reinterpret_cast<float2*>(s.p + i * LDC + j) = make_float2(x, y);
       });
     }
     cp_wait<0>();

@@ -70,7 +70,8 @@ inline size_t saved_layout(void* base, const Plan& p, int dtype, bool exact, int
   Saved s;
   s.chunk_off = (int*)take(4 * (N + 1));
   s.chunk_tab = (longlong2*)take(16 * (size_t)p.MC);
-  s.tinv = (float*)take((dtype == SSLA_F32 ? 4 : 4 * t_planes(exact)) * items * BT * BT);
+  // fp32 [64][64], or t_planes of 10 + 10 blocks of 512 bytes
+  s.tinv = (float*)take((dtype == SSLA_F32 ? 4 * BT * BT : t_planes(exact) * 2 * 10 * 512) * items);
   s.pm = (unsigned char*)take(items * pm_bytes(KP, pm_planes(exact)));
   s.s = (float*)take(4 * items * KP * VP);
   if (out) *out = s;
@@ -332,8 +333,6 @@ struct Gates {
   float start[BT];       // exp(gc)
   float left[BT];        // exp(gC - gc)
   float whole;           // exp(gC)
-  // exp(gc_i - gc_j), i >= j
-  __device__ __forceinline__ float fade(int i, int j) const { return expf((hi[i] - hi[j]) + (lo[i] - lo[j])); }
 };
 
 // One warp.  g below kMinGate counts as kMinGate (both decay to 0), NaN stays.
@@ -371,6 +370,28 @@ __device__ __forceinline__ void load_gates(Gates& s, const Args& a, int64_t t0, 
     s.left[r] = expf((float)(all - c[i]));
   }
   if (lane == 0) s.whole = expf((float)all);
+}
+
+// acc(i, j) *= exp(gc_i - gc_j) where i >= j (STRICT: i > j), 0 elsewhere, in place: with the stores
+// of the results between them, every read of a gate would wait for its own latency.  FAST takes the
+// exponential from the special-function unit (about 2^-22, for results that leave in 16 bits).
+template <bool STRICT, bool FAST, int NT>
+__device__ __forceinline__ void fade_scores(float (&acc)[1][NT][4], const Gates& s, int m0, int n0) {
+  const int lane = threadIdx.x & 31, i0 = m0 + (lane >> 2), j0 = n0 + 2 * (lane & 3);
+  const float hi[2] = {s.hi[i0], s.hi[i0 + 8]}, lo[2] = {s.lo[i0], s.lo[i0 + 8]};
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const float2 h = *reinterpret_cast<const float2*>(s.hi + j0 + 8 * t), l = *reinterpret_cast<const float2*>(s.lo + j0 + 8 * t);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = i0 + (r >> 1) * 8, j = j0 + 8 * t + (r & 1);
+      const float x = (hi[r >> 1] - (r & 1 ? h.y : h.x)) + (lo[r >> 1] - (r & 1 ? l.y : l.x));
+      float e;
+      if (FAST) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(1.4426950408889634f * x));
+      else e = expf(x);
+      acc[0][t][r] = (STRICT ? i > j : i >= j) ? acc[0][t][r] * e : 0.f;
+    }
+  }
 }
 
 __device__ __forceinline__ bool locate(const longlong2* tab, int64_t MC, int64_t chunk, int64_t& t0, int& rows) {

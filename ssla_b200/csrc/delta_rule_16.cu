@@ -25,17 +25,19 @@ template <class TI, int KP, int NI> struct Prep16 {
   Gates gates;
 };
 
-// Planes of T and of its transpose in fragment order.
+// Planes of T, then of its transpose, as fragments.
 template <int NI> __device__ __forceinline__ void write_t(const float* t, bf* out) {
-  for (int i = threadIdx.x; i < 2 * 16 * 32; i += THREADS) {
-    const int lane = i & 31, kb = (i >> 5) & 3, mb = (i >> 7) & 3, tr = i >> 9;
-    const int r = 16 * mb + (lane >> 2), c = 16 * kb + 2 * (lane & 3);
+  for (int i = threadIdx.x; i < 2 * FRAGS; i += THREADS) {
+    const int tr = i >= FRAGS, f = i - tr * FRAGS, lane = f & 31, blk = f >> 5;
+    const int mb = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, kb = blk - mb * (mb + 1) / 2;
+    // the place in T: fragment rows run along T's rows, or its columns for the transpose
+    const int fr = lane >> 2, fc = 2 * (lane & 3);
     uint32_t w[NI][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int rr = r + (j & 1) * 8, cc = c + (j >> 1) * 8;
-      float x = tr ? t[cc * LDC + rr] : t[rr * LDC + cc];
-      float y = tr ? t[(cc + 1) * LDC + rr] : t[rr * LDC + cc + 1];
+      const int rr = fr + (j & 1) * 8, cc = fc + (j >> 1) * 8;
+      float x = tr ? t[(16 * mb + cc) * LDC + 16 * kb + rr] : t[(16 * mb + rr) * LDC + 16 * kb + cc];
+      float y = tr ? t[(16 * mb + cc + 1) * LDC + 16 * kb + rr] : t[(16 * mb + rr) * LDC + 16 * kb + cc + 1];
 #pragma unroll
       for (int p = 0; p < NI; ++p) {
         w[p][j] = pack(x, y);
@@ -44,7 +46,7 @@ template <int NI> __device__ __forceinline__ void write_t(const float* t, bf* ou
     }
 #pragma unroll
     for (int p = 0; p < NI; ++p)
-      reinterpret_cast<uint4*>(out)[((tr * NI + p) * 16 + mb * 4 + kb) * 32 + lane] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+      reinterpret_cast<uint4*>(out)[(tr * NI + p) * FRAGS + f] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
   }
 }
 
@@ -81,15 +83,17 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
     float acc[1][4][4];
     zero(acc);
     if (n0 <= m0) mm(acc, RowA<LDK, PLK, N>(s.k), ColB<LDK, PLK, N>(s.k), m0, n0, 0, KP);
+    fade_scores<true, (NI < 3)>(acc, s.gates, m0, n0);
+    const int i0 = m0 + ((threadIdx.x & 31) >> 2);
+    const float b0 = s.gates.beta[i0], b1 = s.gates.beta[i0 + 8];
     each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
-      const float b = s.gates.beta[i];
-      *reinterpret_cast<float2*>(s.a + i * LDC + j) =
-          make_float2(i > j ? b * s.gates.fade(i, j) * x : 0.f, i > j + 1 ? b * s.gates.fade(i, j + 1) * y : 0.f);
+      const float b = i == i0 ? b0 : b1;
+      *reinterpret_cast<float2*>(s.a + i * LDC + j) = make_float2(b * x, b * y);
     });
   }
   __syncthreads();
   unit_lower_inverse(s.a, s.t, reinterpret_cast<float*>(s.y));
-  write_t<NI>(s.t, tinv + item * (2 * NI * BT * BT));
+  write_t<NI>(s.t, tinv + item * (2 * NI * FRAG_ELEMS));
   auto scale_t = [&](bool w) {  // tc = T diag(beta [exp(gc)])
     for (int i = threadIdx.x; i < BT * BT / 2; i += THREADS) {
       const int r = i >> 5, c = (i & 31) * 2;
@@ -115,8 +119,10 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
       const RowA<LDT, PLT, NI> t(s.tc);
       if (w) mm(acc, t, RowB<LDK, PLK, N>(s.k + c0), m0, n0, 0, m0 + 16);
       else mm(acc, t, RowB<LDT, PLT, N>(s.v), m0, n0, 0, m0 + 16);
+      const int i0 = m0 + ((threadIdx.x & 31) >> 2);
+      const float l0 = s.gates.left[i0], l1 = s.gates.left[i0 + 8];
       each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
-        const float l = s.gates.left[i];
+        const float l = i == i0 ? l0 : l1;
         put<NI, PLT>(s.y + i * LDT + j, x * l, y * l);
       });
     }
@@ -144,6 +150,7 @@ template <class TI, int KP> struct Out16 {
   static constexpr int N = Planes<TI>::n, LDK = KP + 8, CG = KP / 32, NTH = 128 * CG;
   bf k[N * BT * LDK];
   bf q[N * BT * LDK];
+  bf t[2 * FRAG_ELEMS];
   bf p[2 * BT * LDT];
   bf s[2 * KP * LDT];
   bf x[2 * BT * LDT];  // beta X, then U
@@ -171,6 +178,7 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
   load_tokens<TI, LDK, KP, NTH>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   load_tokens<TI, LDK, KP, NTH>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   cp_commit();
+  copy16<NTH>(s.t, tinv + item * (2 * (size_t)tplanes * FRAG_ELEMS), 2 * FRAG_BYTES);
   const bf* st = states + item * (2 * KP * VP);
   load_planes<LDT, KP, 64, NTH>(s.s, st, VP);
   cp_commit();
@@ -181,11 +189,10 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
     float acc[1][NT][4];
     zero(acc);
     if (n0 <= m0 + 15) mm(acc, RowA<LDK, PLK, N>(s.q), ColB<LDK, PLK, N>(s.k), m0, n0, 0, KP);
-    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
-      put<2, PLT>(s.p + i * LDT + j, i >= j ? fade16(s.gates, i, j) * x : 0.f, i > j ? fade16(s.gates, i, j + 1) * y : 0.f);
-    });
+    fade_scores<false, true>(acc, s.gates, m0, n0);
+    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) { put<2, PLT>(s.p + i * LDT + j, x, y); });
   }
-  const FragA<2> t_a(tinv + item * (2 * (size_t)tplanes * BT * BT));
+  const FragA<2, false> t_a(s.t);
   const RowB<LDT, KP * LDT, 2> s_b(s.s);
   const RowB<LDT, PLT, 2> x_b(s.x);
   const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]};
@@ -200,23 +207,7 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
       cp_commit();
     }
     float xv[1][NT][4];
-    each_pair(xv, m0, n0, [&](int i, int n, float& x, float& y) {
-      const int c = v0 + n;
-      x = y = 0.f;
-      if (i < rows) {
-        const TI* p = gv + i * vstride + c;
-        if (even) {
-          if (c < a.V) {
-            const float2 z = pair(p);
-            x = z.x;
-            y = z.y;
-          }
-        } else {
-          if (c < a.V) x = ldf(p);
-          if (c + 1 < a.V) y = ldf(p + 1);
-        }
-      }
-    });
+    load_pairs(xv, gv + v0, vstride, rows, a.V - v0, m0, n0, even);
     cp_wait<0>();
     __syncthreads();
     float aq[1][NT][4], ak[1][NT][4];

@@ -64,13 +64,17 @@ template <int LD, int PLANE, int N> struct ColA {
     ldsm4t(r, at + 2 * (p * PLANE + k * LD + m));
   }
 };
-// Fragments in order: [plane][m / 16][k / 16][lane] of 16 bytes (a [64, 64] matrix).
-template <int N> struct FragA {
+// The 10 blocks of a lower triangular [64, 64] matrix as left operand fragments: [plane][block][lane]
+// of 16 bytes, block (m, k) at m (m + 1) / 2 + k.  TR: fragments of the transpose, block (m, k) at
+// the place of (k, m).
+constexpr int FRAGS = 10 * 32, FRAG_BYTES = FRAGS * 16, FRAG_ELEMS = FRAG_BYTES / 2;  // of a plane
+template <int N, bool TR> struct FragA {
   static constexpr int n = N;
   const uint4* at;
   __device__ __forceinline__ FragA(const void* p) : at((const uint4*)p + (threadIdx.x & 31)) {}
   __device__ __forceinline__ void load(uint32_t (&r)[4], int m, int k, int p) const {
-    const uint4 x = at[((p * 4 + (m >> 4)) * 4 + (k >> 4)) * 32];
+    const int i = (TR ? k : m) >> 4, j = (TR ? m : k) >> 4;
+    const uint4 x = at[p * FRAGS + (i * (i + 1) / 2 + j) * 32];
     r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
   }
 };
@@ -202,13 +206,36 @@ template <int NTH> __device__ __forceinline__ void copy16(void* dst, const void*
   for (int i = threadIdx.x * 16; i < bytes; i += NTH * 16) cp16((char*)dst + i, (const char*)src + i);
 }
 
-constexpr int FRAG_PLANE = 4 * 4 * 32 * 16;  // bytes of one plane of a [64, 64] matrix in fragment order
-
-// exp of an in-chunk difference on the special-function unit (about 2^-22; the results leave in 16 bits)
-__device__ __forceinline__ float fade16(const Gates& s, int i, int j) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.4426950408889634f * ((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]))));
-  return r;
+// Pairs (row i, columns c, c + 1) of a token matrix in the accumulator layout, zeros outside: all
+// loads before the first use.  even: an even number of columns, 4-byte aligned.
+template <class TI, int NT>
+__device__ __forceinline__ void load_pairs(float (&acc)[1][NT][4], const TI* src, size_t stride, int rows, int cols,
+                                           int m0, int n0, bool even) {
+  const int lane = threadIdx.x & 31, i0 = m0 + (lane >> 2), c0 = n0 + 2 * (lane & 3);
+  uint32_t w[NT][2];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int i = i0 + 8 * r, c = c0 + 8 * j;
+      const TI* p = src + i * stride + c;
+      w[j][r] = 0;
+      if (even) {
+        if (i < rows && c < cols) w[j][r] = __ldg(reinterpret_cast<const unsigned*>(p));
+      } else {
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+        if (i < rows && c < cols) w[j][r] = __ldg(q);
+        if (i < rows && c + 1 < cols) w[j][r] |= (uint32_t)__ldg(q + 1) << 16;
+      }
+    }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float2 z = pair(reinterpret_cast<const TI*>(&w[j][r]));
+      acc[0][j][2 * r] = z.x;
+      acc[0][j][2 * r + 1] = z.y;
+    }
 }
 
 }  // namespace h16

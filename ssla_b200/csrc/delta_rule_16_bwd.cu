@@ -14,7 +14,7 @@ template <class TI, int KP, int NI> struct Adj16 {
   bf k[N * BT * LDK];
   bf q[N * BT * LDK];
   bf d[N * BT * LDT];
-  bf t[NI * BT * BT];   // fragment order
+  bf t[NI * FRAG_ELEMS];
   bf w[NI * BT * LDK];  // beta exp(gc) K, then W, then scale qh
   bf p[NI * BT * LDT];
   Gates gates;
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 10
   const size_t qk = ((size_t)t0 * a.H + h) * a.K;
   load_tokens<TI, LDK, KP, THREADS>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   load_tokens<TI, LDK, KP, THREADS>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
-  copy16<THREADS>(s.t, tinv + item * (2 * NI * BT * BT), NI * FRAG_PLANE);
+  copy16<THREADS>(s.t, tinv + item * (2 * NI * FRAG_ELEMS), NI * FRAG_BYTES);
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V;
   const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
   auto load_d = [&](int v0) {
@@ -54,9 +54,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 10
     float acc[1][4][4];
     zero(acc);
     if (n0 <= m0) mm(acc, RowA<LDK, PLK, N>(s.q), ColB<LDK, PLK, N>(s.k), m0, n0, 0, KP);
-    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
-      put<NI, PLT>(s.p + i * LDT + j, i >= j ? s.gates.fade(i, j) * x : 0.f, i > j ? s.gates.fade(i, j + 1) * y : 0.f);
-    });
+    fade_scores<false, (NI < 3)>(acc, s.gates, m0, n0);
+    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) { put<NI, PLT>(s.p + i * LDT + j, x, y); });
   }
   for (int i = threadIdx.x; i < BT * KP / 2; i += THREADS) {
     const int r = i / (KP / 2), c = (i % (KP / 2)) * 2;
@@ -73,23 +72,27 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 10
   const RowB<LDK, PLK, NI> wb(s.w);
   float acc[1][NK][4];
   zero(acc);
-  mm(acc, FragA<NI>(s.t), wb, m0, k0, 0, m0 + 16);
+  mm(acc, FragA<NI, false>(s.t), wb, m0, k0, 0, m0 + 16);
   __syncthreads();
   each_pair(acc, m0, k0, [&](int i, int n, float x, float y) { put<NI, PLK>(s.w + i * LDK + n, x, y); });
   __syncthreads();
   zero(acc);
   mm(acc, RowA<LDT, PLT, NI>(s.p), wb, m0, k0, 0, m0 + 16);
   __syncthreads();
-  each_pair(acc, m0, k0, [&](int i, int n, float x, float y) {
+  const int i0 = m0 + ((threadIdx.x & 31) >> 2);
+  const float e0 = s.gates.start[i0], e1 = s.gates.start[i0 + 8];
+  each_pair(acc, m0, k0, [&](int i, int n, float& x, float& y) {
     float2 z = pair(s.q + i * LDK + n);
     if (N > 1) {
       const float2 y2 = pair(s.q + PLK * (N - 1) + i * LDK + n);
       z.x += y2.x;
       z.y += y2.y;
     }
-    const float e = s.gates.start[i];
-    put<NI, PLK>(s.w + i * LDK + n, a.scale * (e * z.x - x), a.scale * (e * z.y - y));
+    const float e = i == i0 ? e0 : e1;
+    x = a.scale * (e * z.x - x);
+    y = a.scale * (e * z.y - y);
   });
+  each_pair(acc, m0, k0, [&](int i, int n, float x, float y) { put<NI, PLK>(s.w + i * LDK + n, x, y); });
   constexpr int MT = KP / 64;
   const int mk = (warp >> 1) * 16 * MT;
   for (int v0 = 0; v0 < VP; v0 += 64) {
@@ -111,10 +114,11 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 10
 // ------------------------------------------------------------------ gradients of a chunk
 // Warps: 4 groups of 16 rows x CG column groups.
 template <class TI, int KP> struct Bwd16 {
-  static constexpr int N = Planes<TI>::n, LDK = KP + 8, VB = KP / 2, LDX = VB + 8, CG = KP / 32, NTH = 128 * CG;
+  static constexpr int N = Planes<TI>::n, LDK = KP + 8, VB = N > 1 ? 32 : KP / 2, LDX = VB + 8, CG = VB / 16, NTH = 128 * CG;
   bf k[N * BT * LDK];
   bf q[N * BT * LDK];
   bf d[N * BT * LDX];
+  bf t[4 * FRAG_ELEMS];  // T, transpose of T
   bf p[2 * BT * LDT];  // P, then dP
   bf x[2 * BT * LDX];  // beta X, then U;  x and f at last -beta E
   bf f[2 * BT * LDX];  // dU, then F
@@ -158,8 +162,11 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
   const bool even = a.V % 2 == 0 && (reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(dv)) % 4 == 0;
   const TI* gv = (const TI*)a.v + vo;
-  const bf* tf = tinv + item * (2 * (size_t)tplanes * BT * BT);
-  const FragA<2> t_a(tf), tt_a(tf + (size_t)tplanes * BT * BT);
+  const bf* tf = tinv + item * (2 * (size_t)tplanes * FRAG_ELEMS);
+  copy16<NTH>(s.t, tf, 2 * FRAG_BYTES);
+  copy16<NTH>(s.t + 2 * FRAG_ELEMS, tf + (size_t)tplanes * FRAG_ELEMS, 2 * FRAG_BYTES);
+  const FragA<2, false> t_a(s.t);
+  const FragA<2, true> tt_a(s.t + 2 * FRAG_ELEMS);
   const bf* gs = states + item * (2 * KP * VP);
   const bf* ge = ds + item * (2 * KP * VP);
   const RowA<LDK, PLK, N> k_a(s.k), q_a(s.q);
@@ -190,28 +197,11 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
       float acc[1][NP][4];
       zero(acc);
       if (low) mm(acc, q_a, ColB<LDK, PLK, N>(s.k), m0, p0, 0, KP);
-      each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
-        put<2, PLT>(s.p + i * LDT + j, i >= j ? fade16(s.gates, i, j) * x : 0.f, i > j ? fade16(s.gates, i, j + 1) * y : 0.f);
-      });
+      fade_scores<false, true>(acc, s.gates, m0, p0);
+      each_pair(acc, m0, p0, [&](int i, int j, float x, float y) { put<2, PLT>(s.p + i * LDT + j, x, y); });
     }
     float xv[1][NT][4];
-    each_pair(xv, m0, n0, [&](int i, int n, float& x, float& y) {
-      const int c = v0 + n;
-      x = y = 0.f;
-      if (i < rows) {
-        const TI* p = gv + i * vstride + c;
-        if (even) {
-          if (c < a.V) {
-            const float2 z = pair(p);
-            x = z.x;
-            y = z.y;
-          }
-        } else {
-          if (c < a.V) x = ldf(p);
-          if (c + 1 < a.V) y = ldf(p + 1);
-        }
-      }
-    });
+    load_pairs(xv, gv + v0, vstride, rows, a.V - v0, m0, n0, even);
     cp_wait<0>();
     __syncthreads();
     float ks[1][NT][4], du[1][NT][4];
@@ -220,13 +210,13 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
     mm(ks, k_a, s_b, m0, n0, 0, KP);
     mm(du, k_a, e_b, m0, n0, 0, KP);
     const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]};
+    const float ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]}, le[2] = {s.gates.left[i0], s.gates.left[i0 + 8]};
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = i0 + (r >> 1) * 8;
-        xv[0][j][r] -= s.gates.start[i] * ks[0][j][r];
-        du[0][j][r] *= s.gates.left[i];
+        xv[0][j][r] -= ee[r >> 1] * ks[0][j][r];
+        du[0][j][r] *= le[r >> 1];
       }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -290,15 +280,14 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   }
   __syncthreads();
   bf* const sE = s.s;  // E;  -beta E at s.x
-  each_pair(ap, m0, p0, [&](int i, int j, float x, float y) {
-    put<2, PLT>(s.p + i * LDT + j, i >= j ? a.scale * fade16(s.gates, i, j) * x : 0.f,
-                i > j ? a.scale * fade16(s.gates, i, j + 1) * y : 0.f);
-  });
+  const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]}, ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]};
+  const float le[2] = {s.gates.left[i0], s.gates.left[i0 + 8]};
+  fade_scores<false, true>(ap, s.gates, m0, p0);
+  fade_scores<true, true>(ae, s.gates, m0, p0);
+  each_pair(ap, m0, p0, [&](int i, int j, float x, float y) { put<2, PLT>(s.p + i * LDT + j, a.scale * x, a.scale * y); });
   each_pair(ae, m0, p0, [&](int i, int j, float x, float y) {
-    x = i > j ? fade16(s.gates, i, j) * x : 0.f;
-    y = i > j + 1 ? fade16(s.gates, i, j + 1) * y : 0.f;
     put<2, PLT>(sE + i * LDT + j, x, y);
-    const float b = -s.gates.beta[i];
+    const float b = i == i0 ? -be[0] : -be[1];
     put<2, PLT>(s.x + i * LDT + j, b * x, b * y);
   });
   __syncthreads();
@@ -327,11 +316,9 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
     for (int j = 0; j < NK; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = i0 + (r >> 1) * 8;
-        const float b = s.gates.beta[i], e = s.gates.start[i];
-        ar[0][j][r] = -b * fmaf(e, ar[0][j][r], ag[0][j][r]);
-        aq[0][j][r] *= a.scale * e;
-        ac[0][j][r] *= s.gates.left[i];
+        ar[0][j][r] = -be[r >> 1] * fmaf(ee[r >> 1], ar[0][j][r], ag[0][j][r]);
+        aq[0][j][r] *= a.scale * ee[r >> 1];
+        ac[0][j][r] *= le[r >> 1];
       }
   }
   row_dot(ar, s.k, rr);

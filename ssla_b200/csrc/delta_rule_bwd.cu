@@ -65,9 +65,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2
     if (n0 <= m0)
       warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
                          [&](int k, int n) { return pair(sk + n * LDK + k); });
+    fade_scores<false, false>(acc, s.gates, m0, n0);
     each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
-      *reinterpret_cast<float2*>(s.p + i * LDC + j) =
-          stage2<SP>(i >= j ? s.gates.fade(i, j) * x : 0.f, i > j ? s.gates.fade(i, j + 1) * y : 0.f);
+      *reinterpret_cast<float2*>(s.p + i * LDC + j) = make_float2(x, y);
     });
   }
   float acc[1][NK][4];
@@ -182,9 +182,9 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
       if (low)
         warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
                            [&](int k, int n) { return pair(sk + n * LDK + k); });
+      fade_scores<false, false>(acc, s.gates, m0, p0);
       each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
-        *reinterpret_cast<float2*>(s.p + i * LDP + j) =
-            stage2<SP>(i >= j ? s.gates.fade(i, j) * x : 0.f, i > j ? s.gates.fade(i, j + 1) * y : 0.f);
+        *reinterpret_cast<float2*>(s.p + i * LDP + j) = make_float2(x, y);
       });
     }
     float xv[1][NT][4];
@@ -276,13 +276,13 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   }
   __syncthreads();
   // dP and E take the places of P and T
+  fade_scores<false, false>(ap, s.gates, m0, p0);
+  fade_scores<true, false>(ae, s.gates, m0, p0);
   each_pair(ap, m0, p0, [&](int i, int j, float x, float y) {
-    *reinterpret_cast<float2*>(s.p + i * LDP + j) = stage2<SP>(
-        i >= j ? a.scale * s.gates.fade(i, j) * x : 0.f, i > j ? a.scale * s.gates.fade(i, j + 1) * y : 0.f);
+    *reinterpret_cast<float2*>(s.p + i * LDP + j) = make_float2(a.scale * x, a.scale * y);
   });
   each_pair(ae, m0, p0, [&](int i, int j, float x, float y) {
-    *reinterpret_cast<float2*>(s.t + i * LDP + j) =
-        stage2<SP>(i > j ? s.gates.fade(i, j) * x : 0.f, i > j + 1 ? s.gates.fade(i, j + 1) * y : 0.f);
+    *reinterpret_cast<float2*>(s.t + i * LDP + j) = make_float2(x, y);
   });
   __syncthreads();
   auto fk_tok = [&](int k, int n) { return column<LDK>(sk + k * LDK + n); };

@@ -335,21 +335,36 @@ struct Gates {
   float whole;           // exp(gC)
 };
 
+// Two entries of a gate array, 0 behind the end: every load leaves before the first is used.
+__device__ __forceinline__ uint32_t gate_raw(const void* p, int dt, size_t i, bool in) {
+  uint32_t x = 0;
+  if (in && dt == SSLA_F32) x = __ldg((const uint32_t*)p + i);
+  if (in && dt != SSLA_F32) x = __ldg((const unsigned short*)p + i);
+  return x;
+}
+__device__ __forceinline__ float gate_value(uint32_t x, int dt) {
+  if (dt == SSLA_F32) return __uint_as_float(x);
+  if (dt == SSLA_BF16) return __uint_as_float(x << 16);
+  return __half2float(__ushort_as_half((unsigned short)x));
+}
+
 // One warp.  g below kMinGate counts as kMinGate (both decay to 0), NaN stays.
 __device__ __forceinline__ void load_gates(Gates& s, const Args& a, int64_t t0, int rows, int hv) {
   const int lane = threadIdx.x & 31;
+  uint32_t raw[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const size_t at = (size_t)(t0 + 2 * lane + i) * a.HV + hv;
+    const bool in = 2 * lane + i < rows;
+    raw[i][0] = gate_raw(a.g, a.dt_g, at, in);
+    raw[i][1] = gate_raw(a.beta, a.dt_b, at, in);
+  }
   double x[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = 2 * lane + i;
-    float g = 0.f, b = 0.f;
-    if (r < rows) {
-      const size_t at = (size_t)(t0 + r) * a.HV + hv;
-      g = ld_any(a.g, a.dt_g, at);
-      b = ld_any(a.beta, a.dt_b, at);
-      g = g < kMinGate ? kMinGate : g;
-    }
-    s.beta[r] = b;
+    float g = gate_value(raw[i][0], a.dt_g);
+    g = g < kMinGate ? kMinGate : g;
+    s.beta[2 * lane + i] = gate_value(raw[i][1], a.dt_b);
     x[i] = g;
   }
   double sum = x[0] + x[1];

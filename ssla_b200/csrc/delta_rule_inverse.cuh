@@ -6,26 +6,46 @@ namespace delta {
 
 // (I + A)^-1 of a 64 x 64 tile by one block of THREADS threads:
 // sA strictly lower triangular -> sT, upper triangle zero; sY is scratch (>= 2048 floats).
-// Diagonal 16 x 16 blocks by substitution (one thread a column), then pairs of blocks twice as
-// large: the block below the diagonal is -T22 A21 T11.
+// Diagonal 8 x 8 blocks by substitution (one thread a column, its block's entries in registers
+// first), then pairs of blocks twice as large: the block below the diagonal is -T22 A21 T11.
 __device__ __forceinline__ void unit_lower_inverse(const float* sA, float* sT, float* sY) {
   const int tid = threadIdx.x;
-  for (int i = tid; i < BT * BT; i += THREADS) {
-    const int r = i >> 6, c = i & 63;
-    if ((r >> 4) != (c >> 4)) sT[r * LDC + c] = 0.f;
+  for (int i = tid; i < BT * BT / 4; i += THREADS) {
+    const int r = i >> 4, c = (i & 15) * 4;
+    if ((r >> 3) != (c >> 3)) *reinterpret_cast<float4*>(sT + r * LDC + c) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   if (tid < 64) {
-    const int b = (tid >> 4) * 16, c = tid & 15;
-    float x[16];
+    const int b = tid & ~7, c = tid & 7;
+    float a[8][8], x[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float acc = i == c ? 1.f : 0.f;
+    for (int i = 1; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < i; ++j) acc = fmaf(-sA[(b + i) * LDC + b + j], x[j], acc);
-      x[i] = acc;
+      for (int j = 0; j < i; j += 4) {
+        const float4 z = *reinterpret_cast<const float4*>(sA + (b + i) * LDC + b + j);
+        a[i][j] = z.x; a[i][j + 1] = z.y; a[i][j + 2] = z.z; a[i][j + 3] = z.w;
+      }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = i == c ? 1.f : 0.f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) x[i] = fmaf(-a[i][j], x[j], x[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sT[(b + i) * LDC + b + c] = x[i];
+    for (int i = 0; i < 8; ++i) sT[(b + i) * LDC + b + c] = x[i];
+  }
+  __syncthreads();
+  {  // 8 -> 16, four pairs, 64 threads each: thread = (row, column)
+    const int d = (tid >> 6) * 16, r = (tid >> 3) & 7, c = tid & 7;
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x = fmaf(sA[(d + 8 + r) * LDC + d + j], sT[(d + j) * LDC + d + c], x);
+    sY[tid] = x;
+    __syncthreads();
+    x = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x = fmaf(-sT[(d + 8 + r) * LDC + d + 8 + j], sY[(tid & ~63) + j * 8 + c], x);
+    __syncthreads();
+    sT[(d + 8 + r) * LDC + d + c] = x;
   }
   __syncthreads();
   {  // 16 -> 32, two pairs, 128 threads each: thread = (row, 2 columns)

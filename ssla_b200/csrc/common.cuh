@@ -8,6 +8,7 @@
 #include <stdio.h>
 #include <stdarg.h>
 
+#include <atomic>
 #include <utility>
 
 #include "../../include/ssla_b200.h"
@@ -78,6 +79,18 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
   cfg.attrs = at;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// Allows KERN `bytes` of dynamic shared memory on the current device, once per device (the driver
+// call costs a microsecond at every launch).
+template <auto KERN> inline void allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
+  if (cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess)
+    done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 inline size_t dtype_size(int dt) { return dt == SSLA_F32 ? 4 : 2; }

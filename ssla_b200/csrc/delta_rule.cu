@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
 
 template <int KP, int VS, bool TRANS, int NP> int launch_chain(const ChainArgs& a, int64_t N, cudaStream_t st) {
   constexpr int smem = ChainSmem<KP, VS, NP>::bytes;
-  cudaFuncSetAttribute(chain_kernel<KP, VS, TRANS, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  allow_smem<chain_kernel<KP, VS, TRANS, NP>>((int)smem);
   const int64_t grid = N * a.HV * a.slices;
   if (grid == 0) return SSLA_OK;
   chain_kernel<KP, VS, TRANS, NP><<<(unsigned)grid, KP * 2, smem, st>>>(a);
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlo
 template <int KP>
 int prep32(const Args& a, const Saved& sv, int VP, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(PrepSmem<KP>);
-  cudaFuncSetAttribute(prep_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<prep_kernel<KP>>((int)smem);
   prep_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.pm, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
@@ -451,7 +451,7 @@ template <int KP>
 int output32(const Args& a, const Saved& sv, int VP, void* o, int64_t items, cudaStream_t st) {
   constexpr int VB = KP == 64 ? 64 : 32;
   const size_t smem = sizeof(OutSmem<KP, VB>);
-  cudaFuncSetAttribute(output_kernel<KP, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<output_kernel<KP, VB>>((int)smem);
   output_kernel<KP, VB><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.s, (TI*)o);
   SSLA_CHECK_LAUNCH("gated_delta_rule output");
   return SSLA_OK;

@@ -145,15 +145,17 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
 }
 
 // ------------------------------------------------------------------ output
-// 4 row groups of 16 x CG column groups of warps; panels of 64 value columns.
+// 4 row groups of 16 x 2 column groups of warps; panels of VB value columns, so that two or three
+// blocks fit an SM (KP = 128 with panels of 64, one block of 16 warps: 340 us against XXX for the
+// 32768-token prompt).
 template <class TI, int KP> struct Out16 {
-  static constexpr int N = Planes<TI>::n, LDK = KP + 8, CG = KP / 32, NTH = 128 * CG;
+  static constexpr int N = Planes<TI>::n, LDK = KP + 8, VB = KP == 64 ? 64 : 32, LDX = VB + 8, CG = 2, NTH = 128 * CG;
   bf k[N * BT * LDK];
   bf q[N * BT * LDK];
   bf t[2 * FRAG_ELEMS];
   bf p[2 * BT * LDT];
-  bf s[2 * KP * LDT];
-  bf x[2 * BT * LDT];  // beta X, then U
+  bf s[2 * KP * LDX];
+  bf x[2 * BT * LDX];  // beta X, then U
   Gates gates;
   static constexpr int resident(size_t bytes) { return bytes <= 75 * 1024 ? 3 : bytes <= 113 * 1024 ? 2 : 1; }
 };
@@ -163,7 +165,7 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
                                                const bf* __restrict__ tinv, const bf* __restrict__ states,
                                                TI* __restrict__ o) {
   using S = Out16<TI, KP>;
-  constexpr int N = S::N, LDK = S::LDK, CG = S::CG, NTH = S::NTH, PLK = BT * LDK, PLT = BT * LDT, NT = 8 / CG;
+  constexpr int N = S::N, LDK = S::LDK, CG = S::CG, NTH = S::NTH, PLK = BT * LDK, PLT = BT * LDT, VB = S::VB, LDX = S::LDX, PLX = BT * LDX, NT = VB / CG / 8, NP = 8 / CG;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
   const int64_t chunk = blockIdx.x / a.HV;
@@ -173,37 +175,37 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
   int rows;
   if (!locate(tab, a.MC, chunk, t0, rows)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cg = warp & (CG - 1), m0 = (warp / CG) * 16, n0 = cg * (64 / CG), i0 = m0 + (lane >> 2);
+  const int cg = warp & (CG - 1), m0 = (warp / CG) * 16, n0 = cg * (VB / CG), p0 = cg * (64 / CG), i0 = m0 + (lane >> 2);
   const size_t qk = ((size_t)t0 * a.H + h) * a.K;
   load_tokens<TI, LDK, KP, NTH>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   load_tokens<TI, LDK, KP, NTH>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   cp_commit();
   copy16<NTH>(s.t, tinv + item * (2 * (size_t)tplanes * FRAG_ELEMS), 2 * FRAG_BYTES);
   const bf* st = states + item * (2 * KP * VP);
-  load_planes<LDT, KP, 64, NTH>(s.s, st, VP);
+  load_planes<LDX, KP, VB, NTH>(s.s, st, VP);
   cp_commit();
   if (warp == 0) load_gates(s.gates, a, t0, rows, hv);
   cp_wait<1>();
   __syncthreads();
   {
-    float acc[1][NT][4];
+    float acc[1][NP][4];
     zero(acc);
-    if (n0 <= m0 + 15) mm(acc, RowA<LDK, PLK, N>(s.q), ColB<LDK, PLK, N>(s.k), m0, n0, 0, KP);
-    fade_scores<false, true>(acc, s.gates, m0, n0);
-    each_pair(acc, m0, n0, [&](int i, int j, float x, float y) { put<2, PLT>(s.p + i * LDT + j, x, y); });
+    if (p0 <= m0 + 15) mm(acc, RowA<LDK, PLK, N>(s.q), ColB<LDK, PLK, N>(s.k), m0, p0, 0, KP);
+    fade_scores<false, true>(acc, s.gates, m0, p0);
+    each_pair(acc, m0, p0, [&](int i, int j, float x, float y) { put<2, PLT>(s.p + i * LDT + j, x, y); });
   }
   const FragA<2, false> t_a(s.t);
-  const RowB<LDT, KP * LDT, 2> s_b(s.s);
-  const RowB<LDT, PLT, 2> x_b(s.x);
+  const RowB<LDX, KP * LDX, 2> s_b(s.s);
+  const RowB<LDX, PLX, 2> x_b(s.x);
   const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]};
   const float ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]};
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
   const TI* gv = (const TI*)a.v + vo;
   const bool even = a.V % 2 == 0 && (reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(o)) % 4 == 0;
-  for (int v0 = 0; v0 < a.V; v0 += 64) {
+  for (int v0 = 0; v0 < a.V; v0 += VB) {
     if (v0) {
       __syncthreads();  // readers of the previous panel are done
-      load_planes<LDT, KP, 64, NTH>(s.s, st + v0, VP);
+      load_planes<LDX, KP, VB, NTH>(s.s, st + v0, VP);
       cp_commit();
     }
     float xv[1][NT][4];
@@ -219,14 +221,14 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        put<2, PLT>(s.x + (i0 + 8 * r) * LDT + n0 + 8 * j + 2 * (lane & 3),
+        put<2, PLX>(s.x + (i0 + 8 * r) * LDX + n0 + 8 * j + 2 * (lane & 3),
                     be[r] * (xv[0][j][2 * r] - ee[r] * ak[0][j][2 * r]),
                     be[r] * (xv[0][j][2 * r + 1] - ee[r] * ak[0][j][2 * r + 1]));
     __syncthreads();
     zero(ak);
     mm(ak, t_a, x_b, m0, n0, 0, m0 + 16);  // U
     __syncthreads();
-    each_pair(ak, m0, n0, [&](int i, int n, float x, float y) { put<2, PLT>(s.x + i * LDT + n, x, y); });
+    each_pair(ak, m0, n0, [&](int i, int n, float x, float y) { put<2, PLX>(s.x + i * LDX + n, x, y); });
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(Out16<TI, KP>::NTH, Out16<TI, KP>::resident(si
 template <class TI, int KP, int NI>
 int prep(const Args& a, const Saved& sv, int VP, float* b, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Prep16<TI, KP, NI>);
-  cudaFuncSetAttribute(prep16_kernel<TI, KP, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<prep16_kernel<TI, KP, NI>>((int)smem);
   prep16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, (bf*)sv.tinv, sv.pm, b);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
@@ -268,7 +270,7 @@ int prep(const Args& a, const Saved& sv, int VP, float* b, int64_t items, cudaSt
 template <class TI, int KP>
 int output(const Args& a, const Saved& sv, int VP, bool exact, void* o, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Out16<TI, KP>);
-  cudaFuncSetAttribute(output16_kernel<TI, KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<output16_kernel<TI, KP>>((int)smem);
   output16_kernel<TI, KP><<<(unsigned)items, Out16<TI, KP>::NTH, smem, st>>>(
       a, sv.chunk_tab, VP, t_planes(exact), (const bf*)sv.tinv, (const bf*)sv.s, (TI*)o);
   SSLA_CHECK_LAUNCH("gated_delta_rule output");

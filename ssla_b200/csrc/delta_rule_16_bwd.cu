@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(Bwd16<TI, KP>::NTH, sizeof(Bwd16<TI, KP>) <= 1
 template <class TI, int KP, int NI>
 int adjoint(const Args& a, const Saved& sv, int VP, const void* dout, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Adj16<TI, KP, NI>);
-  cudaFuncSetAttribute(adjoint16_kernel<TI, KP, NI>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<adjoint16_kernel<TI, KP, NI>>((int)smem);
   adjoint16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, (const bf*)sv.tinv,
                                                                       (const TI*)dout, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule adjoint");
@@ -435,7 +435,7 @@ template <class TI, int KP>
 int backward(const Args& a, const Saved& sv, int VP, int tplanes, const bf* ds, const Grads& g, int64_t items,
              cudaStream_t st) {
   const size_t smem = sizeof(Bwd16<TI, KP>);
-  cudaFuncSetAttribute(backward16_kernel<TI, KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<backward16_kernel<TI, KP>>((int)smem);
   backward16_kernel<TI, KP><<<(unsigned)items, Bwd16<TI, KP>::NTH, smem, st>>>(
       a, sv.chunk_tab, VP, tplanes, (const bf*)sv.tinv, (const bf*)sv.s, ds, (const TI*)g.dout, (TI*)g.dq, (TI*)g.dk,
       (TI*)g.dv, g.dg, g.dbeta, g.dqk);

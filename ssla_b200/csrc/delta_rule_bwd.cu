@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict_
 template <int KP>
 int adjoint32(const Args& a, const Saved& sv, int VP, const void* dout, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(AdjSmem<KP>);
-  cudaFuncSetAttribute(adjoint_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<adjoint_kernel<KP>>((int)smem);
   adjoint_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, (const TI*)dout, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule adjoint");
   return SSLA_OK;
@@ -444,7 +444,7 @@ int adjoint32(const Args& a, const Saved& sv, int VP, const void* dout, float* i
 template <int KP>
 int backward32(const Args& a, const Saved& sv, int VP, const float* ds, const Grads& g, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(BwdSmem<KP>);
-  cudaFuncSetAttribute(backward_kernel<KP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  allow_smem<backward_kernel<KP>>((int)smem);
   backward_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.s, ds, (const TI*)g.dout,
                                                              (TI*)g.dq, (TI*)g.dk, (TI*)g.dv, g.dg, g.dbeta, g.dqk);
   SSLA_CHECK_LAUNCH("gated_delta_rule backward");

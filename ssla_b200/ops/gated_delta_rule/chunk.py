@@ -29,7 +29,7 @@ def norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, what):
             f"v {tuple(v.shape)}"
         )
     T, H, K = q.shape
-    HV, V = v.shape[1:]
+    _, HV, V = v.shape
     if H == 0 or HV == 0 or HV % H:
         raise ValueError(f"{what}: the {HV} value heads must be a positive multiple of the {H} key heads")
     if g.shape != (T, HV) or beta.shape != (T, HV):
@@ -42,7 +42,9 @@ def norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, what):
     for x in (k, v, g, beta, initial_state):
         if x is not None and x.device != dev:
             raise RuntimeError(f"{what}: all tensors must be on one device, got {dev} and {x.device}")
-    cu = prepare_cu_seqlens(cu_seqlens, dev)
+    cu = cu_seqlens
+    if cu is None or cu.dim() != 1 or cu.device != dev or cu.dtype != torch.int64 or not cu.is_contiguous() or not len(cu):
+        cu = prepare_cu_seqlens(cu_seqlens, dev)
     if initial_state is not None:
         N = cu.numel() - 1
         if initial_state.dim() == 0 or initial_state.shape[0] != N:
@@ -50,7 +52,7 @@ def norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, what):
                 f"The number of initial states is expected to be equal to the number of input sequences, "
                 f"i.e., {N} rather than {initial_state.shape[0] if initial_state.dim() else 0}."
             )
-        if initial_state.shape != (N, HV, K, V):
+        if tuple(initial_state.shape) != (N, HV, K, V):
             raise ValueError(f"{what}: initial_state must be [N, HV, K, V] = {(N, HV, K, V)}; got "
                              f"{tuple(initial_state.shape)}")
         initial_state = initial_state.float().contiguous()
@@ -67,10 +69,11 @@ def norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, what):
 
 def tensor_args(q, k, v, g, beta, cu, scale):
     """The arguments that every entry point of the family starts with."""
+    code = _lib._DT
     T, H, K = q.shape
-    HV, V = v.shape[1:]
-    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), _lib.dtype_code(q),
-            _lib.dtype_code(g), _lib.dtype_code(beta), cu.data_ptr(), cu.numel() - 1, T, H, HV, K, V, float(scale))
+    _, HV, V = v.shape
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), code[q.dtype], code[g.dtype],
+            code[beta.dtype], cu.data_ptr(), cu.shape[0] - 1, T, H, HV, K, V, scale)
 
 
 def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):

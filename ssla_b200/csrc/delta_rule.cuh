@@ -47,7 +47,7 @@ inline int t_planes(bool exact) { return exact ? 3 : 2; }
 
 // What the forward leaves for the backward (caller's `states` buffer), states padded to KP x VP:
 //   chunk_off [N+1] (device), chunk_tab [MC] {first token, rows | seq << 32}; per (chunk, value
-//   head) item: tinv: T, fp32 [64,64], or for 16-bit tokens planes of T and T^T in fragment order;
+//   head) item: tinv: T, fp32 [64,64], or for 16-bit tokens planes of it in fragment order;
 //   pm: the record of pm_bytes that a step of the chain copies; s [KP,VP] = state at the chunk's
 //   start, fp32, or for 16-bit tokens two bf16 planes.
 struct Saved {
@@ -70,8 +70,8 @@ inline size_t saved_layout(void* base, const Plan& p, int dtype, bool exact, int
   Saved s;
   s.chunk_off = (int*)take(4 * (N + 1));
   s.chunk_tab = (longlong2*)take(16 * (size_t)p.MC);
-  // fp32 [64][64], or t_planes of 10 + 10 blocks of 512 bytes
-  s.tinv = (float*)take((dtype == SSLA_F32 ? 4 * BT * BT : t_planes(exact) * 2 * 10 * 512) * items);
+  // fp32 [64][64], or t_planes of 10 blocks of 512 bytes
+  s.tinv = (float*)take((dtype == SSLA_F32 ? 4 * BT * BT : t_planes(exact) * 10 * 512) * items);
   s.pm = (unsigned char*)take(items * pm_bytes(KP, pm_planes(exact)));
   s.s = (float*)take(4 * items * KP * VP);
   if (out) *out = s;

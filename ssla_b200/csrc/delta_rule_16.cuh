@@ -65,9 +65,14 @@ template <int LD, int PLANE, int N> struct ColA {
   }
 };
 // The 10 blocks of a lower triangular [64, 64] matrix as left operand fragments: [plane][block][lane]
-// of 16 bytes, block (m, k) at m (m + 1) / 2 + k.  TR: fragments of the transpose, block (m, k) at
-// the place of (k, m).
+// of 16 bytes, block (m, k) at m (m + 1) / 2 + k.  TR: the transpose, its 8 x 8 pieces turned in
+// registers.
 constexpr int FRAGS = 10 * 32, FRAG_BYTES = FRAGS * 16, FRAG_ELEMS = FRAG_BYTES / 2;  // of a plane
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 template <int N, bool TR> struct FragA {
   static constexpr int n = N;
   const uint4* at;
@@ -75,7 +80,10 @@ template <int N, bool TR> struct FragA {
   __device__ __forceinline__ void load(uint32_t (&r)[4], int m, int k, int p) const {
     const int i = (TR ? k : m) >> 4, j = (TR ? m : k) >> 4;
     const uint4 x = at[p * FRAGS + (i * (i + 1) / 2 + j) * 32];
-    r[0] = x.x; r[1] = x.y; r[2] = x.z; r[3] = x.w;
+    r[0] = TR ? turned(x.x) : x.x;
+    r[1] = TR ? turned(x.z) : x.y;
+    r[2] = TR ? turned(x.y) : x.z;
+    r[3] = TR ? turned(x.w) : x.w;
   }
 };
 // Right operand, 16 x 16 blocks at (k, n).  RowB: stored [k][n].  ColB: stored [n][k].

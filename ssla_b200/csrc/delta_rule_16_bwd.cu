@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 10
   const size_t qk = ((size_t)t0 * a.H + h) * a.K;
   load_tokens<TI, LDK, KP, THREADS>(s.k, (const TI*)a.k + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
   load_tokens<TI, LDK, KP, THREADS>(s.q, (const TI*)a.q + qk, (size_t)a.H * a.K, rows, a.K, a.vec_k);
-  copy16<THREADS>(s.t, tinv + item * (2 * NI * FRAG_ELEMS), NI * FRAG_BYTES);
+  copy16<THREADS>(s.t, tinv + item * (NI * FRAG_ELEMS), NI * FRAG_BYTES);
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V;
   const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
   auto load_d = [&](int v0) {
@@ -118,7 +118,7 @@ template <class TI, int KP> struct Bwd16 {
   bf k[N * BT * LDK];
   bf q[N * BT * LDK];
   bf d[N * BT * LDX];
-  bf t[4 * FRAG_ELEMS];  // T, transpose of T
+  bf t[2 * FRAG_ELEMS];
   bf p[2 * BT * LDT];  // P, then dP
   bf x[2 * BT * LDX];  // beta X, then U;  x and f at last -beta E
   bf f[2 * BT * LDX];  // dU, then F
@@ -162,11 +162,9 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
   const bool even = a.V % 2 == 0 && (reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(dv)) % 4 == 0;
   const TI* gv = (const TI*)a.v + vo;
-  const bf* tf = tinv + item * (2 * (size_t)tplanes * FRAG_ELEMS);
-  copy16<NTH>(s.t, tf, 2 * FRAG_BYTES);
-  copy16<NTH>(s.t + 2 * FRAG_ELEMS, tf + (size_t)tplanes * FRAG_ELEMS, 2 * FRAG_BYTES);
+  copy16<NTH>(s.t, tinv + item * ((size_t)tplanes * FRAG_ELEMS), 2 * FRAG_BYTES);
   const FragA<2, false> t_a(s.t);
-  const FragA<2, true> tt_a(s.t + 2 * FRAG_ELEMS);
+  const FragA<2, true> tt_a(s.t);
   const bf* gs = states + item * (2 * KP * VP);
   const bf* ge = ds + item * (2 * KP * VP);
   const RowA<LDK, PLK, N> k_a(s.k), q_a(s.q);

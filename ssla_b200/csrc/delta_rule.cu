@@ -480,7 +480,7 @@ int check_args(const char* name, int dtype, int dtype_g, int dtype_b, int64_t N,
                  (long long)H);
   SSLA_CHECK_ARG(K >= 1 && V >= 1 && K <= 128 && V <= 256, "%s: K=%lld V=%lld not supported (1 <= K <= 128, 1 <= V <= 256)",
                  name, (long long)K, (long long)V);
-  SSLA_CHECK_ARG(N < (int64_t(1) << 31) && (max_chunks(N, T) + N) * (HV > 0 ? HV : 1) < (int64_t(1) << 26),
+  SSLA_CHECK_ARG(N < (int64_t(1) << 31) && (max_chunks(N, T) + N) * (HV > 0 ? HV : 1) < (int64_t(1) << 25),
                  "%s: too many chunks (%lld sequences, %lld tokens, %lld heads)", name, (long long)N, (long long)T,
                  (long long)HV);
   return SSLA_OK;

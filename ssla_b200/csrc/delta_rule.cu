@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
 // prep leaves PM in planes scaled by a power of two, and every warp scales its 16 rows of S by one
 // of its own before it shares them, so that 16 rows of the contraction have one scale, undone when
 // their MMA's result is added.  A step streams the chunk's record and its slice of B through a ring
-// of bulk copies (one thread issues them; the memory has the layout of shared memory), and has one
+// of bulk copies (a warp of its own issues them; the memory has the layout of shared memory), and has one
 // barrier.  A wait that gives up makes the rest of the chain NaN.
 // What bounds it: the dependent chain of a step (barrier, MMAs, rescaling).
 template <int KP, int VS, int NP> struct ChainSmem {
@@ -169,10 +169,10 @@ __device__ __forceinline__ void mma16h(float (&c)[4], const uint32_t (&a)[4], ui
 }
 
 template <int KP, int VS, bool TRANS, int NP>
-__global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
+__global__ void __launch_bounds__(KP * 2 + 32) chain_kernel(ChainArgs a) {
   using M = ChainSmem<KP, VS, NP>;
-  constexpr int NTH = KP * 2, NT = VS / 8, LDP = M::LDP, LDS = M::LDS, ST = M::stages, NB = KP / 16;
-  extern __shared__ __align__(128) unsigned char raw[];
+  constexpr int NT = VS / 8, LDP = M::LDP, LDS = M::LDS, ST = M::stages, NB = KP / 16;
+  extern __shared__ __align__(16) unsigned char raw[];
   uint64_t* const full = reinterpret_cast<uint64_t*>(raw + M::STATE);
   unsigned char* const ring = raw + M::STATE + 64;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, m0 = warp * 16;
@@ -181,21 +181,35 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
   const int list = (int)(lh / (unsigned)a.HV), hv = (int)(lh - (unsigned)list * a.HV);
   const int first = a.off[list], count = a.off[list + 1] - first;
   auto at = [&](int i) { return (size_t)(first + (a.reverse ? count - 1 - i : i)) * a.HV + hv; };
-  auto load = [&](int i) {  // thread 0
+  auto load = [&](int i) {  // one thread
     const size_t it = at(i);
     unsigned char* dst = ring + (i % ST) * M::STAGE;
     tc::mbar_arrive_expect_tx(full + i % ST, M::STAGE);
     bulk_load(dst, a.pm + it * M::PM, M::PM, full + i % ST);
     bulk_load(dst + M::PM, a.inc + it * KP * a.VP + (size_t)c0 * KP, M::B, full + i % ST);
   };
-  if (threadIdx.x == 0) {
+  const bool producer = warp == KP / 16;
+  if (producer && lane == 0) {
     for (int i = 0; i < ST; ++i) tc::mbar_init(full + i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     for (int i = 0; i < ST - 1 && i < count; ++i) load(i);
   }
   __syncthreads();
   bool good = true;
-  int bad_at = 0;
+  if (producer) {
+    int late = 0;  // copies under way when a wait gave up
+    for (int i = 0; i < count; ++i) {
+      if (good && !tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20)) {
+        good = false;
+        late = i;
+      }
+      __syncthreads();
+      if (lane == 0 && good && i + ST - 1 < count) load(i + ST - 1);
+    }
+    if (!good)  // let them end, within limits, before the block's memory goes
+      for (int i = late; i < late + ST - 1 && i < count; ++i) tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20);
+    return;
+  }
   float S[1][NT][4];
   each_pair(S, m0, 0, [&](int r, int c, float& x, float& y) {
     x = y = 0.f;
@@ -225,10 +239,7 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
     each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
       put_half<NP>(sc + r * LDS + c, KP * LDS, x * scale, y * scale);
     });
-    if (good && !tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20)) {
-      good = false;
-      bad_at = i;
-    }
+    good = good && tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20);
     __syncthreads();  // the state is there, step i - 1 is read
     const unsigned char* stage = ring + (i % ST) * M::STAGE;
     const float* ps = reinterpret_cast<const float*>(stage) + 1;
@@ -237,6 +248,16 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
     float acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    // products of 16 rows of the contraction; of a single column tile all of them stay open while the
+    // state is stored
+    float parts[NT == 1 ? NB : 1][NT][4];
+    auto join = [&](int kb) {
+      const float f = TRANS ? un[kb] : un[kb] * ps[kb / 4];
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(f, parts[NT == 1 ? kb : 0][j][r], acc[j][r]);
+    };
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
       uint32_t fa[NP][4];
@@ -267,20 +288,18 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
             fb[p][j + (NT > 1)][1] = r[3];
           }
       }
-      const float f = TRANS ? un[kb] : un[kb] * ps[kb / 4];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        float(&part)[4] = parts[NT == 1 ? kb : 0][j];
+        part[0] = part[1] = part[2] = part[3] = 0.f;
         if (NP > 1) {
           mma16h(part, fa[NP - 1], fb[0][j][0], fb[0][j][1]);
           mma16h(part, fa[0], fb[NP - 1][j][0], fb[NP - 1][j][1]);
         }
         mma16h(part, fa[0], fb[0][j][0], fb[0][j][1]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(f, part[r], acc[j][r]);
       }
+      if (NT > 1) join(kb);
     }
-    if (threadIdx.x == 0 && good && i + ST - 1 < count) load(i + ST - 1);
     if (a.s)
       each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
         if (a.planes)
@@ -288,6 +307,9 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
         else
           *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
       });
+    if (NT == 1)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) join(kb);
     const float* bc = reinterpret_cast<const float*>(stage + M::PM);
     const float f = TRANS ? ps[m0 / 64] : 1.f;
 #pragma unroll
@@ -300,8 +322,6 @@ __global__ void __launch_bounds__(KP * 2) chain_kernel(ChainArgs a) {
         y = fmaf(d, y, b.y - f * acc[j][2 * r + 1]);
       }
   }
-  if (!good && threadIdx.x == 0)  // let the copies under way end before the block's memory goes
-    for (int i = bad_at; i < bad_at + ST && i < count; ++i) tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20);
   if (a.last)
     each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
       const int cc = c0 + c;
@@ -318,7 +338,7 @@ template <int KP, int VS, bool TRANS, int NP> int launch_chain(const ChainArgs& 
   allow_smem<chain_kernel<KP, VS, TRANS, NP>>((int)smem);
   const int64_t grid = N * a.HV * a.slices;
   if (grid == 0) return SSLA_OK;
-  chain_kernel<KP, VS, TRANS, NP><<<(unsigned)grid, KP * 2, smem, st>>>(a);
+  chain_kernel<KP, VS, TRANS, NP><<<(unsigned)grid, KP * 2 + 32, smem, st>>>(a);
   SSLA_CHECK_LAUNCH("gated_delta_rule chain");
   return SSLA_OK;
 }

@@ -151,8 +151,7 @@ template <class TI, int KP> struct Out16 {
   bf q[N * BT * LDK];
   bf t[2 * FRAG_ELEMS];
   bf p[2 * BT * LDT];
-  bf s[2 * KP * LDX];
-  bf x[2 * BT * LDX];  // beta X, then U
+  bf s[2 * KP * LDX];  // S, then beta X, then U
   Gates gates;
   static constexpr int resident(size_t bytes) { return bytes <= 75 * 1024 ? 3 : bytes <= 113 * 1024 ? 2 : 1; }
 };
@@ -193,7 +192,8 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
   }
   const FragA<2, false> t_a(s.t);
   const RowB<LDX, KP * LDX, 2> s_b(s.s);
-  const RowB<LDX, PLX, 2> x_b(s.x);
+  bf* const sx = s.s;
+  const RowB<LDX, PLX, 2> x_b(sx);
   const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]};
   const float ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]};
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
@@ -214,18 +214,19 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
     zero(ak);
     mm(ak, RowA<LDK, PLK, N>(s.k), s_b, m0, n0, 0, KP);
     mm(aq, RowA<LDK, PLK, N>(s.q), s_b, m0, n0, 0, KP);
+    __syncthreads();  // S is read
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        put<2, PLX>(s.x + (i0 + 8 * r) * LDX + n0 + 8 * j + 2 * (lane & 3),
+        put<2, PLX>(sx + (i0 + 8 * r) * LDX + n0 + 8 * j + 2 * (lane & 3),
                     be[r] * (xv[0][j][2 * r] - ee[r] * ak[0][j][2 * r]),
                     be[r] * (xv[0][j][2 * r + 1] - ee[r] * ak[0][j][2 * r + 1]));
     __syncthreads();
     zero(ak);
     mm(ak, t_a, x_b, m0, n0, 0, m0 + 16);  // U
     __syncthreads();
-    each_pair(ak, m0, n0, [&](int i, int n, float x, float y) { put<2, PLX>(s.x + i * LDX + n, x, y); });
+    each_pair(ak, m0, n0, [&](int i, int n, float x, float y) { put<2, PLX>(sx + i * LDX + n, x, y); });
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll

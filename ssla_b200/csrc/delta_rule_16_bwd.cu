@@ -21,7 +21,7 @@ template <class TI, int KP, int NI> struct Adj16 {
 };
 
 template <class TI, int KP, int NI>
-__global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
+__global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 75 * 1024 ? 3 : sizeof(Adj16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
     adjoint16_kernel(Args a, const longlong2* __restrict__ tab, int VP, const bf* __restrict__ tinv,
                      const TI* __restrict__ dout, float* __restrict__ inc) {
   using S = Adj16<TI, KP, NI>;

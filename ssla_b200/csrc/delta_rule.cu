@@ -31,6 +31,8 @@ template <int KP>
 __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong2* __restrict__ tab, int VP,
                                                           float* __restrict__ tinv, unsigned char* __restrict__ pm,
                                                           float* __restrict__ inc) {
+  griddep_launch_dependents();
+  griddep_wait();
   using S = PrepSmem<KP>;
   constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDV = S::LDV;
@@ -170,6 +172,8 @@ __device__ __forceinline__ void mma16h(float (&c)[4], const uint32_t (&a)[4], ui
 
 template <int KP, int VS, bool TRANS, int NP>
 __global__ void __launch_bounds__(KP * 2 + 32) chain_kernel(ChainArgs a) {
+  griddep_launch_dependents();
+  griddep_wait();
   using M = ChainSmem<KP, VS, NP>;
   constexpr int NT = VS / 8, LDP = M::LDP, LDS = M::LDS, ST = M::stages, NB = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -338,7 +342,7 @@ template <int KP, int VS, bool TRANS, int NP> int launch_chain(const ChainArgs& 
   allow_smem<chain_kernel<KP, VS, TRANS, NP>>((int)smem);
   const int64_t grid = N * a.HV * a.slices;
   if (grid == 0) return SSLA_OK;
-  chain_kernel<KP, VS, TRANS, NP><<<(unsigned)grid, KP * 2 + 32, smem, st>>>(a);
+  launch_pdl(chain_kernel<KP, VS, TRANS, NP>, dim3((unsigned)grid), dim3(KP * 2 + 32), smem, st, a);
   SSLA_CHECK_LAUNCH("gated_delta_rule chain");
   return SSLA_OK;
 }
@@ -454,6 +458,8 @@ template <int KP, int VB>
 __global__ void __launch_bounds__(THREADS, 2) output_kernel(Args a, const longlong2* __restrict__ tab, int VP,
                                                             const float* __restrict__ tinv,
                                                             const float* __restrict__ states, TI* __restrict__ o) {
+  griddep_launch_dependents();
+  griddep_wait();
   output_chunk<KP, VB>(a, tab, VP, tinv, states, o);
   zero_uncovered(o, a, (int64_t)a.HV * a.V);
 }
@@ -462,7 +468,7 @@ template <int KP>
 int prep32(const Args& a, const Saved& sv, int VP, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(PrepSmem<KP>);
   allow_smem<prep_kernel<KP>>((int)smem);
-  prep_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.pm, inc);
+  launch_pdl(prep_kernel<KP>, dim3((unsigned)items), dim3(THREADS), smem, st, a, sv.chunk_tab, VP, sv.tinv, sv.pm, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
 }
@@ -472,7 +478,7 @@ int output32(const Args& a, const Saved& sv, int VP, void* o, int64_t items, cud
   constexpr int VB = KP == 64 ? 64 : 32;
   const size_t smem = sizeof(OutSmem<KP, VB>);
   allow_smem<output_kernel<KP, VB>>((int)smem);
-  output_kernel<KP, VB><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.s, (TI*)o);
+  launch_pdl(output_kernel<KP, VB>, dim3((unsigned)items), dim3(THREADS), smem, st, a, sv.chunk_tab, VP, sv.tinv, sv.s, (TI*)o);
   SSLA_CHECK_LAUNCH("gated_delta_rule output");
   return SSLA_OK;
 }

@@ -51,6 +51,8 @@ template <class TI, int KP, int NI>
 __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 1024 ? 3 : sizeof(Prep16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
     prep16_kernel(Args a, const longlong2* __restrict__ tab, int VP, bf* __restrict__ tinv, unsigned char* __restrict__ pm,
                   float* __restrict__ inc) {
+  griddep_launch_dependents();
+  griddep_wait();
   using S = Prep16<TI, KP, NI>;
   constexpr int N = S::NT, LDK = S::LDK, PLK = BT * LDK, PLT = BT * LDT;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -252,6 +254,8 @@ template <class TI, int KP>
 __global__ void __launch_bounds__(Out16<TI, KP>::NTH, Out16<TI, KP>::resident(sizeof(Out16<TI, KP>)))
     output16_kernel(Args a, const longlong2* __restrict__ tab, int VP, int tplanes, const bf* __restrict__ tinv,
                     const bf* __restrict__ states, TI* __restrict__ o) {
+  griddep_launch_dependents();
+  griddep_wait();
   output16_chunk<TI, KP>(a, tab, VP, tplanes, tinv, states, o);
   zero_uncovered(o, a, (int64_t)a.HV * a.V);
 }
@@ -260,7 +264,7 @@ template <class TI, int KP, int NI>
 int prep(const Args& a, const Saved& sv, int VP, float* b, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Prep16<TI, KP, NI>);
   allow_smem<prep16_kernel<TI, KP, NI>>((int)smem);
-  prep16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, (bf*)sv.tinv, sv.pm, b);
+  launch_pdl(prep16_kernel<TI, KP, NI>, dim3((unsigned)items), dim3(THREADS), smem, st, a, sv.chunk_tab, VP, (bf*)sv.tinv, sv.pm, b);
   SSLA_CHECK_LAUNCH("gated_delta_rule prep");
   return SSLA_OK;
 }
@@ -269,8 +273,7 @@ template <class TI, int KP>
 int output(const Args& a, const Saved& sv, int VP, bool exact, void* o, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Out16<TI, KP>);
   allow_smem<output16_kernel<TI, KP>>((int)smem);
-  output16_kernel<TI, KP><<<(unsigned)items, Out16<TI, KP>::NTH, smem, st>>>(
-      a, sv.chunk_tab, VP, t_planes(exact), (const bf*)sv.tinv, (const bf*)sv.s, (TI*)o);
+  launch_pdl(output16_kernel<TI, KP>, dim3((unsigned)items), dim3(Out16<TI, KP>::NTH), smem, st, a, sv.chunk_tab, VP, t_planes(exact), (const bf*)sv.tinv, (const bf*)sv.s, (TI*)o);
   SSLA_CHECK_LAUNCH("gated_delta_rule output");
   return SSLA_OK;
 }

@@ -24,6 +24,8 @@ template <class TI, int KP, int NI>
 __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 75 * 1024 ? 3 : sizeof(Adj16<TI, KP, NI>) <= 113 * 1024 ? 2 : 1)
     adjoint16_kernel(Args a, const longlong2* __restrict__ tab, int VP, const bf* __restrict__ tinv,
                      const TI* __restrict__ dout, float* __restrict__ inc) {
+  griddep_launch_dependents();
+  griddep_wait();
   using S = Adj16<TI, KP, NI>;
   constexpr int N = S::N, LDK = S::LDK, PLK = BT * LDK, PLT = BT * LDT, NK = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
@@ -415,6 +417,8 @@ __global__ void __launch_bounds__(Bwd16<TI, KP>::NTH, sizeof(Bwd16<TI, KP>) <= 1
                       const bf* __restrict__ states, const bf* __restrict__ ds, const TI* __restrict__ dout,
                       TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv, void* __restrict__ dg,
                       void* __restrict__ dbeta, float* __restrict__ dqk) {
+  griddep_launch_dependents();
+  griddep_wait();
   backward16_chunk<TI, KP>(a, tab, VP, tplanes, tinv, states, ds, dout, dq, dk, dv, dg, dbeta, dqk);
   zero_gradients(a, dq, dk, dv, dg, dbeta, dqk);
 }
@@ -423,7 +427,7 @@ template <class TI, int KP, int NI>
 int adjoint(const Args& a, const Saved& sv, int VP, const void* dout, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(Adj16<TI, KP, NI>);
   allow_smem<adjoint16_kernel<TI, KP, NI>>((int)smem);
-  adjoint16_kernel<TI, KP, NI><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, (const bf*)sv.tinv,
+  launch_pdl(adjoint16_kernel<TI, KP, NI>, dim3((unsigned)items), dim3(THREADS), smem, st, a, sv.chunk_tab, VP, (const bf*)sv.tinv,
                                                                       (const TI*)dout, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule adjoint");
   return SSLA_OK;
@@ -434,8 +438,7 @@ int backward(const Args& a, const Saved& sv, int VP, int tplanes, const bf* ds, 
              cudaStream_t st) {
   const size_t smem = sizeof(Bwd16<TI, KP>);
   allow_smem<backward16_kernel<TI, KP>>((int)smem);
-  backward16_kernel<TI, KP><<<(unsigned)items, Bwd16<TI, KP>::NTH, smem, st>>>(
-      a, sv.chunk_tab, VP, tplanes, (const bf*)sv.tinv, (const bf*)sv.s, ds, (const TI*)g.dout, (TI*)g.dq, (TI*)g.dk,
+  launch_pdl(backward16_kernel<TI, KP>, dim3((unsigned)items), dim3(Bwd16<TI, KP>::NTH), smem, st, a, sv.chunk_tab, VP, tplanes, (const bf*)sv.tinv, (const bf*)sv.s, ds, (const TI*)g.dout, (TI*)g.dq, (TI*)g.dk,
       (TI*)g.dv, g.dg, g.dbeta, g.dqk);
   SSLA_CHECK_LAUNCH("gated_delta_rule backward");
   return SSLA_OK;

@@ -34,6 +34,8 @@ template <int KP>
 __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2 : 1)
     adjoint_kernel(Args a, const longlong2* __restrict__ tab, int VP, const float* __restrict__ tinv,
                    const TI* __restrict__ dout, float* __restrict__ inc) {
+  griddep_launch_dependents();
+  griddep_wait();
   using S = AdjSmem<KP>;
   constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDW = S::LDW, LDO = S::LDO, NK = KP / 16;
@@ -399,6 +401,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<KP>) <= 113 * 1024 ? 2
                     const float* __restrict__ states, const float* __restrict__ ds, const TI* __restrict__ dout,
                     TI* __restrict__ dq, TI* __restrict__ dk, TI* __restrict__ dv, void* __restrict__ dg,
                     void* __restrict__ dbeta, float* __restrict__ dqk) {
+  griddep_launch_dependents();
+  griddep_wait();
   backward_chunk<KP>(a, tab, VP, tinv, states, ds, dout, dq, dk, dv, dg, dbeta, dqk);
   zero_gradients(a, dq, dk, dv, dg, dbeta, dqk);
 }
@@ -407,6 +411,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<KP>) <= 113 * 1024 ? 2
 template <class TO>
 __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ dqk, int64_t TH, int R, int K,
                                                         TO* __restrict__ dq, TO* __restrict__ dk) {
+  griddep_launch_dependents();
+  griddep_wait();
   const float* p = dqk + (blockIdx.y ? (size_t)TH * R * K : 0);
   TO* out = blockIdx.y ? dk : dq;
   const int lane = threadIdx.x & 31;
@@ -436,7 +442,7 @@ template <int KP>
 int adjoint32(const Args& a, const Saved& sv, int VP, const void* dout, float* inc, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(AdjSmem<KP>);
   allow_smem<adjoint_kernel<KP>>((int)smem);
-  adjoint_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, (const TI*)dout, inc);
+  launch_pdl(adjoint_kernel<KP>, dim3((unsigned)items), dim3(THREADS), smem, st, a, sv.chunk_tab, VP, sv.tinv, (const TI*)dout, inc);
   SSLA_CHECK_LAUNCH("gated_delta_rule adjoint");
   return SSLA_OK;
 }
@@ -445,7 +451,7 @@ template <int KP>
 int backward32(const Args& a, const Saved& sv, int VP, const float* ds, const Grads& g, int64_t items, cudaStream_t st) {
   const size_t smem = sizeof(BwdSmem<KP>);
   allow_smem<backward_kernel<KP>>((int)smem);
-  backward_kernel<KP><<<(unsigned)items, THREADS, smem, st>>>(a, sv.chunk_tab, VP, sv.tinv, sv.s, ds, (const TI*)g.dout,
+  launch_pdl(backward_kernel<KP>, dim3((unsigned)items), dim3(THREADS), smem, st, a, sv.chunk_tab, VP, sv.tinv, sv.s, ds, (const TI*)g.dout,
                                                              (TI*)g.dq, (TI*)g.dk, (TI*)g.dv, g.dg, g.dbeta, g.dqk);
   SSLA_CHECK_LAUNCH("gated_delta_rule backward");
   return SSLA_OK;
@@ -453,8 +459,7 @@ int backward32(const Args& a, const Saved& sv, int VP, const float* ds, const Gr
 
 template <class TO> int sum_heads(const Args& a, const Grads& g, cudaStream_t st) {
   const int64_t blocks = (a.T * a.H + 7) / 8;
-  sum_heads_kernel<TO><<<dim3((unsigned)(blocks < 16 * kNumSMs ? blocks : 16 * kNumSMs), 2), 256, 0, st>>>(
-      g.dqk, a.T * a.H, a.R, a.K, (TO*)g.dq, (TO*)g.dk);
+  launch_pdl(sum_heads_kernel<TO>, dim3((unsigned)(blocks < 16 * kNumSMs ? blocks : 16 * kNumSMs), 2), dim3(256), 0, st, g.dqk, a.T * a.H, a.R, a.K, (TO*)g.dq, (TO*)g.dk);
   SSLA_CHECK_LAUNCH("gated_delta_rule sum_heads");
   return SSLA_OK;
 }

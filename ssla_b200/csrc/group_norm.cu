@@ -84,6 +84,8 @@ template <class TI, int VEC, int NV>
 __global__ void __launch_bounds__(TH) token_fwd(const TI* __restrict__ x, int64_t T, int C, int G, TokMap m,
                                                 const float* __restrict__ w, const float* __restrict__ b, float eps,
                                                 int act, TI* __restrict__ y) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int Cg = C / G, slot = threadIdx.x / m.L, l = threadIdx.x % m.L;
   const int g = blockIdx.y * m.GB + slot % m.GB, tp = slot / m.GB;
   const bool live = tp < m.TP && g < G;
@@ -165,6 +167,8 @@ __global__ void __launch_bounds__(TH, tok_resident(VEC * NV)) token_bwd(const TI
                                                 int G, TokMap m, const float* __restrict__ w,
                                                 const float* __restrict__ b, float eps, int act, TI* __restrict__ dx,
                                                 float* __restrict__ part) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int Cg = C / G, slot = threadIdx.x / m.L, l = threadIdx.x % m.L;
   const int g = blockIdx.y * m.GB + slot % m.GB, tp = slot / m.GB;
   const bool live = tp < m.TP && g < G;
@@ -275,6 +279,8 @@ __global__ void __launch_bounds__(TH, tok_resident(VEC * NV)) token_bwd(const TI
 // out[c] = sum over rows of part[rows][C], blockIdx.y = 0: dw, 1: db
 __global__ void __launch_bounds__(1024) column_sums(const float* __restrict__ part, int64_t rows, int C,
                                                     float* __restrict__ dw, float* __restrict__ db) {
+  griddep_launch_dependents();
+  griddep_wait();
   __shared__ double sm[32][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + tx;
   const float* p = part + (blockIdx.y ? (size_t)rows * C : 0);
@@ -310,6 +316,8 @@ __device__ __forceinline__ bool chunk_at(const longlong2* tab, int64_t c, int64_
 template <class TI, int VEC>
 __global__ void __launch_bounds__(TH) pack_stats(const TI* __restrict__ x, int C, int G, PackMap m,
                                                  const longlong2* __restrict__ tab, double2* __restrict__ part) {
+  griddep_launch_dependents();
+  griddep_wait();
   __shared__ double2 sm[TH];
   int64_t t0, seq;
   int rows;
@@ -363,6 +371,8 @@ __device__ __forceinline__ int64_t seq_tokens(const int64_t* cu, int64_t n, int6
 __global__ void __launch_bounds__(TH) pack_moments(const double2* __restrict__ part, const int* __restrict__ off,
                                                    const int64_t* __restrict__ cu, int64_t N, int64_t T, int G, int Cg,
                                                    float eps, float2* __restrict__ stats) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int64_t id = (int64_t)blockIdx.x * (TH / 32) + (threadIdx.x >> 5);
   if (id >= N * G) return;
   const int64_t n = id / G;
@@ -402,6 +412,8 @@ __global__ void __launch_bounds__(TH) pack_fwd(const TI* __restrict__ x, int64_t
                                                const int64_t* __restrict__ cu, int64_t N,
                                                const float2* __restrict__ stats, const float* __restrict__ w,
                                                const float* __restrict__ b, int act, TI* __restrict__ y) {
+  griddep_launch_dependents();
+  griddep_wait();
   zero_rest(y, cu, N, T, C);
   int64_t t0, seq;
   int rows;
@@ -435,6 +447,8 @@ __global__ void __launch_bounds__(TH) pack_sums(const TI* __restrict__ x, const 
                                                 PackMap m, const longlong2* __restrict__ tab, int64_t MC,
                                                 const float2* __restrict__ stats, const float* __restrict__ w,
                                                 const float* __restrict__ b, int act, float* __restrict__ part) {
+  griddep_launch_dependents();
+  griddep_wait();
   __shared__ float sm[2][VEC][TH];
   int64_t t0, seq;
   int rows;
@@ -493,6 +507,8 @@ __global__ void __launch_bounds__(TH) pack_sums(const TI* __restrict__ x, const 
 // seq [2][N][C] = sums of part [2][MC][C] over the chunks of a sequence; 32 channels a block
 __global__ void __launch_bounds__(TH) pack_join(const float* __restrict__ part, int64_t MC, const int* __restrict__ off,
                                                 int64_t N, int C, float* __restrict__ seq) {
+  griddep_launch_dependents();
+  griddep_wait();
   __shared__ double sm[2][TH / 32][32];
   const int64_t n = blockIdx.x;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.y * 32 + tx;
@@ -520,6 +536,8 @@ __global__ void __launch_bounds__(TH) pack_join(const float* __restrict__ part, 
 __global__ void __launch_bounds__(TH) pack_means(const float* __restrict__ seq, const int64_t* __restrict__ cu,
                                                  int64_t N, int64_t T, int C, int G, const float* __restrict__ w,
                                                  float2* __restrict__ means) {
+  griddep_launch_dependents();
+  griddep_wait();
   const int64_t id = (int64_t)blockIdx.x * (TH / 32) + (threadIdx.x >> 5);
   if (id >= N * G) return;
   const int64_t n = id / G;
@@ -548,6 +566,8 @@ __global__ void __launch_bounds__(TH) pack_bwd(const TI* __restrict__ x, const T
                                                const float2* __restrict__ stats, const float2* __restrict__ means,
                                                const float* __restrict__ w, const float* __restrict__ b, int act,
                                                TI* __restrict__ dx) {
+  griddep_launch_dependents();
+  griddep_wait();
   zero_rest(dx, cu, N, T, C);
   int64_t t0, seq;
   int rows;
@@ -725,16 +745,15 @@ struct Call {
 template <class TI, int VEC, int NV> int token_call(const Call& c, const TokMap& m, cudaStream_t st) {
   const int gy = (c.G + m.GB - 1) / m.GB;
   if (!c.dy) {
-    token_fwd<TI, VEC, NV><<<dim3(tok_blocks(c.T, gy, m.TP, 32), gy), TH, 0, st>>>(
-        (const TI*)c.x, c.T, c.C, c.G, m, c.w, c.b, c.eps, c.act, (TI*)c.y);
+    launch_pdl(token_fwd<TI, VEC, NV>, dim3(tok_blocks(c.T, gy, m.TP, 32), gy), dim3(TH), 0, st, (const TI*)c.x, c.T, c.C, c.G, m, c.w, c.b, c.eps, c.act, (TI*)c.y);
     SSLA_CHECK_LAUNCH("group_norm forward");
     return SSLA_OK;
   }
   const int gx = tok_blocks(c.T, gy, m.TP, tok_resident(VEC * NV));  // one wave: the sums stay in registers
-  token_bwd<TI, VEC, NV><<<dim3(gx, gy), TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.T, c.C, c.G, m, c.w, c.b, c.eps,
+  launch_pdl(token_bwd<TI, VEC, NV>, dim3(gx, gy), dim3(TH), 0, st, (const TI*)c.x, (const TI*)c.dy, c.T, c.C, c.G, m, c.w, c.b, c.eps,
                                                       c.act, (TI*)c.y, (float*)c.ws);
   SSLA_CHECK_LAUNCH("group_norm backward");
-  column_sums<<<dim3((c.C + 31) / 32, 2), 1024, 0, st>>>((const float*)c.ws, (int64_t)gx * m.TP, c.C, c.dw, c.db);
+  launch_pdl(column_sums, dim3((c.C + 31) / 32, 2), dim3(1024), 0, st, (const float*)c.ws, (int64_t)gx * m.TP, c.C, c.dw, c.db);
   SSLA_CHECK_LAUNCH("group_norm column sums");
   return SSLA_OK;
 }
@@ -768,36 +787,36 @@ template <class TI, int VEC> int pack_call(const Call& c, cudaStream_t st) {
     int rc = launch_pack_tables(c.cu, c.N, c.T, m.R, MC, sv.off, sv.tab, st);
     if (rc) return rc;
     if (MC > 0) {
-      pack_stats<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, c.C, c.G, m, sv.tab, w.part);
+      launch_pdl(pack_stats<TI, VEC>, grid, dim3(TH), 0, st, (const TI*)c.x, c.C, c.G, m, sv.tab, w.part);
       SSLA_CHECK_LAUNCH("group_norm statistics");
     }
     if (ngrid) {
-      pack_moments<<<ngrid, TH, 0, st>>>(w.part, sv.off, c.cu, c.N, c.T, c.G, c.C / c.G, c.eps, sv.stats);
+      launch_pdl(pack_moments, dim3(ngrid), dim3(TH), 0, st, w.part, sv.off, c.cu, c.N, c.T, c.G, c.C / c.G, c.eps, sv.stats);
       SSLA_CHECK_LAUNCH("group_norm moments");
     }
     if (c.T == 0) return SSLA_OK;
-    pack_fwd<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, c.T, c.C, c.G, m, sv.tab, MC, c.cu, c.N, sv.stats, c.w, c.b,
+    launch_pdl(pack_fwd<TI, VEC>, grid, dim3(TH), 0, st, (const TI*)c.x, c.T, c.C, c.G, m, sv.tab, MC, c.cu, c.N, sv.stats, c.w, c.b,
                                            c.act, (TI*)c.y);
     SSLA_CHECK_LAUNCH("group_norm forward");
     return SSLA_OK;
   }
   if (MC > 0) {
-    pack_sums<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.C, c.G, m, sv.tab, MC, sv.stats, c.w, c.b,
+    launch_pdl(pack_sums<TI, VEC>, grid, dim3(TH), 0, st, (const TI*)c.x, (const TI*)c.dy, c.C, c.G, m, sv.tab, MC, sv.stats, c.w, c.b,
                                             c.act, w.sums);
     SSLA_CHECK_LAUNCH("group_norm sums");
   }
   if (c.N > 0) {
-    pack_join<<<dim3((unsigned)c.N, (c.C + 31) / 32), TH, 0, st>>>(w.sums, MC, sv.off, c.N, c.C, w.seq);
+    launch_pdl(pack_join, dim3((unsigned)c.N, (c.C + 31) / 32), dim3(TH), 0, st, w.sums, MC, sv.off, c.N, c.C, w.seq);
     SSLA_CHECK_LAUNCH("group_norm join");
   }
-  column_sums<<<dim3((c.C + 31) / 32, 2), 1024, 0, st>>>(w.seq, c.N, c.C, c.dw, c.db);
+  launch_pdl(column_sums, dim3((c.C + 31) / 32, 2), dim3(1024), 0, st, w.seq, c.N, c.C, c.dw, c.db);
   SSLA_CHECK_LAUNCH("group_norm column sums");
   if (ngrid) {
-    pack_means<<<ngrid, TH, 0, st>>>(w.seq, c.cu, c.N, c.T, c.C, c.G, c.w, w.means);
+    launch_pdl(pack_means, dim3(ngrid), dim3(TH), 0, st, w.seq, c.cu, c.N, c.T, c.C, c.G, c.w, w.means);
     SSLA_CHECK_LAUNCH("group_norm means");
   }
   if (c.T == 0) return SSLA_OK;
-  pack_bwd<TI, VEC><<<grid, TH, 0, st>>>((const TI*)c.x, (const TI*)c.dy, c.T, c.C, c.G, m, sv.tab, MC, c.cu, c.N,
+  launch_pdl(pack_bwd<TI, VEC>, grid, dim3(TH), 0, st, (const TI*)c.x, (const TI*)c.dy, c.T, c.C, c.G, m, sv.tab, MC, c.cu, c.N,
                                          sv.stats, w.means, c.w, c.b, c.act, (TI*)c.y);
   SSLA_CHECK_LAUNCH("group_norm backward");
   return SSLA_OK;

@@ -9,6 +9,8 @@ __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { 
 
 __global__ void __launch_bounds__(1024) tables_kernel(const int64_t* __restrict__ cu, int64_t N, int64_t T, int R,
                                                       int64_t MC, int* chunk_off, longlong2* chunk_tab) {
+  griddep_launch_dependents();
+  griddep_wait();
   constexpr int KEPT = 1024;  // bounds of this many sequences stay in shared memory
   __shared__ int part[32], run, kept_off[KEPT + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -77,7 +79,7 @@ __global__ void __launch_bounds__(1024) tables_kernel(const int64_t* __restrict_
 
 int launch_pack_tables(const int64_t* cu, int64_t N, int64_t T, int rows, int64_t MC, int* chunk_off,
                        longlong2* chunk_tab, cudaStream_t st) {
-  tables_kernel<<<1, 1024, 0, st>>>(cu, N, T, rows, MC, chunk_off, chunk_tab);
+  launch_pdl(tables_kernel, dim3(1), dim3(1024), 0, st, cu, N, T, rows, MC, chunk_off, chunk_tab);
   SSLA_CHECK_LAUNCH("chunk tables");
   return SSLA_OK;
 }

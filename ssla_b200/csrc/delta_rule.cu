@@ -1,8 +1,10 @@
 // Chunked gated delta rule, forward (delta_rule.cuh has the formulas).
-//   tables      chunk and segment lists of the packed sequences (device only, no host read)
+//   tables      chunk list of the packed sequences (pack_tables.cu; device only, no host read)
 //   prep        per (chunk, value head): T, PM = Kl^T W, B = Kl^T T beta V, exp(gC)
 //   chain       S' = exp(gC) S - PM S + B along every sequence: the one sequential part
 //   output      per (chunk, value head): O from the start state
+// The prep and output kernels here are those of fp32 tokens (split TF32 products); the chain serves
+// every type.
 #include "delta_rule_16.cuh"
 #include "delta_rule_inverse.cuh"
 #include "pack_tables.cuh"
@@ -34,7 +36,6 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
   griddep_launch_dependents();
   griddep_wait();
   using S = PrepSmem<KP>;
-  constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDV = S::LDV;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -63,7 +64,7 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
     float acc[1][4][4];
     zero(acc);
     if (n0 <= m0)
-      warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sk + m * LDK + k); },
+      warp_mma(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sk + m * LDK + k); },
                          [&](int k, int n) { return pair(sk + n * LDK + k); });
     fade_scores<true, false>(acc, s.gates, m0, n0);
     const int i0 = m0 + ((threadIdx.x & 31) >> 2);
@@ -100,12 +101,12 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
         return make_float2(x.x * c.x, x.y * c.y);
       };
       if (w)
-        warp_mma<false, X, SP>(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return column<LDK>(sk + j * LDK + c0 + n); });
+        warp_mma(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return column<LDK>(sk + j * LDK + c0 + n); });
       else
-        warp_mma<false, X, SP>(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return column<LDV>(s.v + j * LDV + n); });
+        warp_mma(acc, m0, n0, 0, m0 + 16, fa, [&](int j, int n) { return column<LDV>(s.v + j * LDV + n); });
       each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
         const float l = s.gates.left[i];
-        *reinterpret_cast<float2*>(s.y + i * 68 + j) = stage2<SP>(x * l, y * l);
+        *reinterpret_cast<float2*>(s.y + i * 68 + j) = make_float2(x * l, y * l);
       });
     }
     __syncthreads();
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
       float acc[MT][4][4];
       zero(acc);
       const int mk = (warp >> 1) * 16 * MT;
-      warp_mma<X, !SP, SP>(acc, mk, n0, 0, BT, [&](int m, int j) { return column<LDK>(sk + j * LDK + m); },
+      warp_mma(acc, mk, n0, 0, BT, [&](int m, int j) { return column<LDK>(sk + j * LDK + m); },
                            [&](int j, int n) { return column<68>(s.y + j * 68 + n); });
       if (w)
         store_pm<KP, 2>(acc, mk, c0, n0, s.red, record);
@@ -135,7 +136,10 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
 // their MMA's result is added.  A step streams the chunk's record and its slice of B through a ring
 // of bulk copies (a warp of its own issues them; the memory has the layout of shared memory), and has one
 // barrier.  A wait that gives up makes the rest of the chain NaN.
-// What bounds it: the dependent chain of a step (barrier, MMAs, rescaling).
+// What bounds it: the dependent chain of a step (barrier, MMAs, rescaling), 0.6 us for 64 x 64; for
+// 128 x 128 at fp32 accuracy the 74 KB a step from L2, 1.0 us with 8 columns on 128 SMs.  (Two CTAs that
+// share a state over distributed shared memory halve those bytes, but the cluster barrier took a step
+// to 1.7 us; two buffers instead of three, 2.0 us.)
 template <int KP, int VS, int NP> struct ChainSmem {
   static constexpr int LDP = KP + 8, LDS = VS == 8 ? 8 : VS + 8;  // ldmatrix without conflicts
   static constexpr int PM = pm_bytes(KP, NP), B = 4 * KP * VS, STAGE = PM + B;  // bytes
@@ -376,7 +380,6 @@ __device__ __forceinline__ void output_chunk(const Args& a, const longlong2* __r
                                              const float* __restrict__ tinv, const float* __restrict__ states,
                                              TI* __restrict__ o) {
   using S = OutSmem<KP, VB>;
-  constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDV = S::LDV, LDX = S::LDX, NT = VB / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -409,7 +412,7 @@ __device__ __forceinline__ void output_chunk(const Args& a, const longlong2* __r
       float acc[1][4][4];
       zero(acc);
       if (p0 <= m0)
-        warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
+        warp_mma(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
                            [&](int k, int n) { return pair(sk + n * LDK + k); });
       fade_scores<false, false>(acc, s.gates, m0, p0);
       each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
@@ -422,27 +425,27 @@ __device__ __forceinline__ void output_chunk(const Args& a, const longlong2* __r
     zero(aq);
     zero(ak);
     auto fs = [&](int k, int n) { return column<LDX>(s.s + k * LDX + n); };
-    warp_mma<X, !SP, SP>(ak, m0, n0, 0, KP, [&](int m, int k) { return pair(sk + m * LDK + k); }, fs);
-    warp_mma<X, !SP, SP>(aq, m0, n0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); }, fs);
+    warp_mma(ak, m0, n0, 0, KP, [&](int m, int k) { return pair(sk + m * LDK + k); }, fs);
+    warp_mma(aq, m0, n0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); }, fs);
     each_pair(ak, m0, n0, [&](int i, int n, float x, float y) {
       const float b = s.gates.beta[i], e = s.gates.start[i];
       *reinterpret_cast<float2*>(s.x + i * LDX + n) =
-          stage2<SP>(b * (ldf(s.v + i * LDV + n) - e * x), b * (ldf(s.v + i * LDV + n + 1) - e * y));
+          make_float2(b * (ldf(s.v + i * LDV + n) - e * x), b * (ldf(s.v + i * LDV + n + 1) - e * y));
     });
     __syncthreads();
     zero(ak);
     auto fx = [&](int k, int n) { return column<LDX>(s.x + k * LDX + n); };
-    warp_mma<false, !SP, SP>(ak, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDC + k); }, fx);
+    warp_mma(ak, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDC + k); }, fx);
     __syncthreads();
     each_pair(ak, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.x + i * LDX + n) = stage2<SP>(x, y);
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(x, y);
     });
     each_pair(aq, m0, n0, [&](int i, int, float& x, float& y) {
       x *= s.gates.start[i];
       y *= s.gates.start[i];
     });
     __syncthreads();
-    warp_mma<!SP, !SP, SP>(aq, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.p + m * LDC + k); }, fx);
+    warp_mma(aq, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.p + m * LDC + k); }, fx);
     each_pair(aq, m0, n0, [&](int i, int n, float x, float y) {
       const int c = v0 + n;
       if (i < rows) {

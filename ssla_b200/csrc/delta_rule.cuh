@@ -126,39 +126,17 @@ __device__ __forceinline__ void st_any(void* p, int dt, size_t i, float x) {
   else ((__half*)p)[i] = __float2half_rn(x);
 }
 
-// ------------------------------------------------------------------ tensor-core products
-// Warp-level C += A B on mma.sync m16n8k8 TF32 with fp32 accumulators.  Operands come from shared
-// memory through functors that return a pair along the contraction, fa(row, k) = {A[row][k],
-// A[row][k+1]}, fb(k, col) likewise: the order of k inside an MMA is free as long as both agree, so
-// lane t takes k = 2t, 2t + 1 of every 8, one 64-bit (16-bit tiles: 32-bit) load for tiles that are
-// contiguous in k.
-//
-// AX, BX: the operand is exact in TF32 (a value of a 16-bit input, or rounded when it was stored).
-// SPLIT: x = hi + lo with hi the TF32 rounding, hi hi + lo hi + hi lo, about 2^-22 relative; the
-// small products have accumulators of their own, which also shortens the chain of additions that
-// the tensor core truncates.  Without SPLIT one product of TF32-rounded operands.
-__device__ __forceinline__ float tf32(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return __uint_as_float(r);
-}
-// what a tile stores for later products: fp32 for split ones, else the TF32 rounding
-template <bool SPLIT> __device__ __forceinline__ float stage(float x) { return SPLIT ? x : tf32(x); }
-template <bool SPLIT> __device__ __forceinline__ float2 stage2(float x, float y) {
-  return make_float2(stage<SPLIT>(x), stage<SPLIT>(y));
-}
-
-template <bool EXACT, bool SPLIT>
+// ------------------------------------------------------------------ products of fp32 tiles
+// Warp-level C += A B on mma.sync m16n8k8 TF32 with fp32 accumulators, for fp32 tokens.  Operands come
+// from shared memory through functors that return a pair along the contraction, fa(row, k) =
+// {A[row][k], A[row][k+1]}, fb(k, col) likewise: the order of k inside an MMA is free as long as both
+// agree, so lane t takes k = 2t, 2t + 1 of every 8, one 64-bit load for tiles that are contiguous in k.
+// x = hi + lo with hi the TF32 rounding, products hi hi + lo hi + hi lo, about 2^-22 relative; the
+// small products have accumulators of their own, which also shortens the chain of additions that the
+// tensor core truncates.  An infinity or NaN leaves lo NaN, so it is not lost.
 __device__ __forceinline__ void operand(float x, uint32_t& hi, uint32_t& lo) {
-  if (EXACT) {
-    hi = __float_as_uint(x);
-  } else if (SPLIT) {
-    // round to nearest by hand, ties away: a NaN or infinity leaves lo NaN, so it is not lost
-    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-    lo = __float_as_uint(x - __uint_as_float(hi));
-  } else {
-    hi = __float_as_uint(tf32(x));
-  }
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;  // nearest, ties away
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
 __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
@@ -168,48 +146,45 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], cons
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-template <bool AX, bool BX, bool SPLIT, int UNROLL = 2, int MT, int NT, class FA, class FB>
+template <int MT, int NT, class FA, class FB>
 __device__ __forceinline__ void warp_mma(float (&acc)[MT][NT][4], int m0, int n0, int k0, int k1, FA fa, FB fb) {
-  constexpr bool SMALL = SPLIT && !(AX && BX);
   const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
-  float small[SMALL ? MT : 1][SMALL ? NT : 1][4];
-  if (SMALL)
+  float small[MT][NT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) small[i][j][0] = small[i][j][1] = small[i][j][2] = small[i][j][3] = 0.f;
-#pragma unroll UNROLL
+    for (int j = 0; j < NT; ++j) small[i][j][0] = small[i][j][1] = small[i][j][2] = small[i][j][3] = 0.f;
+#pragma unroll 2
   for (int k = k0; k < k1; k += 8) {
     uint32_t ah[MT][4], al[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const float2 x = fa(m0 + 16 * i + g, k + 2 * t), y = fa(m0 + 16 * i + g + 8, k + 2 * t);
-      operand<AX, SPLIT>(x.x, ah[i][0], al[i][0]);
-      operand<AX, SPLIT>(y.x, ah[i][1], al[i][1]);
-      operand<AX, SPLIT>(x.y, ah[i][2], al[i][2]);
-      operand<AX, SPLIT>(y.y, ah[i][3], al[i][3]);
+      operand(x.x, ah[i][0], al[i][0]);
+      operand(y.x, ah[i][1], al[i][1]);
+      operand(x.y, ah[i][2], al[i][2]);
+      operand(y.y, ah[i][3], al[i][3]);
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       uint32_t bh[2], bl[2];
       const float2 z = fb(k + 2 * t, n0 + 8 * j + g);
-      operand<BX, SPLIT>(z.x, bh[0], bl[0]);
-      operand<BX, SPLIT>(z.y, bh[1], bl[1]);
+      operand(z.x, bh[0], bl[0]);
+      operand(z.y, bh[1], bl[1]);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         mma8(acc[i][j], ah[i], bh);
-        if (SPLIT && !AX) mma8(small[i][j], al[i], bh);
-        if (SPLIT && !BX) mma8(small[i][j], ah[i], bl);
+        mma8(small[i][j], al[i], bh);
+        mma8(small[i][j], ah[i], bl);
       }
     }
   }
-  if (SMALL)
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] += small[i][j][r];
+      for (int r = 0; r < 4; ++r) acc[i][j][r] += small[i][j][r];
 }
 
 // pairs along a row of a tile (contiguous), and along a column
@@ -218,7 +193,7 @@ __device__ __forceinline__ float2 pair(const __nv_bfloat16* p) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
 }
 __device__ __forceinline__ float2 pair(const __half* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
-template <int LD, class T> __device__ __forceinline__ float2 column(const T* p) { return make_float2(ldf(p), ldf(p + LD)); }
+template <int LD> __device__ __forceinline__ float2 column(const float* p) { return make_float2(p[0], p[LD]); }
 
 template <int MT, int NT> __device__ __forceinline__ void zero(float (&acc)[MT][NT][4]) {
 #pragma unroll

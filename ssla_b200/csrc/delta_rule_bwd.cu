@@ -1,4 +1,5 @@
-// Chunked gated delta rule, backward.  With P = G o Q K^T (lower), S the state at a chunk's start,
+// Chunked gated delta rule, backward (the kernels here: fp32 tokens; 16-bit ones: delta_rule_16_bwd.cu).
+// With P = G o Q K^T (lower), S the state at a chunk's start,
 // D the adjoint of the state at its end, X = V - exp(gc) K S, U = T beta X:
 //   adjoint of the chunk map   dB = scale qh^T dO,  qh = exp(gc) Q - P W,  W = T beta exp(gc) K
 //   dU = scale P^T dO + Kl D;  F = T^T dU;  dV = beta F
@@ -37,7 +38,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2
   griddep_launch_dependents();
   griddep_wait();
   using S = AdjSmem<KP>;
-  constexpr bool X = false, SP = true;
   constexpr int LDK = S::LDK, LDW = S::LDW, LDO = S::LDO, NK = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2
     float acc[1][4][4];
     zero(acc);
     if (n0 <= m0)
-      warp_mma<X, X, SP>(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
+      warp_mma(acc, m0, n0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
                          [&](int k, int n) { return pair(sk + n * LDK + k); });
     fade_scores<false, false>(acc, s.gates, m0, n0);
     each_pair(acc, m0, n0, [&](int i, int j, float x, float y) {
@@ -74,24 +74,24 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2
   }
   float acc[1][NK][4];
   zero(acc);
-  warp_mma<false, X, SP>(acc, m0, k0, 0, m0 + 16,
+  warp_mma(acc, m0, k0, 0, m0 + 16,
                          [&](int i, int j) {
                            const float2 x = pair(s.t + i * LDC + j), b = pair(s.gates.beta + j), e = pair(s.gates.start + j);
                            return make_float2(x.x * (b.x * e.x), x.y * (b.y * e.y));
                          },
                          [&](int j, int n) { return column<LDK>(sk + j * LDK + n); });
   each_pair(acc, m0, k0, [&](int i, int n, float x, float y) {
-    *reinterpret_cast<float2*>(s.w + i * LDW + n) = stage2<SP>(x, y);
+    *reinterpret_cast<float2*>(s.w + i * LDW + n) = make_float2(x, y);
   });
   __syncthreads();
   zero(acc);
-  warp_mma<!SP, !SP, SP>(acc, m0, k0, 0, m0 + 16, [&](int i, int j) { return pair(s.p + i * LDC + j); },
+  warp_mma(acc, m0, k0, 0, m0 + 16, [&](int i, int j) { return pair(s.p + i * LDC + j); },
                          [&](int j, int n) { return column<LDW>(s.w + j * LDW + n); });
   __syncthreads();
   each_pair(acc, m0, k0, [&](int i, int n, float x, float y) {
     const float e = s.gates.start[i];
     *reinterpret_cast<float2*>(s.w + i * LDW + n) =
-        stage2<SP>(a.scale * (e * ldf(sq + i * LDK + n) - x), a.scale * (e * ldf(sq + i * LDK + n + 1) - y));
+        make_float2(a.scale * (e * ldf(sq + i * LDK + n) - x), a.scale * (e * ldf(sq + i * LDK + n + 1) - y));
   });
   constexpr int MT = KP / 64;
   const int mk = (warp >> 1) * 16 * MT;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(AdjSmem<KP>) <= 113 * 1024 ? 2
     __syncthreads();
     float db[MT][4][4];
     zero(db);
-    warp_mma<!SP, X, SP>(db, mk, n0, 0, BT, [&](int m, int j) { return column<LDW>(s.w + j * LDW + m); },
+    warp_mma(db, mk, n0, 0, BT, [&](int m, int j) { return column<LDW>(s.w + j * LDW + m); },
                          [&](int j, int n) { return column<LDO>(s.d + j * LDO + n); });
     each_pair(db, mk, n0, [&](int m, int n, float x, float y) {
       *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, v0 + n)) = make_float2(x, y);
@@ -138,7 +138,6 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
                                                void* __restrict__ dg, void* __restrict__ dbeta,
                                                float* __restrict__ dqk) {
   using S = BwdSmem<KP>;
-  constexpr bool X = false, SP = true;
   constexpr int VB = S::VB, LDK = S::LDK, LDO = S::LDO, LDX = S::LDX, LDS = S::LDS, LDP = S::LDP, NT = VB / 16, NK = KP / 16;
   extern __shared__ __align__(16) unsigned char raw[];
   S& s = *reinterpret_cast<S*>(raw);
@@ -182,7 +181,7 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
       float acc[1][4][4];
       zero(acc);
       if (low)
-        warp_mma<X, X, SP>(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
+        warp_mma(acc, m0, p0, 0, KP, [&](int m, int k) { return pair(sq + m * LDK + k); },
                            [&](int k, int n) { return pair(sk + n * LDK + k); });
       fade_scores<false, false>(acc, s.gates, m0, p0);
       each_pair(acc, m0, p0, [&](int i, int j, float x, float y) {
@@ -200,8 +199,8 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
     float ks[1][NT][4], du[1][NT][4];
     zero(ks);
     zero(du);
-    warp_mma<X, !SP, SP>(ks, m0, n0, 0, KP, fk_row, [&](int k, int n) { return column<LDS>(s.s + k * LDS + n); });
-    warp_mma<X, !SP, SP>(du, m0, n0, 0, KP, fk_row, [&](int k, int n) { return column<LDS>(s.e + k * LDS + n); });
+    warp_mma(ks, m0, n0, 0, KP, fk_row, [&](int k, int n) { return column<LDS>(s.s + k * LDS + n); });
+    warp_mma(du, m0, n0, 0, KP, fk_row, [&](int k, int n) { return column<LDS>(s.e + k * LDS + n); });
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -212,7 +211,7 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
       }
     each_pair(xv, m0, n0, [&](int i, int n, float x, float y) {
       const float b = s.gates.beta[i];
-      *reinterpret_cast<float2*>(s.x + i * LDX + n) = stage2<SP>(b * x, b * y);
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(b * x, b * y);
     });
     for (int i = tid; i < KP * (VB / 4); i += THREADS) {
       const int r = i / (VB / 4), c = (i % (VB / 4)) * 4;
@@ -222,11 +221,11 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
     }
     __syncthreads();
     zero(ks);
-    warp_mma<false, !SP, SP>(ks, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDP + k); }, fx);  // U
+    warp_mma(ks, m0, n0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDP + k); }, fx);  // U
     {
       float pd[1][NT][4];
       zero(pd);
-      warp_mma<!SP, X, SP>(pd, m0, n0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
+      warp_mma(pd, m0, n0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
                            [&](int k, int n) { return column<LDO>(sd + k * LDO + n); });
 #pragma unroll
       for (int j = 0; j < NT; ++j)
@@ -235,14 +234,14 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
     }
     __syncthreads();
     each_pair(ks, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.x + i * LDX + n) = stage2<SP>(x, y);
+      *reinterpret_cast<float2*>(s.x + i * LDX + n) = make_float2(x, y);
     });
     each_pair(du, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.f + i * LDX + n) = stage2<SP>(x, y);
+      *reinterpret_cast<float2*>(s.f + i * LDX + n) = make_float2(x, y);
     });
     __syncthreads();
     zero(du);
-    warp_mma<false, !SP, SP>(du, m0, n0, m0, BT, [&](int m, int k) { return column<LDP>(s.t + k * LDP + m); },
+    warp_mma(du, m0, n0, m0, BT, [&](int m, int k) { return column<LDP>(s.t + k * LDP + m); },
                              [&](int k, int n) { return column<LDX>(s.f + k * LDX + n); });  // F
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -260,7 +259,7 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
     });
     __syncthreads();
     each_pair(du, m0, n0, [&](int i, int n, float x, float y) {
-      *reinterpret_cast<float2*>(s.f + i * LDX + n) = stage2<SP>(x, y);
+      *reinterpret_cast<float2*>(s.f + i * LDX + n) = make_float2(x, y);
     });
     __syncthreads();
     auto ff = [&](int m, int k) { return pair(s.f + m * LDX + k); };
@@ -268,12 +267,12 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
     auto fu_t = [&](int k, int n) { return pair(s.x + n * LDX + k); };
     auto fs_t = [&](int k, int n) { return pair(s.s + n * LDS + k); };
     if (low) {
-      warp_mma<X, !SP, SP>(ap, m0, p0, 0, VB, fd, fu_t);
-      warp_mma<!SP, !SP, SP>(ae, m0, p0, 0, VB, ff, fu_t);
+      warp_mma(ap, m0, p0, 0, VB, fd, fu_t);
+      warp_mma(ae, m0, p0, 0, VB, ff, fu_t);
     }
-    warp_mma<X, !SP, SP>(aq, m0, k0, 0, VB, fd, fs_t);
-    warp_mma<!SP, !SP, SP>(ar, m0, k0, 0, VB, ff, fs_t);
-    warp_mma<!SP, !SP, SP>(ac, m0, k0, 0, VB, [&](int m, int k) { return pair(s.x + m * LDX + k); },
+    warp_mma(aq, m0, k0, 0, VB, fd, fs_t);
+    warp_mma(ar, m0, k0, 0, VB, ff, fs_t);
+    warp_mma(ac, m0, k0, 0, VB, [&](int m, int k) { return pair(s.x + m * LDX + k); },
                            [&](int k, int n) { return pair(s.e + n * LDS + k); });
   }
   __syncthreads();
@@ -302,7 +301,7 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   {
     float ag[1][NK][4];
     zero(ag);
-    warp_mma<!SP, X, SP>(ag, m0, k0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDP + k); }, fk_tok);
+    warp_mma(ag, m0, k0, 0, m0 + 16, [&](int m, int k) { return pair(s.t + m * LDP + k); }, fk_tok);
     row_dot(ag, sk, rg);
 #pragma unroll
     for (int j = 0; j < NK; ++j)
@@ -317,11 +316,11 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   }
   row_dot(ar, sk, rr);
   row_dot(ac, sk, rl);
-  warp_mma<!SP, X, SP>(aq, m0, k0, 0, m0 + 16, [&](int m, int k) { return pair(s.p + m * LDP + k); }, fk_tok);
+  warp_mma(aq, m0, k0, 0, m0 + 16, [&](int m, int k) { return pair(s.p + m * LDP + k); }, fk_tok);
   row_dot(aq, sq, rq);
-  warp_mma<!SP, X, SP>(ac, m0, k0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
+  warp_mma(ac, m0, k0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
                        [&](int k, int n) { return column<LDK>(sq + k * LDK + n); });
-  warp_mma<false, X, SP>(ac, m0, k0, m0, BT,
+  warp_mma(ac, m0, k0, m0, BT,
                          [&](int m, int k) {
                            const float2 x = column<LDP>(s.t + k * LDP + m), b = pair(s.gates.beta + k);
                            return make_float2(-b.x * x.x, -b.y * x.y);

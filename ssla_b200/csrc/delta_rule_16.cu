@@ -214,8 +214,7 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
     float aq[1][NT][4], ak[1][NT][4];
     zero(aq);
     zero(ak);
-    mm(ak, RowA<LDK, PLK, N>(s.k), s_b, m0, n0, 0, KP);
-    mm(aq, RowA<LDK, PLK, N>(s.q), s_b, m0, n0, 0, KP);
+    mm_ab_cb(ak, RowA<LDK, PLK, N>(s.k), aq, RowA<LDK, PLK, N>(s.q), s_b, m0, n0, 0, KP);
     __syncthreads();  // S is read
 #pragma unroll
     for (int j = 0; j < NT; ++j)

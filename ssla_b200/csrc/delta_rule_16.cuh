@@ -112,33 +112,78 @@ template <int LD, int PLANE, int N> struct ColB {
   }
 };
 
+// The kept products of planes of one 16 x 16 block of A with two column tiles, small ones first.
+template <int NA, int NB>
+__device__ __forceinline__ void plane_products(float (&c0)[4], float (&c1)[4], const uint32_t (&fa)[NA][4],
+                                               const uint32_t (&fb)[NB][4]) {
+  constexpr int MOST = NA > NB ? NA : NB;
+#pragma unroll
+  for (int s = MOST - 1; s >= 0; --s)
+#pragma unroll
+    for (int p = 0; p <= s; ++p)
+      if (p < NA && s - p < NB) {
+        mma16(c0, fa[p], fb[s - p][0], fb[s - p][1]);
+        mma16(c1, fa[p], fb[s - p][2], fb[s - p][3]);
+      }
+}
+// all planes of a block of either operand
+template <class A> __device__ __forceinline__ void planes_at(uint32_t (&f)[A::n][4], const A& a, int i, int j) {
+#pragma unroll
+  for (int p = 0; p < A::n; ++p) a.load(f[p], i, j, p);
+}
+
 // acc += A B over k in [k0, k1) (multiples of 16), columns n0 .. n0 + 8 NT
 template <int MT, int NT, class A, class B>
 __device__ __forceinline__ void mm(float (&acc)[MT][NT][4], const A& a, const B& b, int m0, int n0, int k0, int k1) {
   static_assert(NT % 2 == 0, "columns come in pairs of tiles");
-  constexpr int MOST = A::n > B::n ? A::n : B::n;
 #pragma unroll 4
   for (int k = k0; k < k1; k += 16) {
     uint32_t fa[MT][A::n][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int p = 0; p < A::n; ++p) a.load(fa[i][p], m0 + 16 * i, k, p);
+    for (int i = 0; i < MT; ++i) planes_at(fa[i], a, m0 + 16 * i, k);
 #pragma unroll
     for (int j = 0; j < NT; j += 2) {
       uint32_t fb[B::n][4];
+      planes_at(fb, b, k, n0 + 8 * j);
 #pragma unroll
-      for (int p = 0; p < B::n; ++p) b.load(fb[p], k, n0 + 8 * j, p);
+      for (int i = 0; i < MT; ++i) plane_products<A::n, B::n>(acc[i][j], acc[i][j + 1], fa[i], fb);
+    }
+  }
+}
+// Two left operands with one right operand, read once: the loads of shared memory are what these
+// kernels wait for beside the tensor pipe.
+template <int NT, class A, class C, class B>
+__device__ __forceinline__ void mm_ab_cb(float (&x)[1][NT][4], const A& a, float (&y)[1][NT][4], const C& c, const B& b,
+                                         int m0, int n0, int k0, int k1) {
+#pragma unroll 4
+  for (int k = k0; k < k1; k += 16) {
+    uint32_t fa[A::n][4], fc[C::n][4];
+    planes_at(fa, a, m0, k);
+    planes_at(fc, c, m0, k);
 #pragma unroll
-      for (int s = MOST - 1; s >= 0; --s)  // small products first
+    for (int j = 0; j < NT; j += 2) {
+      uint32_t fb[B::n][4];
+      planes_at(fb, b, k, n0 + 8 * j);
+      plane_products<A::n, B::n>(x[0][j], x[0][j + 1], fa, fb);
+      plane_products<C::n, B::n>(y[0][j], y[0][j + 1], fc, fb);
+    }
+  }
+}
+// One left operand with two right operands.
+template <int NT, class A, class B, class C>
+__device__ __forceinline__ void mm_ab_ac(float (&x)[1][NT][4], const B& b, float (&y)[1][NT][4], const C& c, const A& a,
+                                         int m0, int n0, int k0, int k1) {
+#pragma unroll 4
+  for (int k = k0; k < k1; k += 16) {
+    uint32_t fa[A::n][4];
+    planes_at(fa, a, m0, k);
 #pragma unroll
-        for (int p = 0; p <= s; ++p)
-          if (p < A::n && s - p < B::n)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              mma16(acc[i][j], fa[i][p], fb[s - p][0], fb[s - p][1]);
-              mma16(acc[i][j + 1], fa[i][p], fb[s - p][2], fb[s - p][3]);
-            }
+    for (int j = 0; j < NT; j += 2) {
+      uint32_t fb[B::n][4], fc[C::n][4];
+      planes_at(fb, b, k, n0 + 8 * j);
+      planes_at(fc, c, k, n0 + 8 * j);
+      plane_products<A::n, B::n>(x[0][j], x[0][j + 1], fa, fb);
+      plane_products<A::n, C::n>(y[0][j], y[0][j + 1], fa, fc);
     }
   }
 }

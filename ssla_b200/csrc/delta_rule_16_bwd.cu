@@ -207,8 +207,7 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
     float ks[1][NT][4], du[1][NT][4];
     zero(ks);
     zero(du);
-    mm(ks, k_a, s_b, m0, n0, 0, KP);
-    mm(du, k_a, e_b, m0, n0, 0, KP);
+    mm_ab_ac(ks, s_b, du, e_b, k_a, m0, n0, 0, KP);
     const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]};
     const float ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]}, le[2] = {s.gates.left[i0], s.gates.left[i0 + 8]};
 #pragma unroll
@@ -270,12 +269,8 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
     __syncthreads();
     each_pair(du, m0, n0, [&](int i, int n, float x, float y) { put<2, PLX>(s.f + i * LDX + n, x, y); });
     __syncthreads();
-    if (low) {
-      mm(ap, d_a, x_t, m0, p0, 0, VB);
-      mm(ae, f_a, x_t, m0, p0, 0, VB);
-    }
-    mm(aq, d_a, s_t, m0, k0, 0, VB);
-    mm(ar, f_a, s_t, m0, k0, 0, VB);
+    if (low) mm_ab_cb(ap, d_a, ae, f_a, x_t, m0, p0, 0, VB);
+    mm_ab_cb(aq, d_a, ar, f_a, s_t, m0, k0, 0, VB);
     mm(ac, x_a, e_t, m0, k0, 0, VB);
   }
   __syncthreads();

@@ -140,7 +140,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 def on_device(dev: torch.device):
     """Context with ``dev`` current; free when it already is (a decoding step is bound by the host)."""
-    return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def raw_stream(dev: torch.device) -> int:

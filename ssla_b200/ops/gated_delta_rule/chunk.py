@@ -21,50 +21,69 @@ from ... import _lib
 from ..utils.guard import prepare_cu_seqlens
 
 
-def norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, what):
-    """Checked, contiguous inputs of one dtype (q's) on q's device; gates in their own dtype."""
+def _refuse(q, k, v, g, beta, initial_state, cu, what):
+    """The exception for arguments that do not belong together; None where they do."""
     if q.dim() != 3 or k.shape != q.shape or v.dim() != 3 or v.shape[0] != q.shape[0]:
-        raise ValueError(
+        return ValueError(
             f"{what} expects q, k [T, H, K] and v [T, HV, V]; got q {tuple(q.shape)}, k {tuple(k.shape)}, "
             f"v {tuple(v.shape)}"
         )
     T, H, K = q.shape
     _, HV, V = v.shape
     if H == 0 or HV == 0 or HV % H:
-        raise ValueError(f"{what}: the {HV} value heads must be a positive multiple of the {H} key heads")
+        return ValueError(f"{what}: the {HV} value heads must be a positive multiple of the {H} key heads")
     if g.shape != (T, HV) or beta.shape != (T, HV):
-        raise ValueError(f"{what} expects g, beta [T, HV] = [{T}, {HV}]; got {tuple(g.shape)}, {tuple(beta.shape)}")
+        return ValueError(f"{what} expects g, beta [T, HV] = [{T}, {HV}]; got {tuple(g.shape)}, {tuple(beta.shape)}")
     if not (1 <= K <= 128 and 1 <= V <= 256):
-        raise ValueError(f"{what}: K={K}, V={V} not supported (1 <= K <= 128, 1 <= V <= 256)")
-    _lib.require_cuda(q, k, v, g, beta, initial_state, what=what)
-    dev, dt = q.device, q.dtype
-    _lib.dtype_code(q)
+        return ValueError(f"{what}: K={K}, V={V} not supported (1 <= K <= 128, 1 <= V <= 256)")
+    for x in (q, k, v, g, beta, initial_state):
+        if x is not None and not x.is_cuda:
+            return RuntimeError(f"{what}: tensors must be on a CUDA device (no CPU path)")
+    if q.dtype not in _lib._DT:
+        return TypeError(f"unsupported dtype {q.dtype}; expected float32, bfloat16 or float16")
     for x in (k, v, g, beta, initial_state):
-        if x is not None and x.device != dev:
-            raise RuntimeError(f"{what}: all tensors must be on one device, got {dev} and {x.device}")
-    cu = cu_seqlens
-    if cu is None or cu.dim() != 1 or cu.device != dev or cu.dtype != torch.int64 or not cu.is_contiguous() or not len(cu):
-        cu = prepare_cu_seqlens(cu_seqlens, dev)
-    if initial_state is not None:
+        if x is not None and x.device != q.device:
+            return RuntimeError(f"{what}: all tensors must be on one device, got {q.device} and {x.device}")
+    if initial_state is not None and cu is not None:
         N = cu.numel() - 1
         if initial_state.dim() == 0 or initial_state.shape[0] != N:
-            raise ValueError(
+            return ValueError(
                 f"The number of initial states is expected to be equal to the number of input sequences, "
                 f"i.e., {N} rather than {initial_state.shape[0] if initial_state.dim() else 0}."
             )
-        if tuple(initial_state.shape) != (N, HV, K, V):
-            raise ValueError(f"{what}: initial_state must be [N, HV, K, V] = {(N, HV, K, V)}; got "
-                             f"{tuple(initial_state.shape)}")
+        if initial_state.shape != (N, HV, K, V):
+            return ValueError(f"{what}: initial_state must be [N, HV, K, V] = {(N, HV, K, V)}; got "
+                              f"{tuple(initial_state.shape)}")
+    return None
+
+
+def norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, what):
+    """Checked, contiguous inputs of one dtype (q's) on q's device; gates in their own dtype.  A
+    decoding step is bound by this code, so the usual case passes one chain of comparisons."""
+    dev, dt, code, cu = q.device, q.dtype, _lib._DT, cu_seqlens
+    qs, vs = q.shape, v.shape
+    fits = (
+        len(qs) == 3 and len(vs) == 3 and k.shape == qs and vs[0] == qs[0] and 0 < qs[2] <= 128 and 0 < vs[2] <= 256
+        and qs[1] > 0 and vs[1] > 0 and vs[1] % qs[1] == 0 and g.shape == vs[:2] and beta.shape == vs[:2]
+        and q.is_cuda and k.device == dev and v.device == dev and g.device == dev and beta.device == dev and dt in code
+    )
+    if not fits:
+        raise _refuse(q, k, v, g, beta, initial_state, None, what)
+    if cu is None or cu.dim() != 1 or cu.device != dev or cu.dtype != torch.int64 or not cu.is_contiguous() or not len(cu):
+        cu = prepare_cu_seqlens(cu_seqlens, dev)
+    if initial_state is not None:
+        if initial_state.device != dev or initial_state.shape != (len(cu) - 1, vs[1], qs[2], vs[2]):
+            raise _refuse(q, k, v, g, beta, initial_state, cu, what)
         initial_state = initial_state.float().contiguous()
     if k.dtype != dt:
         k = k.to(dt)
     if v.dtype != dt:
         v = v.to(dt)
-    if g.dtype not in _lib._DT:
+    if g.dtype not in code:
         g = g.float()
-    if beta.dtype not in _lib._DT:
+    if beta.dtype not in code:
         beta = beta.float()
-    return (q.contiguous(), k.contiguous(), v.contiguous(), g.contiguous(), beta.contiguous(), cu, initial_state)
+    return q.contiguous(), k.contiguous(), v.contiguous(), g.contiguous(), beta.contiguous(), cu, initial_state
 
 
 def tensor_args(q, k, v, g, beta, cu, scale):
@@ -73,7 +92,7 @@ def tensor_args(q, k, v, g, beta, cu, scale):
     T, H, K = q.shape
     _, HV, V = v.shape
     return (q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), code[q.dtype], code[g.dtype],
-            code[beta.dtype], cu.data_ptr(), cu.shape[0] - 1, T, H, HV, K, V, scale)
+            code[beta.dtype], cu.data_ptr(), cu.shape[0] - 1, T, H, HV, K, V, float(scale))
 
 
 def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
@@ -143,8 +162,11 @@ class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
         return dq, dk, dv, dg, dbeta, None, None, dh0, None
 
 
-def needs_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def needs_grad(q, k, v, g, beta, initial_state) -> bool:
+    return torch.is_grad_enabled() and (
+        q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
+        or (initial_state is not None and initial_state.requires_grad)
+    )
 
 
 @torch.compiler.disable

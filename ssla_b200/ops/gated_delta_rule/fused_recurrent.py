@@ -19,20 +19,17 @@ _NAME = "fused_recurrent_gated_delta_rule"
 
 
 def recurrent_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
-    HV, V = v.shape[1:]
+    dev = q.device
     o = torch.empty_like(v)
     ht = None
     if output_final_state:
         ht = torch.empty_like(h0) if h0 is not None else torch.empty(
-            (cu.numel() - 1, HV, q.shape[-1], V), device=q.device, dtype=torch.float32)
-    with _lib.on_device(q.device):
-        _lib.check(
-            _lib.load().ssla_recurrent_gated_delta_rule_fwd(
-                *tensor_args(q, k, v, g, beta, cu, scale), _lib.ptr(h0), o.data_ptr(), _lib.ptr(ht),
-                _lib.raw_stream(q.device),
-            ),
-            _NAME,
-        )
+            (len(cu) - 1, v.shape[1], q.shape[2], v.shape[2]), device=dev, dtype=torch.float32)
+    with _lib.on_device(dev):
+        rc = _lib.load().ssla_recurrent_gated_delta_rule_fwd(
+            *tensor_args(q, k, v, g, beta, cu, scale), _lib.ptr(h0), o.data_ptr(), _lib.ptr(ht), _lib.raw_stream(dev))
+    if rc:
+        _lib.check(rc, _NAME)
     return o, ht
 
 

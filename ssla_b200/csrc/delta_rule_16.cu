@@ -144,11 +144,12 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
 }
 
 // ------------------------------------------------------------------ output
-// 4 row groups of 16 x 2 column groups of warps; panels of VB value columns, so that two or three
-// blocks fit an SM (KP = 128 with panels of 64, one block of 16 warps: 340 us against 265 for
-// the 32768-token prompt).
+// 4 row groups of 16 x 2 column groups of warps, panels of 64 value columns.  X and U take the place
+// of the state's panel, so that two blocks (K = 128; three at K = 64) fit an SM: the 32768-token
+// prompt's call takes 1082 us, with panels of 32 columns 1104 us.  One block of 16 warps with places
+// of their own was slower than either (340 us for this kernel against 265 us for panels of 32).
 template <class TI, int KP> struct Out16 {
-  static constexpr int N = Planes<TI>::n, LDK = KP + 8, VB = KP == 64 ? 64 : 32, LDX = VB + 8, CG = 2, NTH = 128 * CG;
+  static constexpr int N = Planes<TI>::n, LDK = KP + 8, VB = 64, LDX = VB + 8, CG = 2, NTH = 128 * CG;
   bf k[N * BT * LDK];
   bf q[N * BT * LDK];
   bf t[2 * FRAG_ELEMS];

@@ -409,7 +409,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(BwdSmem<KP>) <= 113 * 1024 ? 2
 // dq, dk [T, H, K] = sums over the value heads of a key head, in their order.  One warp a row of K.
 template <class TO>
 __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ dqk, int64_t TH, int R, int K,
-                                                        TO* __restrict__ dq, TO* __restrict__ dk) {
+                                                        bool vec, TO* __restrict__ dq,
+                                                        TO* __restrict__ dk) {
   griddep_launch_dependents();
   griddep_wait();
   const float* p = dqk + (blockIdx.y ? (size_t)TH * R * K : 0);
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict_
   const int lane = threadIdx.x & 31;
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < TH; row += (int64_t)gridDim.x * 8) {
     const float* src = p + (size_t)row * R * K;
-    if (K % 4 == 0) {
+    if (vec) {
       for (int c = lane * 4; c < K; c += 128) {
         float4 x = *reinterpret_cast<const float4*>(src + c);
         for (int r = 1; r < R; ++r) {
@@ -458,7 +459,8 @@ int backward32(const Args& a, const Saved& sv, int VP, const float* ds, const Gr
 
 template <class TO> int sum_heads(const Args& a, const Grads& g, cudaStream_t st) {
   const int64_t blocks = (a.T * a.H + 7) / 8;
-  launch_pdl(sum_heads_kernel<TO>, dim3((unsigned)(blocks < 16 * kNumSMs ? blocks : 16 * kNumSMs), 2), dim3(256), 0, st, g.dqk, a.T * a.H, a.R, a.K, (TO*)g.dq, (TO*)g.dk);
+  const bool vec = a.K % 4 == 0 && aligned_to(g.dq, 4 * sizeof(TO)) && aligned_to(g.dk, 4 * sizeof(TO));
+  launch_pdl(sum_heads_kernel<TO>, dim3((unsigned)(blocks < 16 * kNumSMs ? blocks : 16 * kNumSMs), 2), dim3(256), 0, st, g.dqk, a.T * a.H, a.R, a.K, vec, (TO*)g.dq, (TO*)g.dk);
   SSLA_CHECK_LAUNCH("gated_delta_rule sum_heads");
   return SSLA_OK;
 }

@@ -122,6 +122,8 @@ def inputs(T=8, H=1, HV=2, K=4, V=4, N=1, **change):
     ({"v": torch.zeros(7, 2, 4)}, "expects q, k"),
     ({"v": torch.zeros(8, 2, 257)}, "not supported"),
     ({"q": torch.zeros(8, 1, 129), "k": torch.zeros(8, 1, 129)}, "not supported"),
+    ({"q": torch.zeros(8, 1, 0), "k": torch.zeros(8, 1, 0)}, "not supported"),
+    ({"q": torch.zeros(())}, "expects q, k"),
     ({"g": torch.zeros(8, 1)}, "expects g, beta"),
     ({"beta": torch.zeros(8, 2, 1)}, "expects g, beta"),
     ({"q": torch.zeros(8, 3, 4), "k": torch.zeros(8, 3, 4)}, "multiple of the 3 key heads"),
@@ -253,6 +255,29 @@ def test_strides_and_alignment(dtype):
             assert torch.equal(a, b), how
         r = operators()["recurrent"](*[y.detach() for y in xs], cu.cuda(), initial_state=h.detach())[0]
         assert torch.equal(r, operators()["recurrent"](*[y.cuda() for y in x], cu.cuda(), initial_state=h0.cuda())[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+def test_results_off_a_vector_boundary(dtype, monkeypatch):
+    """The C entry points write wherever the caller's results lie."""
+    from ssla_b200.ops.gated_delta_rule import chunk
+
+    x, h0, do, dht, cu = make(100, 1, 2, 64, 64, [0, 30, 100], dtype, seed=9)
+    want = on_gpu(operators()["chunk"], x, h0, do, dht, cu)
+
+    def shifted(y):
+        z = torch.empty(y.numel() + 1, dtype=y.dtype, device=y.device)[1:].view(y.shape)
+        assert z.data_ptr() % 8
+        return z
+
+    monkeypatch.setattr(chunk.torch, "empty_like", shifted)
+    xs = [y.cuda() for y in x]
+    scale = x[0].shape[-1] ** -0.5
+    o, ht, states = chunk.chunk_fwd(*xs, cu.cuda(), scale, h0.cuda(), True)
+    got = chunk.chunk_bwd(*xs, cu.cuda(), scale, True, True, states, do.cuda(), dht.cuda())
+    for a, b in zip([o, ht, *got], [want[0], want[1], *want[2]]):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.gpu

@@ -91,8 +91,9 @@ def tensor_args(q, k, v, g, beta, cu, scale):
     code = _lib._DT
     T, H, K = q.shape
     _, HV, V = v.shape
+    scale = K ** -0.5 if scale is None else float(scale)
     return (q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), code[q.dtype], code[g.dtype],
-            code[beta.dtype], cu.data_ptr(), cu.shape[0] - 1, T, H, HV, K, V, float(scale))
+            code[beta.dtype], cu.data_ptr(), cu.shape[0] - 1, T, H, HV, K, V, scale)
 
 
 def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
@@ -189,15 +190,14 @@ def chunk_gated_delta_rule(
         g: log forget gates ``[T, HV]`` (g <= 0; ``-inf`` empties the state before the token).
         beta: writing strengths ``[T, HV]``.
         cu_seqlens: cumulative sequence lengths ``[N+1]``; tokens outside every sequence get zero
-            outputs and zero gradients.
+            outputs and zero gradients, whatever they hold.  Inside a sequence a NaN or infinity also
+            reaches earlier tokens of its chunk of 64 (not with ``fused_recurrent_gated_delta_rule``).
         scale: read-out scale, default ``K ** -0.5``.
         initial_state: ``[N, HV, K, V]`` or None.
         output_final_state: also return the final state ``[N, HV, K, V]`` (fp32).
     Returns:
         ``(o [T, HV, V], final_state or None)``.
     """
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
     if needs_grad(q, k, v, g, beta, initial_state):
         return ChunkGatedDeltaRuleFunction.apply(q, k, v, g, beta, cu_seqlens, scale, initial_state,
                                                  output_final_state)

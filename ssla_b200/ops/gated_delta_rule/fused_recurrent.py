@@ -64,8 +64,6 @@ def fused_recurrent_gated_delta_rule(
     output_final_state: bool = False,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     r"""Recurrent gated delta rule; arguments and returns as ``chunk_gated_delta_rule``."""
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
     if needs_grad(q, k, v, g, beta, initial_state):
         return FusedRecurrentGatedDeltaRuleFunction.apply(q, k, v, g, beta, cu_seqlens, scale, initial_state,
                                                           output_final_state)

@@ -238,6 +238,19 @@ template <int N> __device__ __forceinline__ void put_half(__half* p, size_t plan
     *reinterpret_cast<__half2*>(p + plane) = __floats2half2_rn(x - z.x, y - z.y);
   }
 }
+// w[j] of lane t of a quad <-> w[t] of lane j
+__device__ __forceinline__ void quad_turn(uint32_t (&w)[4], int t) {
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {  // 2 x 2 blocks of neighbours
+    const uint32_t x = __shfl_xor_sync(0xffffffffu, t & 1 ? w[j] : w[j + 1], 1);
+    (t & 1 ? w[j] : w[j + 1]) = x;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {  // the blocks themselves
+    const uint32_t x = __shfl_xor_sync(0xffffffffu, t & 2 ? w[j] : w[j + 2], 2);
+    (t & 2 ? w[j] : w[j + 2]) = x;
+  }
+}
 // A block's panel of PM (64 columns from c0, the accumulators of all its warps) into planes.
 // red: 8 words of shared memory; ends with the block's barrier passed.
 template <int KP, int NPL, int MT>
@@ -258,9 +271,33 @@ __device__ __forceinline__ void store_pm(float (&acc)[MT][4][4], int mk, int c0,
   for (int w = 0; w < THREADS / 32; ++w) most = max(most, red[w]);
   const float sc = plane_scale(most);
   if (threadIdx.x == 0) reinterpret_cast<float*>(record)[1 + c0 / 64] = plane_unscale(sc);
-  each_pair(acc, mk, n0, [&](int m, int n, float x, float y) {
-    put_half<NPL>(pm + m * (KP + 8) + c0 + n, (size_t)KP * (KP + 8), x * sc, y * sc);
-  });
+  // A row's 32 columns of a warp lie with the four lanes of a quad, two of every tile; turned so that
+  // lane t has tile t's eight, a plane is written 16 bytes at a time (4 bytes: TODO).
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      uint32_t w[NPL][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = acc[i][j][2 * r] * sc, y = acc[i][j][2 * r + 1] * sc;
+#pragma unroll
+        for (int q = 0; q < NPL; ++q) {
+          const __half2 h = __floats2half2_rn(x, y);
+          const float2 z = __half22float2(h);
+          w[q][j] = *reinterpret_cast<const uint32_t*>(&h);
+          x -= z.x;
+          y -= z.y;
+        }
+      }
+      __half* const to = pm + (mk + 16 * i + 8 * r + g) * (KP + 8) + c0 + n0 + 8 * t;
+#pragma unroll
+      for (int q = 0; q < NPL; ++q) {
+        quad_turn(w[q], t);
+        *reinterpret_cast<uint4*>(to + (size_t)q * KP * (KP + 8)) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
+      }
+    }
 }
 
 // ------------------------------------------------------------------ copies into shared memory

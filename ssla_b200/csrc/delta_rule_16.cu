@@ -106,12 +106,6 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
   for (int p = 0; p < panels; ++p) {
     const bool w = p < KP / 64;
     const int c0 = (w ? p : p - KP / 64) * 64;
-    if (!w && (c0 == 0 || VP > 64)) {
-      if (p > KP / 64) load_v(c0);
-      if (c0 == 0) scale_t(false);
-      cp_wait<0>();
-      __syncthreads();
-    }
     {
       float acc[1][4][4];
       zero(acc);
@@ -126,6 +120,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
       });
     }
     __syncthreads();
+    if (p + 1 == KP / 64) scale_t(false);  // tc and v are read: the next panel's
+    if (!w && c0 + 64 < VP) load_v(c0 + 64);
     {
       constexpr int MT = KP / 64;
       float acc[MT][4][4];
@@ -139,7 +135,8 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
           *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, c0 + n)) = make_float2(x, y);
         });
     }
-    __syncthreads();  // the readers of v, tc and y are done
+    cp_wait<0>();
+    __syncthreads();  // the readers of y are done
   }
 }
 

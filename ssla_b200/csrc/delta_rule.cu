@@ -308,29 +308,30 @@ __global__ void __launch_bounds__(KP * 2 + 32) chain_kernel(ChainArgs a) {
       }
       if (NT > 1) join(kb);
     }
-    if (a.s && a.planes && NT == 4) {  // 32 columns: 16 bytes a store, 64 of a row together
+    if (a.s && a.planes) {
+      // piece q: plane q / 2 NT, row g + 8 (q / NT % 2), tile q % NT; a quad turns four of them, so that
+      // lane t writes 16 bytes of piece 4 u + t
+      uint32_t w[NT][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        h16::bf* const to = (h16::bf*)a.s + (2 * it * KP + m0 + g + 8 * r) * a.VP + c0 + 8 * t;
-        uint32_t hi[4], lo[4];
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float x = S[0][j % NT][2 * r], y = S[0][j % NT][2 * r + 1];
-          hi[j] = h16::pack(x, y);
-          h16::rest(hi[j], x, y);
-          lo[j] = h16::pack(x, y);
+        for (int r = 0; r < 2; ++r) {
+          float x = S[0][j][2 * r], y = S[0][j][2 * r + 1];
+          const int hi = r * NT + j, lo = hi + 2 * NT;
+          w[hi / 4][hi % 4] = h16::pack(x, y);
+          h16::rest(w[hi / 4][hi % 4], x, y);
+          w[lo / 4][lo % 4] = h16::pack(x, y);
         }
-        quad_turn(hi, t);
-        quad_turn(lo, t);
-        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(to + (size_t)KP * a.VP) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        quad_turn(w[u], t);
+        const int q = 4 * u + t, row = m0 + g + 8 * (q / NT % 2);
+        h16::bf* const to = (h16::bf*)a.s + ((2 * it + q / (2 * NT)) * KP + row) * a.VP + c0 + 8 * (q % NT);
+        *reinterpret_cast<uint4*>(to) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
       }
     } else if (a.s) {
       each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-        if (a.planes)
-          h16::put_at<2>((h16::bf*)a.s + (2 * it * KP + r) * a.VP + c0 + c, (size_t)KP * a.VP, x, y);
-        else
-          *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
+        *reinterpret_cast<float2*>(a.s + (it * KP + r) * a.VP + c0 + c) = make_float2(x, y);
       });
     }
     if (NT == 1)

@@ -198,7 +198,8 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
   const float ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]};
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
   const TI* gv = (const TI*)a.v + vo;
-  const bool even = a.V % 2 == 0 && (reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(o)) % 4 == 0;
+  const bool even = a.V % 2 == 0 && reinterpret_cast<uintptr_t>(a.v) % 4 == 0;
+  const int width = store_width(o, a.V);
   for (int v0 = 0; v0 < a.V; v0 += VB) {
     if (v0) {
       __syncthreads();  // readers of the previous panel are done
@@ -232,18 +233,7 @@ __device__ __forceinline__ void output16_chunk(const Args& a, const longlong2* _
       for (int r = 0; r < 4; ++r) aq[0][j][r] *= ee[r >> 1];
     __syncthreads();
     mm(aq, RowA<LDT, PLT, 2>(s.p), x_b, m0, n0, 0, m0 + 16);
-    each_pair(aq, m0, n0, [&](int i, int n, float x, float y) {
-      const int c = v0 + n;
-      if (i < rows && c < a.V) {
-        TI* p = o + vo + i * vstride + c;
-        if (even) {
-          store2(p, x * a.scale, y * a.scale);
-        } else {
-          stf(p, x * a.scale);
-          if (c + 1 < a.V) stf(p + 1, y * a.scale);
-        }
-      }
-    });
+    store_rows(aq, a.scale, o + vo + v0, vstride, rows, a.V - v0, m0, n0, width);
   }
 }
 

@@ -261,6 +261,56 @@ template <int NTH> __device__ __forceinline__ void copy16(void* dst, const void*
   for (int i = threadIdx.x * 16; i < bytes; i += NTH * 16) cp16((char*)dst + i, (const char*)src + i);
 }
 
+__device__ __forceinline__ uint32_t pack_as(const __nv_bfloat16*, float x, float y) { return pack(x, y); }
+__device__ __forceinline__ uint32_t pack_as(const __half*, float x, float y) {
+  const __half2 v = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// How many elements of a result's rows (cols of them, stride a multiple of cols) one store can take.
+__device__ __forceinline__ int store_width(const void* p, int cols) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  return cols % 8 == 0 && at % 16 == 0 ? 8 : cols % 2 == 0 && at % 4 == 0 ? 2 : 1;
+}
+// A warp's accumulator, times f, into rows [0, rows) and columns [0, cols) of a 16-bit result.  The two
+// columns that a lane has of each 8-column tile are turned within quads into whole tiles: 16 bytes a
+// store.  Piece q: row q / NT, tile q % NT.
+template <class TO, int NT>
+__device__ __forceinline__ void store_rows(const float (&acc)[1][NT][4], float f, TO* out, size_t stride, int rows,
+                                           int cols, int m0, int n0, int width) {
+  static_assert(NT % 2 == 0, "pieces come in fours");
+  const int lane = threadIdx.x & 31, t = lane & 3, i0 = m0 + (lane >> 2);
+  if (width == 8) {
+#pragma unroll
+    for (int u = 0; u < NT / 2; ++u) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = (4 * u + e) % NT, r = (4 * u + e) / NT;
+        w[e] = pack_as(out, f * acc[0][j][2 * r], f * acc[0][j][2 * r + 1]);
+      }
+      quad_turn(w, t);
+      const int q = 4 * u + t, i = i0 + 8 * (q / NT), c = n0 + 8 * (q % NT);
+      if (i < rows && c < cols) *reinterpret_cast<uint4*>(out + i * stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int i = i0 + 8 * r, c = n0 + 8 * j + 2 * t;
+      if (i >= rows || c >= cols) continue;
+      TO* p = out + i * stride + c;
+      const float x = f * acc[0][j][2 * r], y = f * acc[0][j][2 * r + 1];
+      if (width == 2) {
+        store2(p, x, y);
+      } else {
+        stf(p, x);
+        if (c + 1 < cols) stf(p + 1, y);
+      }
+    }
+}
+
 // Pairs (row i, columns c, c + 1) of a token matrix in the accumulator layout, zeros outside: all
 // loads before the first use.  even: an even number of columns, 4-byte aligned.
 template <class TI, int NT>

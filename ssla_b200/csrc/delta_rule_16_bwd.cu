@@ -16,7 +16,7 @@ template <class TI, int KP, int NI> struct Adj16 {
   bf d[N * BT * LDT];
   bf t[NI * FRAG_ELEMS];
   bf w[NI * BT * LDK];  // beta exp(gc) K, then W, then scale qh
-  bf p[NI * BT * LDT];
+  bf p[NI * BT * LDT];  // P; then every second panel of dO
   Gates gates;
 };
 
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 75 * 102
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V;
   const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
   auto load_d = [&](int v0) {
-    load_tokens<TI, LDT, 64, THREADS>(s.d, dout + vo + v0, (size_t)a.HV * a.V, rows, a.V - v0, vec_d);
+    load_tokens<TI, LDT, 64, THREADS>(v0 & 64 ? s.p : s.d, dout + vo + v0, (size_t)a.HV * a.V, rows, a.V - v0, vec_d);
     cp_commit();
   };
   load_d(0);
@@ -98,15 +98,12 @@ __global__ void __launch_bounds__(THREADS, sizeof(Adj16<TI, KP, NI>) <= 75 * 102
   constexpr int MT = KP / 64;
   const int mk = (warp >> 1) * 16 * MT;
   for (int v0 = 0; v0 < VP; v0 += 64) {
-    if (v0) {
-      __syncthreads();
-      load_d(v0);
-      cp_wait<0>();
-    }
-    __syncthreads();
+    cp_wait<0>();
+    __syncthreads();  // this panel is there, the other place is read
+    if (v0 + 64 < VP) load_d(v0 + 64);
     float o[MT][4][4];
     zero(o);
-    mm(o, ColA<LDK, PLK, NI>(s.w), RowB<LDT, PLT, N>(s.d), mk, n0, 0, BT);
+    mm(o, ColA<LDK, PLK, NI>(s.w), RowB<LDT, PLT, N>(v0 & 64 ? s.p : s.d), mk, n0, 0, BT);
     each_pair(o, mk, n0, [&](int m, int n, float x, float y) {
       *reinterpret_cast<float2*>(inc_at(inc, item, KP, VP, m, v0 + n)) = make_float2(x, y);
     });
@@ -162,7 +159,8 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   const int n0 = cg * (VB / CG), p0 = cg * (BT / CG), k0 = cg * (KP / CG);
   const size_t vo = ((size_t)t0 * a.HV + hv) * a.V, vstride = (size_t)a.HV * a.V;
   const bool vec_d = a.vec_v && (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
-  const bool even = a.V % 2 == 0 && (reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(dv)) % 4 == 0;
+  const bool even = a.V % 2 == 0 && reinterpret_cast<uintptr_t>(a.v) % 4 == 0;
+  const int width_v = store_width(dv, a.V);
   const TI* gv = (const TI*)a.v + vo;
   copy16<NTH>(s.t, tinv + item * ((size_t)tplanes * FRAG_ELEMS), 2 * FRAG_BYTES);
   const FragA<2, false> t_a(s.t);
@@ -250,22 +248,14 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
       rb[0] += du[0][j][0] * xv[0][j][0] + du[0][j][1] * xv[0][j][1];
       rb[1] += du[0][j][2] * xv[0][j][2] + du[0][j][3] * xv[0][j][3];
     }
+    {
+      float out[1][NT][4];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+      for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int i = i0 + 8 * r, c = v0 + n0 + 8 * j + 2 * (lane & 3);
-        if (i < rows && c < a.V) {
-          TI* p = dv + vo + i * vstride + c;
-          const float x = be[r] * du[0][j][2 * r], y = be[r] * du[0][j][2 * r + 1];
-          if (even) {
-            store2(p, x, y);
-          } else {
-            stf(p, x);
-            if (c + 1 < a.V) stf(p + 1, y);
-          }
-        }
-      }
+        for (int r = 0; r < 4; ++r) out[0][j][r] = be[r >> 1] * du[0][j][r];
+      store_rows(out, 1.f, dv + vo + v0, vstride, rows, a.V - v0, m0, n0, width_v);
+    }
     __syncthreads();
     each_pair(du, m0, n0, [&](int i, int n, float x, float y) { put<2, PLX>(s.f + i * LDX + n, x, y); });
     __syncthreads();
@@ -324,8 +314,11 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   mm(ac, ColA<LDT, PLT, 2>(s.x), k_b, m0, k0, m0, BT);
   row_dot(ac, s.k, rc);
   const size_t qo = dqk ? ((size_t)t0 * a.HV + hv) * a.K : qk, qstride = (size_t)(dqk ? a.HV : a.H) * a.K;
-  const bool even_k = a.K % 2 == 0 && (reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk)) % 4 == 0;
   auto write = [&](float (&acc)[1][NK][4], TI* out, float* part) {
+    if (!part) {
+      store_rows(acc, 1.f, out + qo, qstride, rows, a.K, m0, k0, store_width(out, a.K));
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < NK; ++j)
 #pragma unroll
@@ -333,19 +326,12 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
         const int i = i0 + 8 * r, c = k0 + 8 * j + 2 * (lane & 3);
         if (i >= rows || c >= a.K) continue;
         const float x = acc[0][j][2 * r], y = acc[0][j][2 * r + 1];
-        const size_t at = qo + i * qstride + c;
-        if (part) {
-          if (a.K % 2 == 0) {
-            *reinterpret_cast<float2*>(part + at) = make_float2(x, y);
-          } else {
-            part[at] = x;
-            if (c + 1 < a.K) part[at + 1] = y;
-          }
-        } else if (even_k) {
-          store2(out + at, x, y);
+        float* const p = part + qo + i * qstride + c;
+        if (a.K % 2 == 0) {
+          *reinterpret_cast<float2*>(p) = make_float2(x, y);
         } else {
-          stf(out + at, x);
-          if (c + 1 < a.K) stf(out + at + 1, y);
+          p[0] = x;
+          if (c + 1 < a.K) p[1] = y;
         }
       }
   };

@@ -137,9 +137,11 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
 // of bulk copies (a warp of its own issues them; the memory has the layout of shared memory), and has one
 // barrier.  A wait that gives up makes the rest of the chain NaN.
 // What bounds it: the dependent chain of a step (barrier, MMAs, rescaling), 0.6 us for 64 x 64; for
-// 128 x 128 at fp32 accuracy the 74 KB a step from L2, 1.0 us with 8 columns on 128 SMs.  (Two CTAs that
+// 128 x 128 at fp32 accuracy the 74 KB a step from L2, 0.95 us with 8 columns on 128 SMs.  (Two CTAs that
 // share a state over distributed shared memory halve those bytes, but the cluster barrier took a step
-// to 1.7 us; two buffers instead of three, 2.0 us.)
+// to 1.7 us; two buffers instead of three, 2.0 us; two blocks per SM for 32 columns, with B in
+// registers, 106 us instead of 92 for 112 chains.)  States leave in 16-byte pieces: 4-byte stores took 117
+// us there.
 template <int KP, int VS, int NP> struct ChainSmem {
   static constexpr int LDP = KP + 8, LDS = VS == 8 ? 8 : VS + 8;  // ldmatrix without conflicts
   static constexpr int PM = pm_bytes(KP, NP), B = 4 * KP * VS, STAGE = PM + B;  // bytes
@@ -514,9 +516,9 @@ Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V) {
   p.MC = max_chunks(N, T);
   const int VP = pad_v(V);
   // Columns of a chain: 8 while that leaves few blocks (a step is its own latency: 512 steps of 128 x
-  // 128 take 0.51 ms with 8 columns on 128 SMs, 1.0 ms with 16 on 64), up to 32 while at least two
-  // blocks per SM remain (the map is read once per block: 112 chains of 128 x 128 take 198 us with 8
-  // columns, 121 us with 32).
+  // 128 take 0.48 ms with 8 columns on 128 SMs, 0.64 ms with 16 on 64), up to 32 while at least two
+  // blocks per SM remain (the map is read once per block: 112 chains of 128 x 128 take 186 us with 8
+  // columns, 117 us with 16, 92 us with 32).
   p.vs = 8;
   while (p.vs < 32 && N * HV * (VP / (2 * p.vs)) >= 2 * kNumSMs) p.vs *= 2;
   return p;

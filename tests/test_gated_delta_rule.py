@@ -5,8 +5,9 @@ Tolerances (RMS relative, ``conftest.assert_close``; single elements within 5x o
 magnitude).  fp32 and the fp32 states of every type: products of split TF32 operands are off by
 about 2^-21 and fp32 sums of up to 128 terms by a few 2^-24, over a dozen chained products well
 below 1e-5.  16-bit outputs are rounded once (half a step: bf16 2^-8, fp16 2^-11); the products
-behind a bf16 output round their operands to TF32 (2^-11 each, about ten in a row), together below
-one bf16 step's half, and behind an fp16 output they are split: 2^-8 and 2^-10 are above both."""
+behind them take operands of two bf16 planes (2^-17 each, about ten in a row), and behind bf16 outputs
+of calls without any state the chunks' start states have 11 bits (2^-12 once per chunk, decaying with
+the state): together below half a bf16 step, and below half an fp16 step, so 2^-8 and 2^-10 are above both."""
 import pytest
 import torch
 import torch.nn.functional as F
@@ -105,6 +106,37 @@ def test_backward(dtype, T, H, HV, K, V, cu):
                 assert float(a.abs().max()) <= bound, name
                 continue
             assert_close(a, b, TOL[a.dtype], name)
+
+
+# Enough states for chains of 16 and of 32 columns; with and without states that go in and out.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("T,H,HV,K,cu", [
+    (80, 20, 40, 40, [0, 70, 80]),
+    (80, 40, 40, 128, [0, 70, 80]),
+    (90, 60, 60, 40, [0, 66, 70, 90]),
+    (90, 30, 60, 128, [0, 66, 70, 90]),
+    (200, 2, 2, 64, [0, 200]),
+    (200, 1, 2, 128, [0, 150, 200]),
+])
+def test_many_states_and_none(T, H, HV, K, cu, state, dtype):
+    f = operators()["chunk"]
+    x, h0, do, dht, cu_t = make(T, H, HV, K, 64, cu, dtype, seed=T + K, h0=state)
+    if state:
+        o, ht, g = on_gpu(f, x, h0, do, dht, cu_t)
+    else:
+        dht = torch.zeros_like(dht)
+        leaves = [y.cuda().requires_grad_() for y in x]
+        o, ht = f(*leaves, cu_t.cuda())
+        assert ht is None
+        g = torch.autograd.grad(o, leaves, do.cuda())
+    o_r, ht_r, g_r = reference(x, h0, do, dht, cu_t)
+    assert_close(o, o_r, TOL[dtype], "o")
+    if state:
+        assert_close(ht, ht_r, TOL[torch.float32], "ht")
+    for name, a, b in zip(NAMES, g, g_r):
+        assert_close(a, b, TOL[a.dtype], name)
 
 
 # ------------------------------------------------------------------ refusals (no GPU)
@@ -258,17 +290,18 @@ def test_strides_and_alignment(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,off", [(1, 1), (2, 1), (2, 2)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
-def test_results_off_a_vector_boundary(dtype, monkeypatch):
+def test_results_off_a_vector_boundary(dtype, H, off, monkeypatch):
     """The C entry points write wherever the caller's results lie."""
     from ssla_b200.ops.gated_delta_rule import chunk
 
-    x, h0, do, dht, cu = make(100, 1, 2, 64, 64, [0, 30, 100], dtype, seed=9)
+    x, h0, do, dht, cu = make(100, H, 2, 64, 64, [0, 30, 100], dtype, seed=9)
     want = on_gpu(operators()["chunk"], x, h0, do, dht, cu)
 
     def shifted(y):
-        z = torch.empty(y.numel() + 1, dtype=y.dtype, device=y.device)[1:].view(y.shape)
-        assert z.data_ptr() % 8
+        z = torch.empty(y.numel() + off, dtype=y.dtype, device=y.device)[off:].view(y.shape)
+        assert z.data_ptr() % 16
         return z
 
     monkeypatch.setattr(chunk.torch, "empty_like", shifted)

@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ... import _lib
-from ..utils.guard import prepare_cu_seqlens
+from ..utils.guard import prepare_cu_seqlens, refuse_tangents
 
 
 def _refuse(q, k, v, g, beta, initial_state, cu, what):
@@ -198,6 +198,7 @@ def chunk_gated_delta_rule(
     Returns:
         ``(o [T, HV, V], final_state or None)``.
     """
+    refuse_tangents("chunk_gated_delta_rule", q, k, v, g, beta, initial_state)
     if needs_grad(q, k, v, g, beta, initial_state):
         return ChunkGatedDeltaRuleFunction.apply(q, k, v, g, beta, cu_seqlens, scale, initial_state,
                                                  output_final_state)

@@ -13,6 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ... import _lib
+from ..utils.guard import refuse_tangents
 from .chunk import chunk_bwd, chunk_fwd, needs_grad, norm_inputs, tensor_args
 
 _NAME = "fused_recurrent_gated_delta_rule"
@@ -64,6 +65,7 @@ def fused_recurrent_gated_delta_rule(
     output_final_state: bool = False,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     r"""Recurrent gated delta rule; arguments and returns as ``chunk_gated_delta_rule``."""
+    refuse_tangents(_NAME, q, k, v, g, beta, initial_state)
     if needs_grad(q, k, v, g, beta, initial_state):
         return FusedRecurrentGatedDeltaRuleFunction.apply(q, k, v, g, beta, cu_seqlens, scale, initial_state,
                                                           output_final_state)

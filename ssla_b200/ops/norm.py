@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .utils.guard import prepare_cu_seqlens
+from .utils.guard import prepare_cu_seqlens, refuse_tangents
 
 _ACT = {None: 0, "none": 0, "silu": 1, "relu": 2}
 MAX_TOKEN_GROUP = 1024  # channels of a group that is normalised per token
@@ -130,6 +130,7 @@ def group_norm_act(
     Returns:
         y in x's shape and dtype (statistics in fp32 or more, one rounding at the end).
     """
+    refuse_tangents("group_norm_act", x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return GroupNormActFunction.apply(x, num_groups, weight, bias, cu_seqlens, eps, activation)
     x, w, b, cu, T, C = _inputs(x, num_groups, weight, bias, cu_seqlens, activation)

@@ -8,6 +8,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 
 def input_guard(fn):
@@ -35,3 +36,13 @@ def prepare_cu_seqlens(cu_seqlens: torch.Tensor, device: torch.device) -> torch.
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError(f"cu_seqlens must be 1-D [N+1], got shape {tuple(cu_seqlens.shape)}")
     return cu_seqlens.to(device=device, dtype=torch.int64).contiguous()
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """For operators that skip their autograd function where no input requires a gradient: an input
+    with a forward-mode tangent is refused, as that function would refuse it.  The result would carry
+    no tangent, which reads as a derivative of zero.  Free while no dual level is open."""
+    if forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors
+    ):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")

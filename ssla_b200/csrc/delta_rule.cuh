@@ -422,6 +422,39 @@ __device__ __forceinline__ void fade_scores(float (&acc)[1][NT][4], const Gates&
   }
 }
 
+// out[i] = f acc(i, i) for the diagonal entries that a warp's accumulator holds
+template <int NT>
+__device__ __forceinline__ void diagonal(const float (&acc)[1][NT][4], float f, float* out, int m0, int n0) {
+  const int lane = threadIdx.x & 31, i0 = m0 + (lane >> 2), j0 = n0 + 2 * (lane & 3);
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = i0 + (r >> 1) * 8;
+      if (i == j0 + 8 * t + (r & 1)) out[i] = f * acc[0][t][r];
+    }
+}
+
+// One warp: dg of rows 2 lane, 2 lane + 1 of a chunk = sum of rc over this and the later rows + sum of
+// left over the earlier ones + end.
+__device__ __forceinline__ void gate_sums(const float (&rc)[2], const float (&left)[2], float end, float (&dg)[2]) {
+  const int lane = threadIdx.x & 31;
+  float suf = rc[0] + rc[1], pre = left[0] + left[1];
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const float x = __shfl_down_sync(0xffffffffu, suf, m), y = __shfl_up_sync(0xffffffffu, pre, m);
+    if (lane + m < 32) suf += x;
+    if (lane >= m) pre += y;
+  }
+  suf = __shfl_down_sync(0xffffffffu, suf, 1);
+  pre = __shfl_up_sync(0xffffffffu, pre, 1);
+  if (lane == 31) suf = 0.f;
+  if (lane == 0) pre = 0.f;
+  const float last = rc[1] + suf;
+  dg[0] = (rc[0] + last) + pre + end;
+  dg[1] = last + (left[0] + pre) + end;
+}
+
 __device__ __forceinline__ bool locate(const longlong2* tab, int64_t MC, int64_t chunk, int64_t& t0, int& rows) {
   if (chunk >= MC) return false;
   const longlong2 e = tab[chunk];

@@ -118,13 +118,14 @@ template <class TI, int KP> struct Bwd16 {
   bf q[N * BT * LDK];
   bf d[N * BT * LDX];
   bf t[2 * FRAG_ELEMS];
-  bf p[2 * BT * LDT];  // P, then dP
+  bf p[2 * BT * LDT];  // P, then dP below its diagonal
   bf x[2 * BT * LDX];  // beta X, then U;  x and f at last -beta E
   bf f[2 * BT * LDX];  // dU, then F
   bf s[2 * KP * LDX];  // S;  s and e at last E
   bf e[2 * KP * LDX];  // D
   float red[6][CG][BT];
   float dots[NTH / 32];
+  float diag[BT];  // of dP
   Gates gates;
   static_assert(4 * BT * LDX >= 2 * BT * LDT && 4 * KP * LDX >= 2 * BT * LDT, "E fits the panels' places");
 };
@@ -267,7 +268,8 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   bf* const sE = s.s;  // E;  -beta E at s.x
   const float be[2] = {s.gates.beta[i0], s.gates.beta[i0 + 8]}, ee[2] = {s.gates.start[i0], s.gates.start[i0 + 8]};
   const float le[2] = {s.gates.left[i0], s.gates.left[i0 + 8]};
-  fade_scores<false, true>(ap, s.gates, m0, p0);
+  diagonal(ap, a.scale, s.diag, m0, p0);
+  fade_scores<true, true>(ap, s.gates, m0, p0);
   fade_scores<true, true>(ae, s.gates, m0, p0);
   each_pair(ap, m0, p0, [&](int i, int j, float x, float y) { put<2, PLT>(s.p + i * LDT + j, a.scale * x, a.scale * y); });
   each_pair(ae, m0, p0, [&](int i, int j, float x, float y) {
@@ -277,19 +279,35 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   });
   __syncthreads();
   float rl[2] = {0.f, 0.f}, rq[2] = {0.f, 0.f}, rr[2] = {0.f, 0.f}, rc[2] = {0.f, 0.f}, rg[2] = {0.f, 0.f};
+  auto token_pair = [&](const bf* tile, int j, int r) {
+    const bf* p = tile + (i0 + 8 * r) * LDK + k0 + 8 * j + 2 * (lane & 3);
+    float2 z = pair(p);
+    if (N > 1) {
+      const float2 y = pair(p + (N - 1) * PLK);
+      z.x += y.x;
+      z.y += y.y;
+    }
+    return z;
+  };
   auto row_dot = [&](float (&acc)[1][NK][4], const bf* tile, float (&out)[2]) {
 #pragma unroll
     for (int j = 0; j < NK; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const bf* p = tile + (i0 + 8 * r) * LDK + k0 + 8 * j + 2 * (lane & 3);
-        float2 z = pair(p);
-        if (N > 1) {
-          const float2 y = pair(p + (N - 1) * PLK);
-          z.x += y.x;
-          z.y += y.y;
-        }
+        const float2 z = token_pair(tile, j, r);
         out[r] += acc[0][j][2 * r] * z.x + acc[0][j][2 * r + 1] * z.y;
+      }
+  };
+  // acc += dP_ii times row i of a tile
+  auto add_diagonal = [&](float (&acc)[1][NK][4], const bf* tile) {
+    const float d[2] = {s.diag[i0], s.diag[i0 + 8]};
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float2 z = token_pair(tile, j, r);
+        acc[0][j][2 * r] = fmaf(d[r], z.x, acc[0][j][2 * r]);
+        acc[0][j][2 * r + 1] = fmaf(d[r], z.y, acc[0][j][2 * r + 1]);
       }
   };
   {
@@ -308,11 +326,13 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   }
   row_dot(ar, s.k, rr);
   row_dot(ac, s.k, rl);
+#pragma unroll
+  for (int j = 0; j < NK; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ac[0][j][r] += ar[0][j][r];
   mm(aq, RowA<LDT, PLT, 2>(s.p), k_b, m0, k0, 0, m0 + 16);
   row_dot(aq, s.q, rq);
-  mm(ac, p_t, q_b, m0, k0, m0, BT);
-  mm(ac, ColA<LDT, PLT, 2>(s.x), k_b, m0, k0, m0, BT);
-  row_dot(ac, s.k, rc);
+  add_diagonal(aq, s.k);
   const size_t qo = dqk ? ((size_t)t0 * a.HV + hv) * a.K : qk, qstride = (size_t)(dqk ? a.HV : a.H) * a.K;
   auto write = [&](float (&acc)[1][NK][4], TI* out, float* part) {
     if (!part) {
@@ -336,10 +356,15 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
       }
   };
   write(aq, dq, dqk);
+  zero(aq);  // dk[column] without the terms with D
+  mm(aq, p_t, q_b, m0, k0, m0, BT);
+  mm(aq, ColA<LDT, PLT, 2>(s.x), k_b, m0, k0, m0, BT);
+  row_dot(aq, s.k, rc);
 #pragma unroll
   for (int j = 0; j < NK; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) ac[0][j][r] += ar[0][j][r];
+    for (int r = 0; r < 4; ++r) ac[0][j][r] += aq[0][j][r];
+  add_diagonal(ac, s.q);
   write(ac, dk, dqk ? dqk + TK : nullptr);
   auto reduce = [&](float (&x)[2], int slot) {
 #pragma unroll
@@ -361,7 +386,10 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
   if (lane == 0) s.dots[warp] = dot;
   __syncthreads();
   if (warp) return;
-  float sum = 0.f, gc[2];
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < NTH / 32; ++w) all += s.dots[w];
+  float rc2[2], left[2], dg2[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int i = 2 * lane + r;
@@ -371,25 +399,14 @@ __device__ __forceinline__ void backward16_chunk(const Args& a, const longlong2*
       for (int c = 0; c < CG; ++c) x += s.red[slot][c][i];
       return x;
     };
-    gc[r] = row(2) + row(3) - row(4);
-    sum += row(5);
+    rc2[r] = row(2) + row(3) - row(4);
+    left[r] = row(5);
     if (i < rows) st_any(dbeta, a.dt_b, (size_t)(t0 + i) * a.HV + hv, row(0) - row(1));
   }
-#pragma unroll
-  for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-  float all = 0.f;
-#pragma unroll
-  for (int w = 0; w < NTH / 32; ++w) all += s.dots[w];
-  sum = fmaf(s.gates.whole, all, sum);
-  float suf = gc[0] + gc[1];  // inclusive suffix sums over lanes
-#pragma unroll
-  for (int m = 1; m < 32; m <<= 1) {
-    const float y = __shfl_down_sync(0xffffffffu, suf, m);
-    if (lane + m < 32) suf += y;
-  }
+  gate_sums(rc2, left, s.gates.whole * all, dg2);
   const size_t at = (size_t)(t0 + 2 * lane) * a.HV + hv;
-  if (2 * lane < rows) st_any(dg, a.dt_g, at, suf + sum);
-  if (2 * lane + 1 < rows) st_any(dg, a.dt_g, at + a.HV, suf - gc[0] + sum);
+  if (2 * lane < rows) st_any(dg, a.dt_g, at, dg2[0]);
+  if (2 * lane + 1 < rows) st_any(dg, a.dt_g, at + a.HV, dg2[1]);
 }
 
 template <class TI, int KP>

@@ -8,9 +8,15 @@
 //   dK = [-beta exp(gc) F S^T - beta E K] + [exp(gC - gc) U D^T + dP^T Q - E^T beta K]
 //   dbeta_i = F_i . X_i - k_i . (E K)_i
 // The first bracket of dK is K's part as the row (later) index of the scores, the second as the
-// column; every decay exp(gc_i - gc_j) pairs a row with a column, so that
-//   dgc_i = q_i . dq_i + k_i . dk_i[row] - k_i . dk_i[column]
-// plus, at the chunk's last token, sum_j k_j . (exp(gC - gc) U D^T)_j + exp(gC) <S, D>.
+// column; every decay exp(gc_i - gc_j) pairs a row i with a column j and adds the pair's term to dg of
+// the tokens between, j < t <= i (the chunk's start is the column of the terms with S, its end the row of
+// those with D).  So with r_i = q_i . dq_i + k_i . dk_i[row], c_i = k_i . dk_i[column] without the
+// terms with D, and l_i = k_i . (exp(gC - gc) U D^T)_i,
+//   dg_t = sum_{i >= t} (r_i - c_i) + sum_{i < t} l_i + exp(gC) <S, D>.
+// The pairs behind t cancel in the first sum.  The diagonal of dP, a decay of 1 between a token and
+// itself, belongs to no dg, but is by far the largest term where a head forgets fast: it stays out of dP
+// (strictly lower here) and joins dq and dk behind the sums, q_i k_i dP_ii each.  With it inside, dg at
+// g = -20 was its rounding alone.
 #include "delta_rule.cuh"
 
 namespace ssla {
@@ -127,6 +133,7 @@ template <int KP> struct BwdSmem {
   float e[KP * LDS];  // D
   float red[6][2][BT];
   float dots[THREADS / 32];
+  float diag[BT];  // of dP
   Gates gates;
 };
 
@@ -277,7 +284,8 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   }
   __syncthreads();
   // dP and E take the places of P and T
-  fade_scores<false, false>(ap, s.gates, m0, p0);
+  diagonal(ap, a.scale, s.diag, m0, p0);
+  fade_scores<true, false>(ap, s.gates, m0, p0);
   fade_scores<true, false>(ae, s.gates, m0, p0);
   each_pair(ap, m0, p0, [&](int i, int j, float x, float y) {
     *reinterpret_cast<float2*>(s.p + i * LDP + j) = make_float2(a.scale * x, a.scale * y);
@@ -316,17 +324,22 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   }
   row_dot(ar, sk, rr);
   row_dot(ac, sk, rl);
+#pragma unroll
+  for (int j = 0; j < NK; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) ac[0][j][r] += ar[0][j][r];
   warp_mma(aq, m0, k0, 0, m0 + 16, [&](int m, int k) { return pair(s.p + m * LDP + k); }, fk_tok);
   row_dot(aq, sq, rq);
-  warp_mma(ac, m0, k0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
-                       [&](int k, int n) { return column<LDK>(sq + k * LDK + n); });
-  warp_mma(ac, m0, k0, m0, BT,
-                         [&](int m, int k) {
-                           const float2 x = column<LDP>(s.t + k * LDP + m), b = pair(s.gates.beta + k);
-                           return make_float2(-b.x * x.x, -b.y * x.y);
-                         },
-                         fk_tok);
-  row_dot(ac, sk, rc);
+  // acc += dP_ii times row i of a tile
+  auto add_diagonal = [&](float (&acc)[1][NK][4], const TI* tile) {
+    const float d[2] = {s.diag[i0], s.diag[i0 + 8]};
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc[0][j][r] = fmaf(d[r >> 1], ldf(tile + (i0 + 8 * (r >> 1)) * LDK + k0 + 8 * j + 2 * (lane & 3) + (r & 1)), acc[0][j][r]);
+  };
+  add_diagonal(aq, sk);
   const size_t qo = dqk ? ((size_t)t0 * a.HV + hv) * a.K : qk, qstride = (size_t)(dqk ? a.HV : a.H) * a.K;
   auto put = [&](size_t at, int c, float x, float y, TI* out, float* part) {
     if (part) {
@@ -340,10 +353,21 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   each_pair(aq, m0, k0, [&](int i, int c, float x, float y) {
     if (i < rows) put(qo + i * qstride + c, c, x, y, dq, dqk);
   });
+  zero(aq);  // dk[column] without the terms with D
+  warp_mma(aq, m0, k0, m0, BT, [&](int m, int k) { return column<LDP>(s.p + k * LDP + m); },
+                       [&](int k, int n) { return column<LDK>(sq + k * LDK + n); });
+  warp_mma(aq, m0, k0, m0, BT,
+                         [&](int m, int k) {
+                           const float2 x = column<LDP>(s.t + k * LDP + m), b = pair(s.gates.beta + k);
+                           return make_float2(-b.x * x.x, -b.y * x.y);
+                         },
+                         fk_tok);
+  row_dot(aq, sk, rc);
 #pragma unroll
   for (int j = 0; j < NK; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) ac[0][j][r] += ar[0][j][r];
+    for (int r = 0; r < 4; ++r) ac[0][j][r] += aq[0][j][r];
+  add_diagonal(ac, sq);
   each_pair(ac, m0, k0, [&](int i, int c, float x, float y) {
     if (i < rows) put(qo + i * qstride + c, c, x, y, dk, dqk ? dqk + TK : nullptr);
   });
@@ -368,30 +392,22 @@ __device__ __forceinline__ void backward_chunk(const Args& a, const longlong2* _
   if (lane == 0) s.dots[warp] = dot;
   __syncthreads();
   if (warp) return;
-  float sum = 0.f, gc[2];
+  float all = 0.f;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) all += s.dots[w];
+  float rc2[2], left[2], dg2[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int i = 2 * lane + r;
     auto row = [&](int slot) { return s.red[slot][0][i] + s.red[slot][1][i]; };
-    gc[r] = row(2) + row(3) - row(4);
-    sum += row(5);
+    rc2[r] = row(2) + row(3) - row(4);
+    left[r] = row(5);
     if (i < rows) st_any(dbeta, a.dt_b, (size_t)(t0 + i) * a.HV + hv, row(0) - row(1));
   }
-#pragma unroll
-  for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-  float all = 0.f;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) all += s.dots[w];
-  sum = fmaf(s.gates.whole, all, sum);
-  float suf = gc[0] + gc[1];  // inclusive suffix sums over lanes
-#pragma unroll
-  for (int m = 1; m < 32; m <<= 1) {
-    const float y = __shfl_down_sync(0xffffffffu, suf, m);
-    if (lane + m < 32) suf += y;
-  }
+  gate_sums(rc2, left, s.gates.whole * all, dg2);
   const size_t at = (size_t)(t0 + 2 * lane) * a.HV + hv;
-  if (2 * lane < rows) st_any(dg, a.dt_g, at, suf + sum);
-  if (2 * lane + 1 < rows) st_any(dg, a.dt_g, at + a.HV, suf - gc[0] + sum);
+  if (2 * lane < rows) st_any(dg, a.dt_g, at, dg2[0]);
+  if (2 * lane + 1 < rows) st_any(dg, a.dt_g, at + a.HV, dg2[1]);
 }
 
 template <int KP>

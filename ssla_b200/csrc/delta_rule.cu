@@ -131,21 +131,25 @@ __global__ void __launch_bounds__(THREADS, 2) prep_kernel(Args a, const longlong
 // One CTA carries VS columns of one state along its sequence's chunks; every warp owns 16 of the KP
 // rows in the accumulator layout (fp32).  The one product of a step, PM S, runs on fp16 planes (NP =
 // 2: hi + lo, 22 bits, three MMAs; NP = 1: 11 bits, for states whose only readers are bf16 outputs):
-// prep leaves PM in planes scaled by a power of two, and every warp scales its 16 rows of S by one
-// of its own before it shares them, so that 16 rows of the contraction have one scale, undone when
-// their MMA's result is added.  A step streams the chunk's record and its slice of B through a ring
+// prep leaves PM in planes scaled by a power of two per 64 columns, and every warp scales each column of
+// its 16 rows of S by one of its own before it shares them, undone when the MMA over those 16 rows of
+// the contraction is added.  Value columns never meet, so none may set another's scale: with one scale for
+// a warp's columns, a column 1e-8 times its neighbour had lost half its bits, and which columns share it
+// went with the number of chains.  A step streams the chunk's record and its slice of B through a ring
 // of bulk copies (a warp of its own issues them; the memory has the layout of shared memory), and has one
 // barrier.  A wait that gives up makes the rest of the chain NaN.
-// What bounds it: the dependent chain of a step (barrier, MMAs, rescaling), 0.6 us for 64 x 64; for
-// 128 x 128 at fp32 accuracy the 74 KB a step from L2, 0.95 us with 8 columns on 128 SMs.  (Two CTAs that
-// share a state over distributed shared memory halve those bytes, but the cluster barrier took a step
-// to 1.7 us; two buffers instead of three, 2.0 us; two blocks per SM for 32 columns, with B in
-// registers, 106 us instead of 92 for 112 chains.)  States leave in 16-byte pieces: 4-byte stores took 117
-// us there.
+// What bounds it: the dependent chain of a step (barrier, MMAs, rescaling), 0.66 us for 64 x 64; for
+// 128 x 128 at fp32 accuracy the 74 KB a step from L2 too, 1.03 us with 8 columns on 128 SMs.  The scales by
+// column are 0.06 and 0.09 us of that (three dependent shuffles; reductions of the warp under four masks
+// instead: 1.35 us).  Before they came, at 0.95 us and 92 us for 112 chains of 32 columns (105 us now):
+// two CTAs that share a state over distributed shared memory halve the bytes, but the cluster barrier took a
+// step to 1.7 us; two buffers instead of three, 2.0 us; two blocks per SM for 32 columns, with B in
+// registers, 106 us; states leaving in 4-byte instead of 16-byte pieces, 117 us.
 template <int KP, int VS, int NP> struct ChainSmem {
   static constexpr int LDP = KP + 8, LDS = VS == 8 ? 8 : VS + 8;  // ldmatrix without conflicts
   static constexpr int PM = pm_bytes(KP, NP), B = 4 * KP * VS, STAGE = PM + B;  // bytes
-  static constexpr int S = 2 * NP * KP * LDS, STATE = 2 * (S + 4 * (KP / 16)), MOST = 227 * 1024 - 1024;
+  // two buffers of the state's planes and of what undoes their scales: bf16 [KP / 16][4 lanes][tile][2 columns]
+  static constexpr int S = 2 * NP * KP * LDS, UN = 2 * (KP / 16) * VS, STATE = 2 * (S + UN), MOST = 227 * 1024 - 1024;
   static constexpr int fit = (MOST - STATE - 64) / STAGE, stages = fit > 4 ? 4 : fit, bytes = STATE + 64 + stages * STAGE;
   static_assert(stages >= 2 && STATE % 32 == 0 && STAGE % 16 == 0, "a step is loaded while another runs");
 };
@@ -238,17 +242,26 @@ __global__ void __launch_bounds__(KP * 2 + 32) chain_kernel(ChainArgs a) {
   for (int i = 0; i < count; ++i) {
     const size_t it = at(i);
     __half* sc = reinterpret_cast<__half*>(raw + (i & 1) * (M::STATE / 2));
-    float* un = reinterpret_cast<float*>(raw + (i & 1) * (M::STATE / 2) + M::S);
-    unsigned most = 0;
+    uint32_t* un = reinterpret_cast<uint32_t*>(raw + (i & 1) * (M::STATE / 2) + M::S);
+    // largest exponents of a lane's two columns of each tile, in the halves of a word, over the 16 rows
+    unsigned most[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
+      most[j] = __byte_perm(max(finite_bits(S[0][j][0]), finite_bits(S[0][j][2])),
+                            max(finite_bits(S[0][j][1]), finite_bits(S[0][j][3])), 0x7632);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) most = max(most, finite_bits(S[0][j][r]));
-    const float scale = plane_scale(__reduce_max_sync(0xffffffffu, most));
-    if (lane == 0) un[warp] = plane_unscale(scale);
-    each_pair(S, m0, 0, [&](int r, int c, float x, float y) {
-      put_half<NP>(sc + r * LDS + c, KP * LDS, x * scale, y * scale);
-    });
+    for (int d = 4; d < 32; d <<= 1)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) most[j] = __vmaxu2(most[j], __shfl_xor_sync(0xffffffffu, most[j], d));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const uint32_t scales = plane_scales(most[j]);
+      const float x = __uint_as_float(scales << 16), y = __uint_as_float(scales & 0xffff0000u);
+      if (g == 0) un[(warp * 4 + t) * NT + j] = plane_unscales(scales);
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        put_half<NP>(sc + (m0 + g + 8 * r) * LDS + 8 * j + 2 * t, KP * LDS, S[0][j][2 * r] * x, S[0][j][2 * r + 1] * y);
+    }
     good = good && tc::mbar_wait(full + i % ST, (i / ST) & 1, 1u << 20);
     __syncthreads();  // the state is there, step i - 1 is read
     const unsigned char* stage = ring + (i % ST) * M::STAGE;
@@ -261,12 +274,36 @@ __global__ void __launch_bounds__(KP * 2 + 32) chain_kernel(ChainArgs a) {
     // products of 16 rows of the contraction; of a single column tile all of them stay open while the
     // state is stored
     float parts[NT == 1 ? NB : 1][NT][4];
+    float u[NT == 1 ? NB : 1][2 * NT];  // what undoes the scales of a lane's columns, times PM's
+    auto undo = [&](int kb) {
+      const float f = TRANS ? 1.f : ps[kb / 4];
+      const uint32_t* p = un + (kb * 4 + t) * NT;
+      uint32_t w[NT];
+      if constexpr (NT == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+      } else if constexpr (NT == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[0] = x.x; w[1] = x.y;
+      } else {
+        w[0] = *p;
+      }
+      float(&v)[2 * NT] = u[NT == 1 ? kb : 0];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        v[2 * j] = f * __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = f * __uint_as_float(w[j] & 0xffff0000u);
+      }
+    };
+    if (NT == 1)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) undo(kb);
     auto join = [&](int kb) {
-      const float f = TRANS ? un[kb] : un[kb] * ps[kb / 4];
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(f, parts[NT == 1 ? kb : 0][j][r], acc[j][r]);
+        for (int r = 0; r < 4; ++r)
+          acc[j][r] = fmaf(u[NT == 1 ? kb : 0][2 * j + (r & 1)], parts[NT == 1 ? kb : 0][j][r], acc[j][r]);
     };
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
@@ -308,7 +345,10 @@ __global__ void __launch_bounds__(KP * 2 + 32) chain_kernel(ChainArgs a) {
         }
         mma16h(part, fa[0], fb[0][j][0], fb[0][j][1]);
       }
-      if (NT > 1) join(kb);
+      if (NT > 1) {
+        undo(kb);
+        join(kb);
+      }
     }
     if (a.s && a.planes) {
       // piece q: plane q / 2 NT, row g + 8 (q / NT % 2), tile q % NT; a quad turns four of them, so that
@@ -516,9 +556,9 @@ Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V) {
   p.MC = max_chunks(N, T);
   const int VP = pad_v(V);
   // Columns of a chain: 8 while that leaves few blocks (a step is its own latency: 512 steps of 128 x
-  // 128 take 0.48 ms with 8 columns on 128 SMs, 0.64 ms with 16 on 64), up to 32 while at least two
-  // blocks per SM remain (the map is read once per block: 112 chains of 128 x 128 take 186 us with 8
-  // columns, 117 us with 16, 92 us with 32).
+  // 128 take 0.53 ms with 8 columns on 128 SMs, 0.70 ms with 16 on 64), up to 32 while at least two
+  // blocks per SM remain (the map is read once per block: 112 chains of 128 x 128 take 213 us with 8
+  // columns, 130 us with 16, 105 us with 32).
   p.vs = 8;
   while (p.vs < 32 && N * HV * (VP / (2 * p.vs)) >= 2 * kNumSMs) p.vs *= 2;
   return p;

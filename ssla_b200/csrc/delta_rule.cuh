@@ -219,8 +219,11 @@ __device__ __forceinline__ void each_pair(float (&acc)[MT][NT][4], int m0, int n
 
 // ------------------------------------------------------------------ scaled fp16 planes
 // fp32 values as hi + lo in fp16 (22 bits) need a common power of two that brings the largest near
-// 2^14: everything down to 2^-28 of it then keeps all its bits.  Bits of that scale from the largest
-// magnitude's bits (finite values only: an infinity must not shrink its neighbours), and its inverse.
+// 2^14.  Values down to 2^-16 of the largest then keep 22 bits; below, the low plane is subnormal and what
+// is lost is absolute, 2^-38 of the largest.  (hi alone: 11 bits down to 2^-28.)  So a scale is shared only
+// by values that a product adds up: a column of the state over 16 rows, 64 columns of PM.  That scale from
+// the largest magnitude's bits (finite values only: an infinity must not shrink its neighbours; below
+// the exponent they do not matter), and its inverse.
 __device__ __forceinline__ unsigned finite_bits(float x) {
   const unsigned b = __float_as_uint(x) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
@@ -230,6 +233,11 @@ __device__ __forceinline__ float plane_scale(unsigned most) {
   return __uint_as_float((e < 20u ? 247u : 267u - e) << 23);  // 2^(13 - exponent), at most 2^120
 }
 __device__ __forceinline__ float plane_unscale(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
+// plane_scale of two values at once, from the upper halves of their bits, and its inverse, as bf16 pairs
+__device__ __forceinline__ uint32_t plane_scales(uint32_t most) {
+  return __vminu2(0x85808580u - (most & 0x7f807f80u), 0x7b807b80u);
+}
+__device__ __forceinline__ uint32_t plane_unscales(uint32_t scales) { return 0x7f007f00u - scales; }
 template <int N> __device__ __forceinline__ void put_half(__half* p, size_t plane, float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   *reinterpret_cast<__half2*>(p) = h;

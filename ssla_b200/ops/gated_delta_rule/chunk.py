@@ -121,16 +121,18 @@ def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
     return o, ht, states
 
 
-def chunk_bwd(q, k, v, g, beta, cu, scale, has_h0, has_ht, states, do, dht):
+def chunk_bwd(q, k, v, g, beta, cu, scale, has_h0, has_ht, states, do, dht, want_dh0=True):
+    """Gradients from ``states`` of a forward with (``has_h0``) and into (``has_ht``) a state; ``do``,
+    ``dht``: None where nothing used that result."""
     T, H, K = q.shape
     HV, V = v.shape[1:]
     N = cu.numel() - 1
     L = _lib.load()
     dev = q.device
-    do = do.to(q.dtype).contiguous()
+    do = do.to(q.dtype).contiguous() if do is not None else torch.zeros_like(v)
     dht = dht.float().contiguous() if dht is not None else None
     dq, dk, dv, dg, dbeta = (torch.empty_like(x) for x in (q, k, v, g, beta))
-    dh0 = torch.empty((N, HV, K, V), device=dev, dtype=torch.float32) if has_h0 else None
+    dh0 = torch.empty((N, HV, K, V), device=dev, dtype=torch.float32) if has_h0 and want_dh0 else None
     wb = L.ssla_gated_delta_rule_workspace_bytes(N, T, H, HV, K, V, 1)
     ws = torch.empty(wb, device=dev, dtype=torch.uint8)
     with _lib.on_device(dev):
@@ -151,6 +153,7 @@ class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
         q, k, v, g, beta, cu, h0 = norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, "chunk_gated_delta_rule")
         o, ht, states = chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
         ctx.save_for_backward(q, k, v, g, beta, cu, states)
+        ctx.set_materialize_grads(False)
         ctx.scale = scale
         ctx.has_h0, ctx.has_ht = h0 is not None, bool(output_final_state)
         return o, ht
@@ -158,8 +161,11 @@ class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do, dht):
+        if do is None and dht is None:
+            return (None,) * 9
         q, k, v, g, beta, cu, states = ctx.saved_tensors
-        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, ctx.has_h0, ctx.has_ht, states, do, dht)
+        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, ctx.has_h0, ctx.has_ht, states, do, dht,
+                                               ctx.needs_input_grad[7])
         return dq, dk, dv, dg, dbeta, None, None, dh0, None
 
 

@@ -40,15 +40,19 @@ class FusedRecurrentGatedDeltaRuleFunction(torch.autograd.Function):
         q, k, v, g, beta, cu, h0 = norm_inputs(q, k, v, g, beta, cu_seqlens, initial_state, _NAME)
         o, ht = recurrent_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
         ctx.save_for_backward(q, k, v, g, beta, cu, h0)
+        ctx.set_materialize_grads(False)
         ctx.scale = scale
         return o, ht
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do, dht):
+        if do is None and dht is None:
+            return (None,) * 9
         q, k, v, g, beta, cu, h0 = ctx.saved_tensors
         states = chunk_fwd(q, k, v, g, beta, cu, ctx.scale, h0, False)[2]
-        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, h0 is not None, False, states, do, dht)
+        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, h0 is not None, False, states, do, dht,
+                                               ctx.needs_input_grad[7])
         return dq, dk, dv, dg, dbeta, None, None, dh0, None
 
 

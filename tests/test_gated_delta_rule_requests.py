@@ -1,0 +1,57 @@
+"""The backward computes what is asked for: no gradient of a final state that nothing used, no state
+gradient where the initial state needs none."""
+import pytest
+import torch
+
+from conftest import assert_close
+from test_gated_delta_rule import NAMES, TOL, make, operators, reference
+
+NAME = {"chunk": "ssla_b200.ops.gated_delta_rule.chunk", "recurrent": "ssla_b200.ops.gated_delta_rule.fused_recurrent"}
+
+
+def spy(monkeypatch, op):
+    """Records (dht, dh0) of every backward of ``op``."""
+    import importlib
+
+    m, seen = importlib.import_module(NAME[op]), []
+    plain = m.chunk_bwd
+
+    def recorded(*args, **kw):
+        out = plain(*args, **kw)
+        seen.append((args[11], out[5]))
+        return out
+
+    monkeypatch.setattr(m, "chunk_bwd", recorded)
+    return seen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["recurrent", "chunk"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_unused_states_are_left_out(op, dtype, monkeypatch):
+    seen = spy(monkeypatch, op)
+    x, h0, do, dht, cu = make(90, 1, 2, 32, 32, [0, 20, 90], dtype, seed=1)
+    want = reference(x, h0, do, torch.zeros_like(dht), cu)[2]
+    leaves = [y.cuda().requires_grad_() for y in x]
+    o, ht = operators()[op](*leaves, cu.cuda(), initial_state=h0.cuda(), output_final_state=True)
+    got = torch.autograd.grad(o, leaves, do.cuda())
+    for name, a, b in zip(NAMES, got, want):
+        assert_close(a, b, TOL[a.dtype], name)
+    assert seen == [(None, None)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["recurrent", "chunk"])
+@pytest.mark.parametrize("h0", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_only_the_final_state_is_used(op, h0, dtype):
+    x, h, do, dht, cu = make(90, 1, 2, 32, 32, [0, 20, 90], dtype, seed=2, h0=h0)
+    want = reference(x, h, torch.zeros_like(do), dht, cu)[2]
+    leaves = [y.cuda().requires_grad_() for y in (*x, *([h] if h0 else []))]
+    o, ht = operators()[op](*leaves[:5], cu.cuda(), initial_state=leaves[5] if h0 else None, output_final_state=True)
+    got = torch.autograd.grad(ht, leaves, dht.cuda(), allow_unused=True)
+    for name, a, b in zip(NAMES, got, want):
+        if b.any():
+            assert_close(a, b, TOL[a.dtype], name)
+        else:  # dq
+            assert a is None or not a.any(), name

@@ -50,8 +50,9 @@ class FusedRecurrentGatedDeltaRuleFunction(torch.autograd.Function):
         if do is None and dht is None:
             return (None,) * 9
         q, k, v, g, beta, cu, h0 = ctx.saved_tensors
-        states = chunk_fwd(q, k, v, g, beta, cu, ctx.scale, h0, False)[2]
-        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, h0 is not None, False, states, do, dht,
+        has_h0, has_ht = h0 is not None, dht is not None  # the states' accuracy goes by both
+        states = chunk_fwd(q, k, v, g, beta, cu, ctx.scale, h0, has_ht)[2]
+        dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, has_h0, has_ht, states, do, dht,
                                                ctx.needs_input_grad[7])
         return dq, dk, dv, dg, dbeta, None, None, dh0, None
 

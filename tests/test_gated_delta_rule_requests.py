@@ -55,3 +55,18 @@ def test_only_the_final_state_is_used(op, h0, dtype):
             assert_close(a, b, TOL[a.dtype], name)
         else:  # dq
             assert a is None or not a.any(), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("state", [False, True])
+def test_recurrent_gradients_are_the_chunked_ones(dtype, state):
+    """Same function, same kernels, same accuracy of the states: same bits."""
+    x, h0, do, dht, cu = make(300, 2, 4, 64, 64, [0, 100, 300], dtype, seed=3, h0=state, gdtype=torch.float32)
+    got = {}
+    for op, f in operators().items():
+        leaves = [y.cuda().requires_grad_() for y in (*x, *([h0] if state else []))]
+        o, ht = f(*leaves[:5], cu.cuda(), initial_state=leaves[5] if state else None, output_final_state=True)
+        got[op] = torch.autograd.grad([o, ht], leaves, [do.cuda(), dht.cuda()])
+    for name, a, b in zip(NAMES, got["recurrent"], got["chunk"]):
+        assert torch.equal(a, b), name

@@ -133,8 +133,8 @@ int ssla_chunk_gla_fwd_noalloc(const void* q, const void* k, const void* v, cons
  * h0,ht,dht,dh0 [N,HV,K,V] fp32 (nullable).  1 <= K <= 128, 1 <= V <= 256.  Tokens outside every
  * sequence get zero outputs and gradients.  g below -200 (-inf included) acts as -200: its decay
  * is 0 in fp32 either way.
- * The chunked forward fills `states` (ssla_gated_delta_rule_states_bytes) for the backward; both
- * take scratch of ssla_gated_delta_rule_workspace_bytes (backward = 0 / 1).  states and workspace
+ * The chunked forward fills `states` (ssla_gated_delta_rule_states_bytes) for the backward, with o
+ * NULL `states` and ht alone; both take scratch of ssla_gated_delta_rule_workspace_bytes (backward = 0 / 1).  states and workspace
  * are 16-byte aligned.  has_h0, has_ht: whether the forward was given h0 and ht (bf16 calls with
  * neither keep the states in 16 bits between the kernels). */
 size_t ssla_gated_delta_rule_states_bytes(int dtype, int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K,

@@ -644,7 +644,7 @@ extern "C" int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, con
   if (rc) return rc;
   if (HV == 0) return SSLA_OK;
   SSLA_CHECK_ARG(cu_seqlens && states, "%s: null pointer", name);
-  SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "%s: null pointer", name);
+  SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta), "%s: null pointer", name);
   const Plan p = make_plan(n_seqs, T, HV, K, V);
   const int KP = pad_k(K), VP = pad_v(V);
   const bool exact = exact_states(dtype, h0, ht);
@@ -671,7 +671,7 @@ extern "C" int ssla_chunk_gated_delta_rule_fwd(const void* q, const void* k, con
     if (rc) return rc;
   }
   rc = run_chain(p, sv, w, sv.s, h0, ht, n_seqs, (int)HV, (int)K, (int)V, false, exact, !f32, st);
-  if (rc || T == 0) return rc;
+  if (rc || T == 0 || !o) return rc;
   return !f32       ? output16(dtype, a, sv, KP, VP, exact, o, blocks, st)
          : KP == 64 ? output32<64>(a, sv, VP, o, blocks, st)
                     : output32<128>(a, sv, VP, o, blocks, st);

@@ -96,14 +96,15 @@ def tensor_args(q, k, v, g, beta, cu, scale):
             code[beta.dtype], cu.data_ptr(), cu.shape[0] - 1, T, H, HV, K, V, scale)
 
 
-def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
-    """(o, final state or None, states): ``states`` is what the backward needs of the chunks."""
+def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state, output=True):
+    """(o, final state or None, states): ``states`` is what the backward needs of the chunks; without
+    ``output`` o is None and not computed."""
     T, H, K = q.shape
     HV, V = v.shape[1:]
     N = cu.numel() - 1
     L = _lib.load()
     dev = q.device
-    o = torch.empty_like(v)
+    o = torch.empty_like(v) if output else None
     ht = torch.empty((N, HV, K, V), device=dev, dtype=torch.float32) if output_final_state else None
     nb = L.ssla_gated_delta_rule_states_bytes(_lib.dtype_code(q), N, T, H, HV, K, V, h0 is not None,
                                               output_final_state)
@@ -113,7 +114,7 @@ def chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
     with _lib.on_device(dev):
         _lib.check(
             L.ssla_chunk_gated_delta_rule_fwd(
-                *tensor_args(q, k, v, g, beta, cu, scale), _lib.ptr(h0), o.data_ptr(), _lib.ptr(ht),
+                *tensor_args(q, k, v, g, beta, cu, scale), _lib.ptr(h0), _lib.ptr(o), _lib.ptr(ht),
                 states.data_ptr(), nb, ws.data_ptr(), wb, _lib.raw_stream(q.device),
             ),
             "chunk_gated_delta_rule forward",

@@ -3,7 +3,9 @@
 Same arguments and results as ``chunk_gated_delta_rule``; carry ``final_state`` into the next call
 as ``initial_state``.  The forward is ``ssla_recurrent_gated_delta_rule_fwd`` (the state stays in
 registers over a sequence's tokens and crosses HBM once each way); gradients are those of the same
-function and come from the chunked kernels.
+function and come from the chunked kernels, which work on chunks of 64 tokens however few a sequence
+has: the backward's buffers hold three padded states (K to 64 or 128, V to a multiple of 64, fp32),
+one [K, K] map and a 64 x 64 tile per sequence and value head.
 """
 from __future__ import annotations
 
@@ -51,7 +53,7 @@ class FusedRecurrentGatedDeltaRuleFunction(torch.autograd.Function):
             return (None,) * 9
         q, k, v, g, beta, cu, h0 = ctx.saved_tensors
         has_h0, has_ht = h0 is not None, dht is not None  # the states' accuracy goes by both
-        states = chunk_fwd(q, k, v, g, beta, cu, ctx.scale, h0, has_ht)[2]
+        states = chunk_fwd(q, k, v, g, beta, cu, ctx.scale, h0, has_ht, output=False)[2]
         dq, dk, dv, dg, dbeta, dh0 = chunk_bwd(q, k, v, g, beta, cu, ctx.scale, has_h0, has_ht, states, do, dht,
                                                ctx.needs_input_grad[7])
         return dq, dk, dv, dg, dbeta, None, None, dh0, None
@@ -69,7 +71,8 @@ def fused_recurrent_gated_delta_rule(
     initial_state: Optional[torch.Tensor] = None,
     output_final_state: bool = False,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    r"""Recurrent gated delta rule; arguments and returns as ``chunk_gated_delta_rule``."""
+    r"""Recurrent gated delta rule; arguments and returns as ``chunk_gated_delta_rule``.  A gradient of
+    many short sequences takes many times the memory of the call itself (see above)."""
     refuse_tangents(_NAME, q, k, v, g, beta, initial_state)
     if needs_grad(q, k, v, g, beta, initial_state):
         return FusedRecurrentGatedDeltaRuleFunction.apply(q, k, v, g, beta, cu_seqlens, scale, initial_state,

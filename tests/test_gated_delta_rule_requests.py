@@ -1,5 +1,6 @@
 """The backward computes what is asked for: no gradient of a final state that nothing used, no state
-gradient where the initial state needs none."""
+gradient where the initial state needs none, and the token-by-token operator's recomputation leaves out
+the outputs."""
 import pytest
 import torch
 
@@ -70,3 +71,45 @@ def test_recurrent_gradients_are_the_chunked_ones(dtype, state):
         got[op] = torch.autograd.grad([o, ht], leaves, [do.cuda(), dht.cuda()])
     for name, a, b in zip(NAMES, got["recurrent"], got["chunk"]):
         assert torch.equal(a, b), name
+
+
+@pytest.mark.gpu
+def test_states_alone():
+    """The forward's C entry without an output buffer leaves the same states and final state."""
+    from ssla_b200.ops.gated_delta_rule import chunk
+
+    for dtype in (torch.float32, torch.bfloat16):
+        x, h0, _, _, cu = make(200, 1, 2, 64, 64, [0, 64, 200], dtype, seed=4)
+        args = [y.cuda() for y in x]
+        _, ht, states = chunk.chunk_fwd(*args, cu.cuda(), 0.125, h0.cuda(), True)
+        o, ht2, states2 = chunk.chunk_fwd(*args, cu.cuda(), 0.125, h0.cuda(), True, output=False)
+        assert o is None and torch.equal(ht, ht2)
+        assert states.numel() == states2.numel()
+        # through the backward: the buffer holds unused padding
+        do, dht = torch.ones_like(args[2]), torch.ones_like(ht)
+        a, b = (chunk.chunk_bwd(*args, cu.cuda(), 0.125, True, True, s, do, dht) for s in (states, states2))
+        for name, y, z in zip(NAMES, a, b):
+            assert torch.equal(y, z), name
+
+
+@pytest.mark.gpu
+def test_memory_of_a_recurrent_gradient():
+    """The recomputation of many one-token sequences holds the states and one workspace, no outputs."""
+    from ssla_b200 import _lib
+
+    N, HV, K = 4000, 2, 64
+    x, h0, do, dht, cu = make(N, HV, HV, K, K, list(range(N + 1)), torch.float32, seed=5)
+    leaves = [y.cuda().requires_grad_() for y in x]
+    h, cu, do, dht = h0.cuda(), cu.cuda(), do.cuda(), dht.cuda()
+    o, ht = operators()["recurrent"](*leaves, cu, initial_state=h, output_final_state=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    start = torch.cuda.memory_allocated()
+    torch.autograd.grad([o, ht], leaves, [do, dht])
+    L = _lib.load()
+    states = L.ssla_gated_delta_rule_states_bytes(0, N, N, HV, HV, K, K, 1, 1)
+    work = L.ssla_gated_delta_rule_workspace_bytes(N, N, HV, HV, K, K, 1)
+    # five gradients, the recomputed final state (freed before the backward) and the allocator's rounding
+    grads = 3 * leaves[2].numel() * 4 + 2 * leaves[3].numel() * 4
+    most = states + work + grads + (16 << 20)
+    assert torch.cuda.max_memory_allocated() - start <= most

@@ -135,8 +135,11 @@ int ssla_chunk_gla_fwd_noalloc(const void* q, const void* k, const void* v, cons
  * is 0 in fp32 either way.
  * The chunked forward fills `states` (ssla_gated_delta_rule_states_bytes) for the backward, with o
  * NULL `states` and ht alone; both take scratch of ssla_gated_delta_rule_workspace_bytes (backward = 0 / 1).  states and workspace
- * are 16-byte aligned.  has_h0, has_ht: whether the forward was given h0 and ht (bf16 calls with
- * neither keep the states in 16 bits between the kernels). */
+ * are 16-byte aligned.  has_h0, has_ht: whether the forward was given h0 and ht.
+ * Accuracy: fp32 tokens fp32 throughout.  16-bit tokens: products of 16-bit operands, start states of the
+ * chunks and their adjoints held in 16 bits between the kernels, so dg and dbeta are off by about 1e-5 also
+ * where dtype_g, dtype_beta are fp32; ht and dh0 are fp32-accurate.  bf16 calls with neither h0 nor ht carry
+ * the state in fp32 through products of 11-bit operands. */
 size_t ssla_gated_delta_rule_states_bytes(int dtype, int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K,
                                           int64_t V, int has_h0, int has_ht);
 size_t ssla_gated_delta_rule_workspace_bytes(int64_t n_seqs, int64_t T, int64_t H, int64_t HV, int64_t K, int64_t V,

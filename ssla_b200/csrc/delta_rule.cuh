@@ -39,8 +39,10 @@ struct Plan {
 };
 Plan make_plan(int64_t N, int64_t T, int64_t HV, int64_t K, int64_t V);
 
-// Whether the states leave in fp32, so that everything behind them keeps fp32 accuracy; else their
-// only readers are bf16 outputs.  (h0 given: its gradient may be asked for.)
+// Whether the state keeps fp32 accuracy along its chain (22-bit operands, behind three planes of T for 16-bit
+// tokens): for fp32 and fp16 tokens, and where a state leaves in fp32 (h0 given: its gradient may be asked
+// for).  Else the chain's operands have 11 bits.  What 16-bit tokens' kernels read of the states between the
+// chunks, and of their adjoints, has 16 bits either way.
 inline bool exact_states(int dtype, bool h0, bool ht) { return dtype != SSLA_BF16 || h0 || ht; }
 // bf16 planes of T for 16-bit tokens (delta_rule_16.cuh)
 inline int t_planes(bool exact) { return exact ? 3 : 2; }

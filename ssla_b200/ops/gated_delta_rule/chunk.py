@@ -6,6 +6,12 @@ returns for its key is subtracted.  Per value head, with state S [K, V]::
 
     S <- exp(g_t) S;   u_t = beta_t (v_t - S^T k_t);   S <- S + k_t u_t^T;   o_t = scale S^T q_t
 
+fp32 tokens are computed at fp32 accuracy.  16-bit tokens: products of 16-bit operands, which only the
+outputs' own rounding shows; final states and initial states' gradients are fp32-accurate, fp32 ``dg`` and
+``dbeta`` are off by about 1e-5.  Per 64 tokens (or shorter sequence) and value head a call holds two K x V
+matrices and a K x K one, padded to K = 64 or 128 and V a multiple of 64, in fp32; training keeps one of each
+for the backward.
+
 ``beta k^T k`` should stay below 2 (keys of unit length, beta in [0, 1] or [0, 2)): beyond that the
 recurrence itself grows without bound.  The kernels are ``ssla_chunk_gated_delta_rule_fwd`` /
 ``_bwd`` of the C ABI; the project ssla follows has no delta rule.

@@ -142,9 +142,9 @@ __global__ void __launch_bounds__(THREADS, sizeof(Prep16<TI, KP, NI>) <= 75 * 10
 
 // ------------------------------------------------------------------ output
 // 4 row groups of 16 x 2 column groups of warps, panels of 64 value columns.  X and U take the place
-// of the state's panel, so that two blocks (K = 128; three at K = 64) fit an SM: the 32768-token
-// prompt's call takes 22 us less than with panels of 32 columns.  One block of 16 warps with places
-// of their own was slower than either (340 us for this kernel against 265 us for panels of 32).
+// of the state's panel, so that two blocks (K = 128; three at K = 64) fit an SM: 224 us for the 32768-token
+// prompt of 8 heads, 22 us less than with panels of 32 columns.  One block of 16 warps with places of their
+// own was slower than either (340 us).
 template <class TI, int KP> struct Out16 {
   static constexpr int N = Planes<TI>::n, LDK = KP + 8, VB = 64, LDX = VB + 8, CG = 2, NTH = 128 * CG;
   bf k[N * BT * LDK];

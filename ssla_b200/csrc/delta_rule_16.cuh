@@ -9,8 +9,8 @@
 // transposition reads either orientation of a tile as either operand, four 8x8 blocks an
 // instruction.  Against TF32 products (11-bit operands of 4 bytes, one 32-bit load for every
 // operand register) the same tensor time carries 16 bits with half the instructions; 8 x 2048
-// tokens, 4 heads of 64: output 41 us on TF32 and 27 us now, backward 134 and 90 us.  What bounds
-// them now is the dependent chain of a chunk's products (a barrier between each, two or three
+// tokens, 4 heads of 64: output went from 41 us on TF32 to 27 us, backward from 134 to 90 us.  What
+// bounds them now is the dependent chain of a chunk's products (a barrier between each, two or three
 // blocks an SM to hide it) and, at K = 128, shared-memory bandwidth next to the tensor pipe.
 #pragma once
 #include "delta_rule.cuh"

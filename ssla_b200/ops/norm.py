@@ -1,8 +1,9 @@
 """Group norm with an activation over channels-last token features (inference and training).
 
 ``z = weight * (x - mean) / sqrt(var + eps) + bias``, ``y = act(z)``, with biased variance.  Without
-``cu_seqlens`` every token's groups are normalised for themselves (the norm over each head's values
-that closes a linear-attention mixer); with it the statistics of a group run over all tokens of a
+``cu_seqlens`` every token's groups are normalised for themselves (with a head a group: the norm over each
+head's values behind a linear-attention mixer; the activation is of the normalised values, a separate gate
+is the caller's product); with it the statistics of a group run over all tokens of a
 packed sequence (group norm of a sample's event features).  Kernels: ``ssla_group_norm_act_fwd`` /
 ``_bwd``.  The reference closes its layers with ``nn.LayerNorm`` (layers/mos_attention.py:144); it
 has no group norm.

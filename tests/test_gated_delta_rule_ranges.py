@@ -93,3 +93,23 @@ def test_no_decay_over_many_chunks(dtype):
     assert_close(ht, ht_r, TOL[torch.float32], "ht")
     o, _ = f(*args, cu.cuda())
     assert_close(o, o_r, TOL[dtype], "o without states")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("HV", HEADS)
+@pytest.mark.parametrize("size", [1e-30, 1e-20, 1e20, 1e30])
+def test_states_far_from_one(HV, size):
+    """The chain's scales follow the state over the exponents of fp32."""
+    x, h0, do, dht, cu = make(200, HV, HV, 64, 64, [0, 130, 200], torch.float32, seed=HV)
+    x, h0 = (x[0], x[1], x[2] * size, x[3], x[4]), h0 * size
+    o_r, ht_r = gated_delta_rule_ref(*x, cu, None, h0)
+    o, ht = operators()["chunk"](*[y.cuda() for y in x], cu.cuda(), initial_state=h0.cuda(), output_final_state=True)
+    # at 1e-30 the low parts of split operands (2^-22 of them) are still normal numbers
+    for name, a, b in (("o", o, o_r), ("ht", ht, ht_r)):
+        assert_close(a.double() / size, b / size, TOL[torch.float32], name)
+    do, dht = do * size, dht * size
+    leaves = [y.cuda().requires_grad_() for y in (*x[:2], x[2] / size, *x[3:])]
+    o, ht = operators()["chunk"](*leaves, cu.cuda(), output_final_state=True)
+    dv = torch.autograd.grad([o, ht], leaves[2], [do.cuda(), dht.cuda()])[0]
+    one = reference((*x[:2], x[2] / size, *x[3:]), None, do / size, dht / size, cu)[2][2]
+    assert_close(dv.double() / size, one, TOL[torch.float32], "dv")

@@ -113,3 +113,64 @@ def test_memory_of_a_recurrent_gradient():
     grads = 3 * leaves[2].numel() * 4 + 2 * leaves[3].numel() * 4
     most = states + work + grads + (16 << 20)
     assert torch.cuda.max_memory_allocated() - start <= most
+
+
+def step_of(f, x, h0, seeds, cu, use):
+    """A training step on leaves of its own: (leaves, function that runs it)."""
+    leaves = [y.cuda().requires_grad_() for y in (*x, *([h0] if h0 is not None else []))]
+    seeds, cu = [y.cuda() for y in seeds], cu.cuda()
+
+    def step():
+        out = f(*leaves[:5], cu, initial_state=leaves[5] if h0 is not None else None, output_final_state=True)
+        outs = [y for y, u in zip(out, use) if u]
+        return [y.detach() for y in out] + list(torch.autograd.grad(outs, leaves, [s for s, u in zip(seeds, use) if u],
+                                                                    allow_unused=True))
+
+    return leaves, step
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["recurrent", "chunk"])
+@pytest.mark.parametrize("use", [(True, False), (False, True), (True, True)], ids=str)
+def test_captured_steps_replayed_at_once(op, use):
+    """Two captured steps, replayed on two streams at the same time with new inputs: as eager steps."""
+    sets = [make(500, 1, 2, 64, 64, [0, 200, 500], torch.bfloat16, seed=s, h0=h0) for s, h0 in ((6, True), (7, False))]
+    graphs, outs, steps, streams = [], [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s, (x, h0, do, dht, cu) in zip(streams, sets):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            leaves, step = step_of(operators()[op], x, h0, (do, dht), cu, use)
+            step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(step())
+        graphs.append(g)
+        steps.append(step)
+        with torch.no_grad():
+            leaves[2].mul_(-0.5)  # the graph reads its inputs at replay
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for out, step in zip(outs, steps):
+        for a, b in zip(out, step()):
+            assert a is None and b is None or torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["recurrent", "chunk"])
+def test_one_graph_backward_twice(op):
+    x, h0, do, dht, cu = make(150, 2, 4, 48, 40, [0, 64, 150], torch.bfloat16, seed=8)
+    leaves = [y.cuda().requires_grad_() for y in (*x, h0)]
+    o, ht = operators()[op](*leaves[:5], cu.cuda(), initial_state=leaves[5], output_final_state=True)
+    first = torch.autograd.grad([o, ht], leaves, [do.cuda(), dht.cuda()], retain_graph=True)
+    alone = torch.autograd.grad(o, leaves, do.cuda(), retain_graph=True)
+    again = torch.autograd.grad([o, ht], leaves, [do.cuda(), dht.cuda()])
+    for a, b in zip(first, again):
+        assert torch.equal(a, b)
+    want = reference(x, h0, do, torch.zeros_like(dht), cu)[2]
+    for name, a, b in zip(NAMES, alone, want):
+        assert_close(a, b, TOL[a.dtype], name)
